@@ -1,0 +1,634 @@
+// Attention of rays' queries to a memory of another length, forward and backward.
+//
+//     s_ij = c q_i . k_j,   p = softmax_j over j < length,   o_i = sum_j p_ij v_j,   lse_i = log sum_j exp s_ij
+//     delta_i = do_i . o_i,   ds_ij = p_ij (do_i . v_j - delta_i),   dq = c ds k,   dk = c ds^T q,   dv = p^T do
+//
+// Rows: the queries of all heads that share a kv head (row = query * group + head of the group), so that a memory's tile is
+// read once for all of them, and a shared head's gradient is one sum. The forward kernel and the kernel of dq own rows and
+// stream the memory; the kernel of dk and dv owns the memory's rows and streams the queries; both form p again from the
+// saved lse. No atomics. Where the own rows are too few to fill the device (one ray that asks a long memory), the streamed
+// rows are split over workgroups and joined by a closing kernel.
+#include <type_traits>
+
+#include "tiles.inc"
+
+#include "features.h"
+
+namespace {
+
+struct AttendArgs {
+    const void *q, *k, *v;
+    int64_t qs[3], ks[3], vs[3];   // strides in values: batch, row, head
+    const int32_t *lengths;
+    int32_t queries, memory, heads, kv_heads, group, rows;   // rows = queries * group
+    int32_t d, dv;
+    int32_t q_vec, k_vec, v_vec, o_vec;
+    int32_t splits, per_split;
+    int32_t tiles;                 // of own rows, of one kv head of one batch
+    float scale, c;                // c: what brings a product of rows to a score in units of log 2, but for what own rows carry
+    float own_scale;               // 32-bit rows
+    int32_t flip;                  // 16-bit rows
+    void *out;
+    float *lse2, *delta;
+    const void *up;                // upstream gradient, contiguous like out
+    void *dq, *dk, *dvalue;        // contiguous
+    float2 *part;                  // (splits, batch * kv_heads * rows): maximum and sum
+    float *out_part, *out_part2;   // (splits, ...) sums of a split pass
+    int64_t all_rows;              // batch * kv_heads * rows
+    int64_t own_all;               // dk, dv: batch * memory * kv_heads
+};
+
+// Own blocks of 16 rows a wave (registers: own rows and sums, see the use)
+template <class TY, int NK> constexpr int forward_blocks() { return NK <= 4 ? 4 : NK <= 8 ? 2 : 1; }
+template <class TY, int NK> constexpr int dq_blocks() { return NK <= 2 ? 4 : NK <= 4 ? 2 : 1; }
+template <class TY, int NK> constexpr int dkv_blocks() { return NK <= 2 ? (TY::kSize == 2 ? 2 : 4) : NK <= 4 ? 2 : 1; }
+
+struct Place {   // which own tile, split, batch and kv head a workgroup has
+    int split, tile, batch, kv, length;
+};
+__device__ inline Place place_of(const AttendArgs &a) {
+    Place p;
+    uint32_t i = blockIdx.x;
+    p.split = i % (uint32_t)a.splits, i /= (uint32_t)a.splits;
+    p.tile = i % (uint32_t)a.tiles, i /= (uint32_t)a.tiles;
+    p.kv = i % (uint32_t)a.kv_heads, p.batch = i / (uint32_t)a.kv_heads;
+    p.length = a.lengths ? min(max(a.lengths[p.batch], 0), a.memory) : a.memory;
+    return p;
+}
+
+template <class E> __device__ inline const E *query_row(const AttendArgs &a, const Place &p, int row) {
+    if (row >= a.rows) return nullptr;
+    const int query = a.group == 1 ? row : (int)((uint32_t)row / (uint32_t)a.group), head = p.kv * a.group + row - query * a.group;
+    return reinterpret_cast<const E *>(a.q) + p.batch * a.qs[0] + query * a.qs[1] + head * a.qs[2];
+}
+// Rows of out, its gradient and dq (contiguous: batch, query, head): the offset in rows.
+__device__ inline int64_t out_row(const AttendArgs &a, const Place &p, int row) {
+    const int query = a.group == 1 ? row : (int)((uint32_t)row / (uint32_t)a.group), head = p.kv * a.group + row - query * a.group;
+    return ((int64_t)p.batch * a.queries + query) * a.heads + head;
+}
+template <class E> __device__ inline const E *memory_row(const void *base, const int64_t (&s)[3], const Place &p, int row, int last) {
+    return row < last ? reinterpret_cast<const E *>(base) + p.batch * s[0] + row * s[1] + p.kv * s[2] : nullptr;
+}
+// Row of lse, delta and the parts
+__device__ inline int64_t stat_row(const AttendArgs &a, const Place &p, int row) { return ((int64_t)p.batch * a.kv_heads + p.kv) * a.rows + row; }
+
+// What own rows carry of the scores' factor: of 32-bit rows all of it (then the scores come out in units of log 2, and a row with
+// one weight gets exactly 1: score less maximum is 0), of 16-bit rows the sign.
+template <class TY, int NK, int QB> __device__ inline void carry_scale(Own<TY, NK, QB> &own, const AttendArgs &a) {
+#pragma unroll
+    for (int q = 0; q < QB; ++q)
+#pragma unroll
+        for (int k = 0; k < NK; ++k) {
+            if constexpr (TY::kSize == 4) own.f[q][k] = __builtin_bit_cast(u4, __builtin_bit_cast(f4, own.f[q][k]) * a.own_scale);
+            else if (a.flip) own.f[q][k] ^= u4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
+        }
+}
+
+// ---- forward --------------------------------------------------------------------------------------------------------
+// The running maximum is raised (and the sums scaled) only when a value is more than 2^kSlack above it: the weights then
+// stay below 2^kSlack, which every type holds, and most tiles need no exchange between lanes.
+constexpr float kSlack = 8.0f;
+
+template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void k_attend_forward(AttendArgs a) {
+    typedef TileShape<NK> T;
+    typedef typename TY::E E;
+    constexpr int NM = T::kBytes / TY::kSize / 16;
+    __shared__ alignas(16) char tile_k[T::kRows * T::kPitch], tile_v[T::kRows * T::kPitch];
+    const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6;
+    const Place p = place_of(a);
+    const int row0 = p.tile * (kWaves * 16 * QB) + wave * 16 * QB;
+    const int first = p.split * a.per_split * T::kRows;
+    const int last = min(p.length, first + a.per_split * T::kRows);
+
+    Stage<TY, NK> stage_k, stage_v;
+    auto fetch = [&](int at) {
+        stage_k.load([&](int i) { return memory_row<E>(a.k, a.ks, p, at + i, last); }, a.d, a.k_vec);
+        stage_v.load([&](int i) { return memory_row<E>(a.v, a.vs, p, at + i, last); }, a.dv, a.v_vec);
+    };
+    if (first < last) fetch(first);
+    Own<TY, NK, QB> own;
+    own.load([&](int i) { return query_row<E>(a, p, row0 + i); }, a.d, a.q_vec);
+    carry_scale(own, a);
+    float m[QB], l[QB];
+    f4 out[QB][NM];
+#pragma unroll
+    for (int q = 0; q < QB; ++q) {
+        m[q] = -kInf, l[q] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NM; ++i) out[q][i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    for (int at = first; at < last; at += T::kRows) {
+        stage_k.store(tile_k);
+        stage_v.store(tile_v);
+        __syncthreads();
+        if (at + T::kRows < last) fetch(at + T::kRows);
+#pragma unroll
+        for (int pair = 0; pair < T::kBlocks; pair += 2) {
+            f4 s[2][QB];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                for (int q = 0; q < QB; ++q) s[j][q] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+                product<TY, NK, QB>(tile_k, pair + j, own, s[j]);
+            }
+            if (at + T::kRows > last) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (at + (pair + j) * 16 + 4 * g + r >= last)
+#pragma unroll
+                            for (int q = 0; q < QB; ++q) s[j][q][r] = -kInf;
+            }
+            float top[QB];
+            bool raise = false;
+#pragma unroll
+            for (int q = 0; q < QB; ++q) {
+                const f4 u = s[0][q], v = s[1][q];
+                top[q] = a.c * fmaxf(fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])), fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
+                raise |= top[q] > m[q] + kSlack;
+            }
+            if (__any(raise)) {
+#pragma unroll
+                for (int q = 0; q < QB; ++q) {
+                    const float to = fmaxf(m[q], max_group(top[q])), by = exp2_of(m[q] - finite_or_zero(to));
+                    m[q] = to;
+                    l[q] *= by;
+#pragma unroll
+                    for (int i = 0; i < NM; ++i) out[q][i] *= by;
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < QB; ++q) {
+                const float use = finite_or_zero(m[q]);
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[j][q][r] = exp2_of(__builtin_fmaf(s[j][q][r], a.c, -use));
+                const f4 u = s[0][q], v = s[1][q];
+                l[q] += ((u[0] + u[1]) + (u[2] + u[3])) + ((v[0] + v[1]) + (v[2] + v[3]));
+            }
+            accumulate<TY, NK, QB, NM>(tile_v, pair, s[0], s[1], out);
+        }
+        __syncthreads();
+    }
+    const bool four = (a.dv & 3) == 0;
+#pragma unroll
+    for (int q = 0; q < QB; ++q) {
+        const int row = row0 + q * 16 + (lane & 15);
+        const float sum = sum_group(l[q]);
+        if (row >= a.rows) continue;
+        const int64_t at = stat_row(a, p, row);
+        if (a.splits > 1) {
+            const int64_t part = (int64_t)p.split * a.all_rows + at;
+            if (g == 0) a.part[part] = float2{m[q], sum};
+            if (first < last)
+#pragma unroll
+                for (int i = 0; i < NM; ++i) store_four(a.out_part + part * a.dv, i * 16 + 4 * g, a.dv, out[q][i], four);
+            continue;
+        }
+        const float by = p.length > 0 ? 1.0f / sum : 0.0f;
+        if (g == 0 && a.lse2) a.lse2[at] = p.length > 0 ? m[q] + log2_of(sum) : kInf;
+        E *o = reinterpret_cast<E *>(a.out) + out_row(a, p, row) * a.dv;
+#pragma unroll
+        for (int i = 0; i < NM; ++i) store_four(o, i * 16 + 4 * g, a.dv, out[q][i] * by, four);
+    }
+}
+
+// The parts of a split forward pass: a thread for four channels of a row.
+template <class E> __global__ __launch_bounds__(kThreads) void k_attend_join(AttendArgs a, int rows_per_part) {
+    const int words = (a.dv + 3) / 4;
+    const int64_t id = (int64_t)blockIdx.x * kThreads + threadIdx.x, at = id / words;
+    const int c = (int)(id - at * words) * 4;
+    if (at >= a.all_rows) return;
+    Place p;
+    p.kv = (int)(at / a.rows % a.kv_heads), p.batch = (int)(at / a.rows / a.kv_heads);
+    const int row = (int)(at % a.rows);
+    const int length = a.lengths ? min(max(a.lengths[p.batch], 0), a.memory) : a.memory;
+    const int used = (length + rows_per_part - 1) / rows_per_part;   // (parts behind the length left no sums)
+    float m = -kInf;
+    for (int s = 0; s < used; ++s) m = fmaxf(m, a.part[(int64_t)s * a.all_rows + at].x);
+    const float use = finite_or_zero(m);
+    const bool four = (a.dv & 3) == 0;
+    float l = 0.0f;
+    f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < used; ++s) {
+        const int64_t part = (int64_t)s * a.all_rows + at;
+        const float2 ml = a.part[part];
+        const float by = exp2_of(ml.x - use);
+        l += ml.y * by;
+        const float *from = a.out_part + part * a.dv + c;
+        if (four) {
+            o += *reinterpret_cast<const f4 *>(from) * by;
+        } else {
+            for (int i = 0; i < 4; ++i)
+                if (c + i < a.dv) o[i] += from[i] * by;
+        }
+    }
+    if (c == 0 && a.lse2) a.lse2[at] = length > 0 ? m + log2_of(l) : kInf;
+    store_four(reinterpret_cast<E *>(a.out) + out_row(a, p, row) * a.dv, c, a.dv, length > 0 ? o * (1.0f / l) : o, four);
+}
+
+// ---- backward -------------------------------------------------------------------------------------------------------
+// delta of the wave's rows, from fragments: by the matrix instruction that also forms do . v, so that where a row's weight is
+// on one value alone (o = v) the two are the same number and its ds is 0, not a rounding error.
+template <class TY, int NK, int QB> __device__ inline void deltas(const Own<TY, NK, QB> &o, const Own<TY, NK, QB> &up, float (&delta)[QB]) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, l = lane & 15;
+#pragma unroll
+    for (int q = 0; q < QB; ++q) {
+        f4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < NK; ++k) s = TY::mma(o.f[q][k], up.f[q][k], s);
+        const float mine = (l & 2) ? ((l & 1) ? s[3] : s[2]) : ((l & 1) ? s[1] : s[0]);
+        delta[q] = sum_group(g == (l >> 2) ? mine : 0.0f);   // (the diagonal's one value)
+    }
+}
+
+// dq, and delta for the other kernel: queries as own rows, the memory streamed.
+template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void k_attend_dq(AttendArgs a) {
+    typedef TileShape<NK> T;
+    typedef typename TY::E E;
+    constexpr int NM = T::kBytes / TY::kSize / 16;
+    __shared__ alignas(16) char tile_k[T::kRows * T::kPitch], tile_v[T::kRows * T::kPitch];
+    const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6;
+    const Place p = place_of(a);
+    const int row0 = p.tile * (kWaves * 16 * QB) + wave * 16 * QB;
+    const int first = p.split * a.per_split * T::kRows;
+    const int last = a.dq ? min(p.length, first + a.per_split * T::kRows) : 0;
+
+    Stage<TY, NK> stage_k, stage_v;
+    auto fetch = [&](int at) {
+        stage_k.load([&](int i) { return memory_row<E>(a.k, a.ks, p, at + i, last); }, a.d, a.k_vec);
+        stage_v.load([&](int i) { return memory_row<E>(a.v, a.vs, p, at + i, last); }, a.dv, a.v_vec);
+    };
+    if (first < last) fetch(first);
+    Own<TY, NK, QB> own, up;
+    float delta[QB], lse2[QB];
+    up.load([&](int i) { return row0 + i < a.rows ? reinterpret_cast<const E *>(a.up) + out_row(a, p, row0 + i) * a.dv : nullptr; }, a.dv, a.o_vec);
+    own.load([&](int i) { return row0 + i < a.rows ? reinterpret_cast<const E *>(a.out) + out_row(a, p, row0 + i) * a.dv : nullptr; }, a.dv, a.o_vec);
+    deltas<TY, NK, QB>(own, up, delta);
+    own.load([&](int i) { return query_row<E>(a, p, row0 + i); }, a.d, a.q_vec);
+    carry_scale(own, a);
+    f4 out[QB][NM];
+#pragma unroll
+    for (int q = 0; q < QB; ++q) {
+        const int row = row0 + q * 16 + (lane & 15);
+        lse2[q] = row < a.rows ? a.lse2[stat_row(a, p, row)] : kInf;
+        if (row < a.rows && g == 0 && p.split == 0) a.delta[stat_row(a, p, row)] = delta[q];
+#pragma unroll
+        for (int i = 0; i < NM; ++i) out[q][i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    for (int at = first; at < last; at += T::kRows) {
+        stage_k.store(tile_k);
+        stage_v.store(tile_v);
+        __syncthreads();
+        if (at + T::kRows < last) fetch(at + T::kRows);
+#pragma unroll
+        for (int pair = 0; pair < T::kBlocks; pair += 2) {
+            f4 s[2][QB];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                f4 dp[QB];
+#pragma unroll
+                for (int q = 0; q < QB; ++q) s[j][q] = dp[q] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+                product<TY, NK, QB>(tile_k, pair + j, own, s[j]);
+                product<TY, NK, QB>(tile_v, pair + j, up, dp);
+#pragma unroll
+                for (int q = 0; q < QB; ++q)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        s[j][q][r] = exp2_of(__builtin_fmaf(s[j][q][r], a.c, -lse2[q])) * (dp[q][r] - delta[q]);
+            }
+            if (at + T::kRows > last) {   // rows behind the length: their products are with zeros, but not of anything
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (at + (pair + j) * 16 + 4 * g + r >= last)
+#pragma unroll
+                            for (int q = 0; q < QB; ++q) s[j][q][r] = 0.0f;
+            }
+            accumulate<TY, NK, QB, NM>(tile_k, pair, s[0], s[1], out);
+        }
+        __syncthreads();
+    }
+    if (!a.dq) return;
+    const bool four = (a.d & 3) == 0;
+#pragma unroll
+    for (int q = 0; q < QB; ++q) {
+        const int row = row0 + q * 16 + (lane & 15);
+        if (row >= a.rows) continue;
+        const int64_t to = out_row(a, p, row);
+#pragma unroll
+        for (int i = 0; i < NM; ++i) {
+            const f4 v = out[q][i] * a.scale;
+            if (a.splits > 1) store_four(a.out_part + ((int64_t)p.split * a.all_rows + to) * a.d, i * 16 + 4 * g, a.d, v, four);
+            else store_four(reinterpret_cast<E *>(a.dq) + to * a.d, i * 16 + 4 * g, a.d, v, four);
+        }
+    }
+}
+
+// dk and dv: the memory's rows as own rows, the queries streamed.
+template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void k_attend_dkv(AttendArgs a) {
+    typedef TileShape<NK> T;
+    typedef typename TY::E E;
+    constexpr int NM = T::kBytes / TY::kSize / 16;
+    __shared__ alignas(16) char tile_q[T::kRows * T::kPitch], tile_o[T::kRows * T::kPitch];
+    __shared__ alignas(16) float tile_lse2[T::kRows], tile_delta[T::kRows];
+    const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6;
+    const Place p = place_of(a);
+    const int tile0 = p.tile * (kWaves * 16 * QB), row0 = tile0 + wave * 16 * QB;
+    const int first = p.split * a.per_split * T::kRows;
+    const int last = tile0 < p.length ? min(a.rows, first + a.per_split * T::kRows) : 0;
+
+    Stage<TY, NK> stage_q, stage_o;
+    float stage_lse2 = kInf, stage_delta = 0.0f;
+    auto fetch = [&](int at) {
+        stage_q.load([&](int i) { return at + i < last ? query_row<E>(a, p, at + i) : nullptr; }, a.d, a.q_vec);
+        stage_o.load([&](int i) { return at + i < last ? reinterpret_cast<const E *>(a.up) + out_row(a, p, at + i) * a.dv : nullptr; }, a.dv, a.o_vec);
+        if ((int)threadIdx.x < T::kRows) {
+            const int row = at + threadIdx.x;
+            stage_lse2 = row < last ? a.lse2[stat_row(a, p, row)] : kInf;
+            stage_delta = row < last ? a.delta[stat_row(a, p, row)] : 0.0f;
+        }
+    };
+    if (first < last) fetch(first);
+    Own<TY, NK, QB> own_k, own_v;
+    own_k.load([&](int i) { return memory_row<E>(a.k, a.ks, p, row0 + i, p.length); }, a.d, a.k_vec);
+    own_v.load([&](int i) { return memory_row<E>(a.v, a.vs, p, row0 + i, p.length); }, a.dv, a.v_vec);
+    carry_scale(own_k, a);
+    f4 dk[QB][NM], dv[QB][NM];
+#pragma unroll
+    for (int q = 0; q < QB; ++q)
+#pragma unroll
+        for (int i = 0; i < NM; ++i) dk[q][i] = dv[q][i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int at = first; at < last; at += T::kRows) {
+        stage_q.store(tile_q);
+        stage_o.store(tile_o);
+        if ((int)threadIdx.x < T::kRows) tile_lse2[threadIdx.x] = stage_lse2, tile_delta[threadIdx.x] = stage_delta;
+        __syncthreads();
+        if (at + T::kRows < last) fetch(at + T::kRows);
+#pragma unroll
+        for (int pair = 0; pair < T::kBlocks; pair += 2) {
+            f4 s[2][QB], dp[2][QB];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                for (int q = 0; q < QB; ++q) s[j][q] = dp[j][q] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+                product<TY, NK, QB>(tile_q, pair + j, own_k, s[j]);
+                product<TY, NK, QB>(tile_o, pair + j, own_v, dp[j]);
+                const int at4 = (pair + j) * 16 + 4 * g;
+                const f4 lse2 = *reinterpret_cast<const f4 *>(tile_lse2 + at4), delta = *reinterpret_cast<const f4 *>(tile_delta + at4);
+#pragma unroll
+                for (int q = 0; q < QB; ++q)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float e = exp2_of(__builtin_fmaf(s[j][q][r], a.c, -lse2[r]));
+                        s[j][q][r] = e;
+                        dp[j][q][r] = e * (dp[j][q][r] - delta[r]);
+                    }
+            }
+            accumulate<TY, NK, QB, NM>(tile_o, pair, s[0], s[1], dv);
+            accumulate<TY, NK, QB, NM>(tile_q, pair, dp[0], dp[1], dk);
+        }
+        __syncthreads();
+    }
+    const bool four_k = (a.d & 3) == 0, four_v = (a.dv & 3) == 0;
+    const f4 none = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int q = 0; q < QB; ++q) {
+        const int row = row0 + q * 16 + (lane & 15);
+        if (row >= a.memory) continue;
+        const int64_t to = ((int64_t)p.batch * a.memory + row) * a.kv_heads + p.kv;
+        const bool there = row < p.length;   // (a row behind the length has products of zeros with anything)
+        const int64_t part = (int64_t)p.split * a.own_all + to;
+#pragma unroll
+        for (int i = 0; i < NM; ++i) {
+            const f4 k = there ? dk[q][i] * a.scale : none, v = there ? dv[q][i] : none;
+            if (a.splits > 1) {
+                store_four(a.out_part + part * a.d, i * 16 + 4 * g, a.d, k, four_k);
+                store_four(a.out_part2 + part * a.dv, i * 16 + 4 * g, a.dv, v, four_v);
+            } else {
+                if (a.dk) store_four(reinterpret_cast<E *>(a.dk) + to * a.d, i * 16 + 4 * g, a.d, k, four_k);
+                if (a.dvalue) store_four(reinterpret_cast<E *>(a.dvalue) + to * a.dv, i * 16 + 4 * g, a.dv, v, four_v);
+            }
+        }
+    }
+}
+
+}  // namespace
+
+// ---- host -----------------------------------------------------------------------------------------------------------
+namespace {
+
+int check(const DstAttendParams *p) {
+    if (!p) return dst_op_fail(DST_E_INVALID, "params is null");
+    if (p->dtype != DST_DTYPE_F32 && p->dtype != DST_DTYPE_BF16 && p->dtype != DST_DTYPE_F16)
+        return dst_op_fail(DST_E_UNSUPPORTED, "dtype must be float32, bfloat16 or float16");
+    if (p->batch < 0 || p->queries < 0 || p->memory < 0) return dst_op_fail(DST_E_INVALID, "negative size");
+    if (p->heads < 1 || p->kv_heads < 1 || p->heads % p->kv_heads != 0)
+        return dst_op_fail(DST_E_INVALID, "heads must be a multiple of kv_heads");
+    if (p->channels < 1 || p->channels > DST_MAX_CHANNELS || p->value_channels < 1 || p->value_channels > DST_MAX_CHANNELS)
+        return dst_op_fail(DST_E_UNSUPPORTED, "channels must be in 1..%d", DST_MAX_CHANNELS);
+    if (!(p->scale == p->scale) || p->scale - p->scale != 0.0f) return dst_op_fail(DST_E_INVALID, "scale must be finite");
+    const int64_t rows = (int64_t)p->queries * (p->heads / p->kv_heads), most = 0x3fffffff;
+    if (rows > most || p->memory > most || (int64_t)p->batch * p->kv_heads > most ||
+        (int64_t)p->batch * p->kv_heads * (div_up(rows, 16) > div_up(p->memory, 16) ? div_up(rows, 16) : div_up(p->memory, 16)) > most)
+        return dst_op_fail(DST_E_UNSUPPORTED, "too many rows");
+    const bool any = p->batch > 0 && p->queries > 0;
+    if (any && (!p->q || !p->out || (p->memory > 0 && (!p->k || !p->v)))) return dst_op_fail(DST_E_INVALID, "q, k, v and out are required");
+    return DST_OK;
+}
+
+bool strides_align(const void *p, const int64_t (&s)[3], int channels, int size) {
+    return words_align(p, s[0], channels, size) && words_align(p, s[1], channels, size) && words_align(p, s[2], channels, size);
+}
+
+AttendArgs arguments(const DstAttendParams *p) {
+    AttendArgs a = {};
+    const int size = value_size(p->dtype);
+    a.q = p->q, a.k = p->k, a.v = p->v;
+    for (int i = 0; i < 3; ++i) a.qs[i] = p->q_strides[i], a.ks[i] = p->k_strides[i], a.vs[i] = p->v_strides[i];
+    a.lengths = p->lengths;
+    a.queries = p->queries, a.memory = p->memory, a.heads = p->heads, a.kv_heads = p->kv_heads;
+    a.group = p->heads / p->kv_heads, a.rows = p->queries * a.group;
+    a.d = p->channels, a.dv = p->value_channels;
+    a.q_vec = strides_align(p->q, p->q_strides, p->channels, size);
+    a.k_vec = strides_align(p->k, p->k_strides, p->channels, size);
+    a.v_vec = strides_align(p->v, p->v_strides, p->value_channels, size);
+    a.o_vec = words_align(p->out, 0, p->value_channels, size) && words_align(p->upstream, 0, p->value_channels, size);
+    a.scale = p->scale, a.flip = p->scale < 0.0f;
+    // (a scale of 0 stands for all scores equal: the smallest normal number says that of any score that is finite, and leaves
+    // -inf what it is)
+    a.c = __builtin_fabsf(p->scale) * kLog2E;
+    if (a.c < 1.1754944e-38f) a.c = 1.1754944e-38f;
+    if (p->dtype == DST_DTYPE_F32) a.own_scale = a.flip ? -a.c : a.c, a.c = 1.0f;
+    a.out = p->out, a.lse2 = p->lse;
+    a.splits = a.per_split = 1;
+    a.all_rows = (int64_t)p->batch * p->kv_heads * a.rows;
+    return a;
+}
+
+template <class TY, class F> int with_fragments(int nk, F f) {
+    switch (nk) {
+        case 1: return f(TY{}, std::integral_constant<int, 1>{});
+        case 2: return f(TY{}, std::integral_constant<int, 2>{});
+        case 4: return f(TY{}, std::integral_constant<int, 4>{});
+        case 8: return f(TY{}, std::integral_constant<int, 8>{});
+        default:
+            if constexpr (TY::kSize == 4) return f(TY{}, std::integral_constant<int, 16>{});
+            return dst_op_fail(DST_E_UNSUPPORTED, "channels must be in 1..%d", DST_MAX_CHANNELS);
+    }
+}
+int fragments(const DstAttendParams *p) {
+    return fragments_of(p->channels > p->value_channels ? p->channels : p->value_channels, p->dtype);
+}
+template <class F> int with_type(const DstAttendParams *p, F f) {
+    if (p->dtype == DST_DTYPE_F32) return with_fragments<F32>(fragments(p), f);
+    return p->dtype == DST_DTYPE_BF16 ? with_fragments<BF16>(fragments(p), f) : with_fragments<F16>(fragments(p), f);
+}
+
+// Few rows (one query and its heads): a wave with one block of them leaves the others nothing but to load.
+template <class TY, int NK> int forward_rows(const AttendArgs &a) { return kWaves * 16 * (a.rows <= kWaves * 16 ? 1 : forward_blocks<TY, NK>()); }
+
+uint64_t plan_forward(AttendArgs &a, int own, int tile, int64_t heads, char *base) {
+    a.tiles = (int)div_up(a.rows, own);
+    const Split s = split_tiles(a.tiles * heads, div_up(a.memory, tile));
+    a.splits = s.splits, a.per_split = s.per_split;
+    Carve c = {base, 0};
+    if (a.splits > 1) {
+        a.part = c.take<float2>((uint64_t)a.splits * a.all_rows);
+        a.out_part = c.take<float>((uint64_t)a.splits * a.all_rows * a.dv);
+    }
+    return c.used;
+}
+uint64_t plan_dq(AttendArgs &a, int own, int tile, int64_t heads, char *base) {
+    a.tiles = (int)div_up(a.rows, own);
+    const Split s = a.dq ? split_tiles(a.tiles * heads, div_up(a.memory, tile)) : Split{1, 1};
+    a.splits = s.splits, a.per_split = s.per_split;
+    Carve c = {base, 0};
+    a.delta = c.take<float>(a.all_rows);
+    if (a.splits > 1) a.out_part = c.take<float>((uint64_t)a.splits * a.all_rows * a.d);
+    return c.used;
+}
+uint64_t plan_dkv(AttendArgs &a, int own, int tile, int64_t heads, char *base) {
+    a.tiles = (int)div_up(a.memory, own);
+    const Split s = split_tiles(a.tiles * heads, div_up(a.rows, tile));
+    a.splits = s.splits, a.per_split = s.per_split;
+    Carve c = {base, 0};
+    a.delta = c.take<float>(a.all_rows);
+    if (a.splits > 1) {
+        const uint64_t rows = (uint64_t)a.splits * heads * a.memory;
+        a.out_part = c.take<float>(rows * a.d);
+        a.out_part2 = c.take<float>(rows * a.dv);
+    }
+    return c.used;
+}
+
+int check_workspace(const DstAttendParams *p, uint64_t need) {
+    if (need == 0) return DST_OK;
+    if (!p->workspace || p->workspace_bytes < need)
+        return dst_op_fail(DST_E_INVALID, "workspace of %llu bytes is needed", (unsigned long long)need);
+    if (reinterpret_cast<uintptr_t>(p->workspace) & 255u) return dst_op_fail(DST_E_INVALID, "workspace must be aligned to 256 bytes");
+    return DST_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+uint64_t dst_attend_workspace_bytes(const DstAttendParams *p, int pass) {
+    if (check(p) != DST_OK) return 0;
+    uint64_t bytes = 0;
+    with_type(p, [&](auto ty, auto nk) {
+        typedef decltype(ty) TY;
+        constexpr int NK = decltype(nk)::value;
+        AttendArgs a = arguments(p);
+        const int64_t heads = (int64_t)p->batch * p->kv_heads;
+        if (a.all_rows == 0 && pass == DST_PASS_FORWARD) return DST_OK;
+        if (pass == DST_PASS_FORWARD) {
+            bytes = plan_forward(a, forward_rows<TY, NK>(a), TileShape<NK>::kRows, heads, nullptr);
+        } else {
+            a.dq = p->grad_q;
+            bytes = plan_dq(a, kWaves * 16 * dq_blocks<TY, NK>(), TileShape<NK>::kRows, heads, nullptr);
+            if (p->grad_k || p->grad_v) {
+                const uint64_t more = plan_dkv(a, kWaves * 16 * dkv_blocks<TY, NK>(), TileShape<NK>::kRows, heads, nullptr);
+                bytes = more > bytes ? more : bytes;
+            }
+        }
+        return DST_OK;
+    });
+    return bytes;
+}
+
+int dst_attend_forward(const DstAttendParams *p, void *stream) {
+    if (int rc = check(p)) return rc;
+    return with_type(p, [&](auto ty, auto nk) {
+        typedef decltype(ty) TY;
+        typedef typename TY::E E;
+        constexpr int NK = decltype(nk)::value, QB = forward_blocks<TY, NK>();
+        AttendArgs a = arguments(p);
+        if (a.all_rows == 0) return (int)DST_OK;
+        const int64_t heads = (int64_t)p->batch * p->kv_heads;
+        const uint64_t need = plan_forward(a, forward_rows<TY, NK>(a), TileShape<NK>::kRows, heads, (char *)p->workspace);
+        if (int rc = check_workspace(p, need)) return rc;
+        const hipStream_t s = (hipStream_t)stream;
+        const dim3 grid((uint32_t)(a.tiles * heads * a.splits));
+        if (a.rows <= kWaves * 16) k_attend_forward<TY, NK, 1><<<grid, kThreads, 0, s>>>(a);
+        else k_attend_forward<TY, NK, QB><<<grid, kThreads, 0, s>>>(a);
+        DST_OP_LAUNCH("attention");
+        if (a.splits > 1) {
+            const int64_t words = a.all_rows * ((a.dv + 3) / 4);
+            k_attend_join<E><<<dim3((uint32_t)div_up(words, kThreads)), kThreads, 0, s>>>(a, a.per_split * TileShape<NK>::kRows);
+            DST_OP_LAUNCH("attention, joining");
+        }
+        return (int)DST_OK;
+    });
+}
+
+int dst_attend_backward(const DstAttendParams *p, void *stream) {
+    if (int rc = check(p)) return rc;
+    if (p->dtype == DST_DTYPE_F16) return dst_op_fail(DST_E_UNSUPPORTED, "gradients are of float32 and bfloat16 rows");
+    if (!p->grad_q && !p->grad_k && !p->grad_v) return DST_OK;
+    if (p->batch > 0 && p->queries > 0 && (!p->lse || !p->upstream)) return dst_op_fail(DST_E_INVALID, "lse and upstream are required");
+    if ((reinterpret_cast<uintptr_t>(p->grad_q) | reinterpret_cast<uintptr_t>(p->grad_k) | reinterpret_cast<uintptr_t>(p->grad_v)) & 15u)
+        return dst_op_fail(DST_E_INVALID, "gradients must be aligned to 16 bytes");
+    auto launch = [&](auto ty, auto nk) {
+        typedef decltype(ty) TY;
+        typedef typename TY::E E;
+        constexpr int NK = decltype(nk)::value;
+        constexpr int tile = TileShape<NK>::kRows, dq_rows = kWaves * 16 * dq_blocks<TY, NK>(), dkv_rows = kWaves * 16 * dkv_blocks<TY, NK>();
+        const hipStream_t s = (hipStream_t)stream;
+        const int64_t heads = (int64_t)p->batch * p->kv_heads;
+        AttendArgs a = arguments(p);
+        a.up = p->upstream, a.dq = p->grad_q, a.dk = p->grad_k, a.dvalue = p->grad_v;
+        if (a.all_rows > 0) {
+            const uint64_t need = plan_dq(a, dq_rows, tile, heads, (char *)p->workspace);
+            if (int rc = check_workspace(p, need)) return rc;
+            k_attend_dq<TY, NK, dq_blocks<TY, NK>()><<<dim3((uint32_t)(a.tiles * heads * a.splits)), kThreads, 0, s>>>(a);
+            DST_OP_LAUNCH("attention gradient, queries");
+            if (a.splits > 1) {
+                const int64_t n = a.all_rows * a.d;
+                k_sum_parts<E><<<dim3(sum_blocks(n)), 256, 0, s>>>(a.out_part, (E *)a.dq, n, a.splits);
+                DST_OP_LAUNCH("attention gradient, summing");
+            }
+        }
+        if ((a.dk || a.dvalue) && heads * a.memory > 0) {
+            const uint64_t need = plan_dkv(a, dkv_rows, tile, heads, (char *)p->workspace);
+            if (int rc = check_workspace(p, need)) return rc;
+            a.own_all = heads * a.memory;
+            k_attend_dkv<TY, NK, dkv_blocks<TY, NK>()><<<dim3((uint32_t)(a.tiles * heads * a.splits)), kThreads, 0, s>>>(a);
+            DST_OP_LAUNCH("attention gradient, memory");
+            if (a.splits > 1) {
+                const int64_t nk_ = a.own_all * a.d, nv = a.own_all * a.dv;
+                if (a.dk) k_sum_parts<E><<<dim3(sum_blocks(nk_)), 256, 0, s>>>(a.out_part, (E *)a.dk, nk_, a.splits);
+                if (a.dvalue) k_sum_parts<E><<<dim3(sum_blocks(nv)), 256, 0, s>>>(a.out_part2, (E *)a.dvalue, nv, a.splits);
+                DST_OP_LAUNCH("attention gradient, summing");
+            }
+        }
+        return (int)DST_OK;
+    };
+    return p->dtype == DST_DTYPE_F32 ? with_fragments<F32>(fragments(p), launch) : with_fragments<BF16>(fragments(p), launch);
+}
+
+}  // extern "C"

@@ -1,7 +1,10 @@
 // C ABI of libdst.so: context management, argument validation, launches.
 // Replaces the pybind module and host launcher of the reference (ext.cpp, trace_surfels.cpp).
 #include "dst_internal.h"
+#include "features.h"
 
+#include <cstdarg>
+#include <cstdio>
 #include <cstdlib>
 #include <cstring>
 #include <new>
@@ -48,9 +51,23 @@ int check_common(dst_ctx *ctx, const DstParams *p) {
     return DST_OK;
 }
 
+thread_local char op_error[256] = "";
+
 }  // namespace
 
+int dst_op_fail(int code, const char *format, ...) {
+    va_list args;
+    va_start(args, format);
+    std::vsnprintf(op_error, sizeof(op_error), format, args);
+    va_end(args);
+    return code;
+}
+
 extern "C" {
+
+const char *dst_op_error(void) { return op_error; }
+size_t dst_sizeof_label_params(void) { return sizeof(DstLabelParams); }
+size_t dst_sizeof_attend_params(void) { return sizeof(DstAttendParams); }
 
 const char *dst_version(void) { return "dst-mi355x 0.1"; }
 size_t dst_sizeof_params(void) { return sizeof(DstParams); }

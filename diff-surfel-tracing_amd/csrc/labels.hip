@@ -1,0 +1,789 @@
+// Labels of rays: softmax cross entropy of a ray's channels against a table of labels, its gradients, and the best label.
+//
+//     s_rv = x_r . w_v + b_v,   lse_r = log sum_v exp s_rv,   loss_r = lse_r - s_{r,t_r}
+//     ds_rv = g_r (exp(s_rv - lse_r) - [v = t_r]),   dx = ds w,   dw = ds^T x,   db = sum_r ds
+//
+// The (rays, labels) matrix is never stored: the forward kernel goes over the table in tiles and keeps a running maximum
+// and sum for every ray; each of the two backward kernels forms the tiles again from the saved lse, one with the rays
+// as own rows (dx), one with the labels (dw, db). Every sum has one owner and one order: no atomics, the same bits every
+// time. Where the own rows are too few to fill the device, the streamed rows are split over workgroups, and a closing kernel
+// adds the parts.
+#include <type_traits>
+
+#include "tiles.inc"
+
+#include "features.h"
+
+namespace {
+
+// ---- launch parameters as the kernels take them -------------------------------------------------------------------
+struct LabelArgs {
+    const void *x, *w;
+    const float *bias;              // (labels) or nullptr
+    const int64_t *target;          // (rays)
+    int64_t x_pitch, w_pitch;       // values from one row to the next
+    int64_t rays, ignore;
+    int32_t d, labels;
+    int32_t x_vec, w_vec;           // rows can be read in 16-byte words
+    int32_t splits, per_split;      // parts of the streamed rows; tiles of each
+    // forward
+    float2 *part;                   // (splits, rays): maximum and sum, in units of log 2
+    float *target_logit;            // (rays): forward with splits
+    float *lse2;                    // (rays): log2 of the sum of exponentials; +inf where the ray is ignored
+    float *rows;                    // (rays) losses, or nullptr
+    double *sums;                   // (blocks): sums of losses ...
+    uint32_t *counts;               // ... and rays counted in them
+    // the best label
+    const float *bounds;            // (kBoundBlocks, 2): largest row norm of the table, largest |bias|
+    int4 *best;                     // (splits, rays): bits of the best logit, its label, bits of the second best, -
+    int64_t *label;                 // (rays)
+    float *log_prob;                // (rays)
+    uint32_t *near_count;           // rays whose two best labels 32 bits cannot tell apart ...
+    uint32_t *near_list;            // ... and which
+    // backward
+    const float *upstream;          // (rays) or one value
+    const float *inverse;           // one value that multiplies a single upstream value, or nullptr
+    int32_t upstream_rows;
+    void *out;                      // (rays, d) or (labels, d), of the inputs' type
+    float *out_part;                // (splits, rows, d) if splits > 1
+    float *bias_out, *bias_part;    // (labels); (splits, labels)
+};
+
+constexpr int kBoundBlocks = 64;
+
+// Own blocks of 16 rows of a wave: as many as the registers hold with a wave or two on a SIMD: the more, the fewer times a
+// streamed tile is read from LDS.
+template <class TY, int NK> constexpr int forward_blocks() { return NK <= 4 ? 4 : NK <= 8 ? 2 : 1; }
+template <class TY, int NK> constexpr int backward_blocks() {
+    return NK * (TY::kSize == 2 ? 12 : 8) <= 32 ? 4 : NK * (TY::kSize == 2 ? 12 : 8) <= 96 ? 2 : 1;
+}
+
+template <class TY, int NK> __device__ inline const typename TY::E *row_of(const void *base, int64_t row, int64_t rows, int64_t pitch) {
+    return row < rows ? reinterpret_cast<const typename TY::E *>(base) + row * pitch : nullptr;
+}
+
+// The upstream gradient of a ray's loss: 0 where it is ignored, NaN where its label is none.
+__device__ inline float upstream_of(const LabelArgs &a, int64_t row, int64_t t) {
+    if (t == a.ignore) return 0.0f;
+    if (t < 0 || t >= a.labels) return __builtin_nanf("");
+    const float u = a.upstream[a.upstream_rows ? row : 0];
+    return a.inverse ? u * a.inverse[0] : u;
+}
+
+// ---- forward --------------------------------------------------------------------------------------------------------
+// A ray's loss from its maximum and sum; adds it to the thread's sums.
+__device__ inline void finish_row(const LabelArgs &a, int64_t row, Running r, float target_logit, double &sum, uint32_t &count) {
+    const int64_t t = a.target[row];
+    const bool ignored = t == a.ignore;
+    const float lse2 = r.m + log2_of(r.l);
+    float loss = lse2 * kLn2 - target_logit;
+    if (t < 0 || t >= a.labels) loss = __builtin_nanf("");
+    if (ignored) loss = 0.0f;
+    a.lse2[row] = ignored ? kInf : lse2;
+    if (a.rows) a.rows[row] = loss;
+    sum += (double)loss;
+    count += ignored ? 0u : 1u;
+}
+
+// The workgroup's sum of losses and count of rays, in an order of its own.
+__device__ inline void block_sums(const LabelArgs &a, double sum, uint32_t count, char *lds) {
+    if (!a.sums) return;
+    double *s = reinterpret_cast<double *>(lds);
+    uint32_t *c = reinterpret_cast<uint32_t *>(lds + sizeof(double) * kThreads);
+    __syncthreads();
+    s[threadIdx.x] = sum, c[threadIdx.x] = count;
+    for (int step = kThreads / 2; step > 0; step >>= 1) {
+        __syncthreads();
+        if ((int)threadIdx.x < step) s[threadIdx.x] += s[threadIdx.x + step], c[threadIdx.x] += c[threadIdx.x + step];
+    }
+    if (threadIdx.x == 0) a.sums[blockIdx.x] = s[0], a.counts[blockIdx.x] = c[0];
+}
+
+// The best label of a ray, or a place on the list of those that 32 bits cannot decide: a logit of d products is off by less
+// than (d + 16) 2^-22 times the norms (the tile product rounds at most once a product and once a block), twice that between
+// two; a ray without channels has none.
+__device__ inline void finish_best(const LabelArgs &a, int64_t row, Running r, float best, int label, float second, float norm) {
+    float wide = 0.0f, tall = 0.0f;
+    for (int i = 0; i < kBoundBlocks; ++i) wide = fmaxf(wide, a.bounds[2 * i]), tall = fmaxf(tall, a.bounds[2 * i + 1]);
+    const float off = norm > 0.0f ? 2.3841858e-7f * ((float)(a.d + 16) * norm * wide + 2.0f * tall) : 0.0f;
+    a.label[row] = label == 0x7fffffff ? 0 : label;
+    a.log_prob[row] = -log2_of(r.l) * kLn2;
+    if (best - second < 2.0f * off) a.near_list[atomicAdd(a.near_count, 1u)] = (uint32_t)row;
+}
+
+// (best, label) of two lanes or parts: the larger, the lower label where they are equal; `second`: the largest of the others.
+__device__ inline void merge_best(float &best, int &label, float &second, float b, int l, float s) {
+    const bool theirs = b > best || (b == best && l < label);
+    second = fmaxf(fmaxf(second, s), theirs ? best : b);
+    best = theirs ? b : best;
+    label = theirs ? l : label;
+}
+
+template <class TY> __device__ inline float dot_word(u4 a, u4 b) {
+    typename TY::E x[16 / TY::kSize], y[16 / TY::kSize];
+    __builtin_memcpy(x, &a, 16), __builtin_memcpy(y, &b, 16);
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16 / TY::kSize; ++i) s = __builtin_fmaf((float)x[i], (float)y[i], s);
+    return s;
+}
+
+// Rays as own rows, the table streamed. BEST: the best label instead of the loss.
+template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThreads) void k_label_forward(LabelArgs a) {
+    typedef TileShape<NK> T;
+    __shared__ alignas(16) char tile[T::kRows * T::kPitch > kThreads * 12 ? T::kRows * T::kPitch : kThreads * 12];
+    __shared__ alignas(16) float tile_bias[T::kRows];
+    const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6;
+    const int split = blockIdx.x % a.splits;
+    const int64_t row0 = (int64_t)(blockIdx.x / a.splits) * (kWaves * 16 * QB) + wave * 16 * QB;
+    const int first = split * a.per_split * T::kRows;
+    const int last = min(a.labels, (split + 1) * a.per_split * T::kRows);   // (the host keeps labels + a tile below 2^31)
+
+    Stage<TY, NK> stage;
+    float stage_bias = 0.0f;
+    auto fetch = [&](int at) {
+        stage.load([&](int i) { return row_of<TY, NK>(a.w, at + i, last, a.w_pitch); }, a.d, a.w_vec);
+        if ((int)threadIdx.x < T::kRows && a.bias) stage_bias = at + (int)threadIdx.x < last ? a.bias[at + threadIdx.x] : 0.0f;
+    };
+    fetch(first);
+    Own<TY, NK, QB> own;
+    own.load([&](int i) { return row_of<TY, NK>(a.x, row0 + i, a.rays, a.x_pitch); }, a.d, a.x_vec);
+
+    Running run[QB];
+    float best[QB], second[QB];
+    int label[QB];
+#pragma unroll
+    for (int q = 0; q < QB; ++q) run[q] = Running{-kInf, 0.0f}, best[q] = second[q] = -kInf, label[q] = 0x7fffffff;
+
+    for (int at = first; at < last; at += T::kRows) {
+        stage.store(tile);
+        if ((int)threadIdx.x < T::kRows) tile_bias[threadIdx.x] = stage_bias;
+        __syncthreads();
+        if (at + T::kRows < last) fetch(at + T::kRows);
+#pragma unroll
+        for (int pair = 0; pair < T::kBlocks; pair += 2) {
+            f4 s[2][QB];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const f4 b = *reinterpret_cast<const f4 *>(tile_bias + (pair + j) * 16 + 4 * g);
+#pragma unroll
+                for (int q = 0; q < QB; ++q) s[j][q] = b;
+                product<TY, NK, QB>(tile, pair + j, own, s[j]);
+            }
+            if (at + T::kRows > last) {   // rows behind the table's end
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (at + (pair + j) * 16 + 4 * g + r >= last)
+#pragma unroll
+                            for (int q = 0; q < QB; ++q) s[j][q][r] = -kInf;
+            }
+#pragma unroll
+            for (int q = 0; q < QB; ++q) {
+                float top;
+                if constexpr (BEST) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const float v = s[j][q][r];
+                            second[q] = __builtin_amdgcn_fmed3f(v, best[q], second[q]);
+                            label[q] = v > best[q] ? at + (pair + j) * 16 + 4 * g + r : label[q];
+                            best[q] = fmaxf(best[q], v);
+                        }
+                    top = best[q] * kLog2E;
+                } else {
+                    const f4 u = s[0][q], v = s[1][q];
+                    top = fmaxf(fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])), fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]))) * kLog2E;
+                    top = fmaxf(top, run[q].m);
+                }
+                // (eight at a time, added in pairs: the running sum sees an eighth of the additions)
+                const float use = finite_or_zero(top);
+                f4 e[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) e[j][r] = exp2_of(__builtin_fmaf(s[j][q][r], kLog2E, -use));
+                const float sum = ((e[0][0] + e[0][1]) + (e[0][2] + e[0][3])) + ((e[1][0] + e[1][1]) + (e[1][2] + e[1][3]));
+                run[q].l = run[q].l * exp2_of(run[q].m - use) + sum;
+                run[q].m = top;
+            }
+        }
+        __syncthreads();
+    }
+
+    double sum = 0.0;
+    uint32_t count = 0;
+#pragma unroll
+    for (int q = 0; q < QB; ++q) {
+        const int64_t row = row0 + q * 16 + (lane & 15);
+        const Running r = merge_group(run[q]);
+        if constexpr (BEST) {
+            float norm = 0.0f;
+#pragma unroll
+            for (int k = 0; k < NK; ++k) norm += dot_word<TY>(own.f[q][k], own.f[q][k]);
+            norm = sqrtf(sum_group(norm));
+#pragma unroll
+            for (int step = 16; step <= 32; step <<= 1)
+                merge_best(best[q], label[q], second[q], __shfl_xor(best[q], step), __shfl_xor(label[q], step), __shfl_xor(second[q], step));
+            if (row < a.rays && g == 0) {
+                if (a.splits > 1) {
+                    a.part[(int64_t)split * a.rays + row] = float2{r.m, r.l};
+                    a.best[(int64_t)split * a.rays + row] = int4{__builtin_bit_cast(int, best[q]), label[q], __builtin_bit_cast(int, second[q]),
+                                                                 __builtin_bit_cast(int, norm)};
+                } else {
+                    finish_best(a, row, r, best[q], label[q], second[q], norm);
+                }
+            }
+        } else {
+            // the target's logit, from the own row in registers
+            float logit = 0.0f;
+            if (split == 0) {
+                const int64_t t = row < a.rays ? a.target[row] : -1;
+                const bool there = t >= 0 && t < a.labels;
+#pragma unroll
+                for (int k = 0; k < NK; ++k)
+                    if (there) logit += dot_word<TY>(own.f[q][k], load_word<TY>(row_of<TY, NK>(a.w, t, a.labels, a.w_pitch), k * 4 + g, a.d, a.w_vec));
+                logit = sum_group(logit);
+                if (there && a.bias) logit += a.bias[t];
+            }
+            if (row < a.rays && g == 0) {
+                if (a.splits > 1) {
+                    a.part[(int64_t)split * a.rays + row] = float2{r.m, r.l};
+                    if (split == 0) a.target_logit[row] = logit;
+                } else {
+                    finish_row(a, row, r, logit, sum, count);
+                }
+            }
+        }
+    }
+    if constexpr (!BEST)
+        if (a.splits == 1) block_sums(a, sum, count, tile);
+}
+
+// The parts of a split forward pass, a thread a ray.
+template <bool BEST> __global__ __launch_bounds__(kThreads) void k_label_join(LabelArgs a) {
+    __shared__ alignas(16) char lds[kThreads * 12];
+    const int64_t row = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    double sum = 0.0;
+    uint32_t count = 0;
+    if (row < a.rays) {
+        Running r = {-kInf, 0.0f};
+        float best = -kInf, second = -kInf, norm = 0.0f;
+        int label = 0x7fffffff;
+        for (int s = 0; s < a.splits; ++s) {
+            const float2 p = a.part[(int64_t)s * a.rays + row];
+            r = merge(r, Running{p.x, p.y});
+            if constexpr (BEST) {
+                const int4 b = a.best[(int64_t)s * a.rays + row];
+                merge_best(best, label, second, __builtin_bit_cast(float, b.x), b.y, __builtin_bit_cast(float, b.z));
+                norm = __builtin_bit_cast(float, b.w);
+            }
+        }
+        if constexpr (BEST) finish_best(a, row, r, best, label, second, norm);
+        else finish_row(a, row, r, a.target_logit[row], sum, count);
+    }
+    if constexpr (!BEST) block_sums(a, sum, count, lds);
+}
+
+// The sum of the blocks' losses, or their mean over the rays counted (none counted: 0 / 0), and what an upstream gradient
+// of it is multiplied by for one ray.
+__global__ __launch_bounds__(kThreads) void k_label_mean(const double *sums, const uint32_t *counts, uint32_t blocks, int mean, float *loss, float *inverse) {
+    __shared__ double s[kThreads];
+    __shared__ unsigned long long c[kThreads];
+    double sum = 0.0;
+    unsigned long long count = 0;
+    for (uint32_t i = threadIdx.x; i < blocks; i += kThreads) sum += sums[i], count += counts[i];
+    s[threadIdx.x] = sum, c[threadIdx.x] = count;
+    for (int step = kThreads / 2; step > 0; step >>= 1) {
+        __syncthreads();
+        if ((int)threadIdx.x < step) s[threadIdx.x] += s[threadIdx.x + step], c[threadIdx.x] += c[threadIdx.x + step];
+    }
+    if (threadIdx.x == 0) {
+        *loss = (float)(mean ? s[0] / (double)c[0] : s[0]);
+        *inverse = mean ? (float)(1.0 / (double)c[0]) : 1.0f;
+    }
+}
+
+// ---- the best label where 32 bits do not decide ---------------------------------------------------------------------
+// Largest norm of a row of the table and largest |bias|, for every block; empties the list of near rays.
+template <class TY> __global__ __launch_bounds__(kThreads) void k_label_bounds(LabelArgs a, float *bounds) {
+    __shared__ float s[2 * kThreads];
+    const int lane = threadIdx.x & 63;
+    float wide = 0.0f, tall = 0.0f;
+    for (int64_t v = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6); v < a.labels; v += (int64_t)kBoundBlocks * kWaves) {
+        const typename TY::E *w = reinterpret_cast<const typename TY::E *>(a.w) + v * a.w_pitch;
+        float n = 0.0f;
+        for (int i = lane; i < a.d; i += 64) n = __builtin_fmaf((float)w[i], (float)w[i], n);
+        for (int step = 32; step > 0; step >>= 1) n += __shfl_xor(n, step);
+        wide = fmaxf(wide, n);
+        if (a.bias) {   // (a label switched off by an infinite bias bounds nothing)
+            const float b = __builtin_fabsf(a.bias[v]);
+            tall = fmaxf(tall, b == kInf ? 0.0f : b);
+        }
+    }
+    s[threadIdx.x] = wide, s[kThreads + threadIdx.x] = tall;
+    for (int step = kThreads / 2; step > 0; step >>= 1) {
+        __syncthreads();
+        if ((int)threadIdx.x < step) {
+            s[threadIdx.x] = fmaxf(s[threadIdx.x], s[threadIdx.x + step]);
+            s[kThreads + threadIdx.x] = fmaxf(s[kThreads + threadIdx.x], s[kThreads + threadIdx.x + step]);
+        }
+    }
+    if (threadIdx.x == 0) {
+        bounds[2 * blockIdx.x] = sqrtf(s[0]) * 1.0001f, bounds[2 * blockIdx.x + 1] = s[kThreads];
+        if (blockIdx.x == 0) *a.near_count = 0u;
+    }
+}
+
+// The rays on the list, decided in 64 bits, a workgroup a ray.
+template <class TY> __global__ __launch_bounds__(kThreads) void k_label_near(LabelArgs a) {
+    __shared__ double x[256], top[kThreads];
+    __shared__ int at[kThreads];
+    const uint32_t n = *a.near_count;
+    for (uint32_t i = blockIdx.x; i < n; i += gridDim.x) {
+        const int64_t row = a.near_list[i];
+        const typename TY::E *xr = reinterpret_cast<const typename TY::E *>(a.x) + row * a.x_pitch;
+        __syncthreads();
+        if ((int)threadIdx.x < a.d) x[threadIdx.x] = (double)(float)xr[threadIdx.x];
+        __syncthreads();
+        double best = -__builtin_huge_val();
+        int label = 0x7fffffff;
+        for (int v = threadIdx.x; v < a.labels; v += kThreads) {
+            const typename TY::E *w = reinterpret_cast<const typename TY::E *>(a.w) + (int64_t)v * a.w_pitch;
+            double s = 0.0;
+            for (int k = 0; k < a.d; ++k) s = __builtin_fma(x[k], (double)(float)w[k], s);
+            if (a.bias) s += (double)a.bias[v];
+            if (s > best) best = s, label = v;
+        }
+        top[threadIdx.x] = best, at[threadIdx.x] = label;
+        for (int step = kThreads / 2; step > 0; step >>= 1) {
+            __syncthreads();
+            if ((int)threadIdx.x < step) {
+                const double b = top[threadIdx.x + step];
+                const int l = at[threadIdx.x + step];
+                if (b > top[threadIdx.x] || (b == top[threadIdx.x] && l < at[threadIdx.x])) top[threadIdx.x] = b, at[threadIdx.x] = l;
+            }
+        }
+        if (threadIdx.x == 0 && at[0] != 0x7fffffff) a.label[row] = at[0];
+    }
+}
+
+// ---- backward -------------------------------------------------------------------------------------------------------
+// dx: rays as own rows, the table streamed.
+template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void k_label_dx(LabelArgs a) {
+    typedef TileShape<NK> T;
+    constexpr int NM = T::kBytes / TY::kSize / 16;
+    __shared__ alignas(16) char tile[T::kRows * T::kPitch];
+    __shared__ alignas(16) float tile_bias[T::kRows];
+    const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6;
+    const int split = blockIdx.x % a.splits;
+    const int64_t row0 = (int64_t)(blockIdx.x / a.splits) * (kWaves * 16 * QB) + wave * 16 * QB;
+    const int first = split * a.per_split * T::kRows;
+    const int last = min(a.labels, (split + 1) * a.per_split * T::kRows);
+
+    Stage<TY, NK> stage;
+    float stage_bias = 0.0f;
+    auto fetch = [&](int at) {
+        stage.load([&](int i) { return row_of<TY, NK>(a.w, at + i, last, a.w_pitch); }, a.d, a.w_vec);
+        if ((int)threadIdx.x < T::kRows && a.bias) stage_bias = at + (int)threadIdx.x < last ? a.bias[at + threadIdx.x] : 0.0f;
+    };
+    fetch(first);
+    Own<TY, NK, QB> own;
+    own.load([&](int i) { return row_of<TY, NK>(a.x, row0 + i, a.rays, a.x_pitch); }, a.d, a.x_vec);
+    float lse2[QB], up[QB];
+    int label[QB];   // relative to the lane's first row of a tile
+    f4 out[QB][NM];
+#pragma unroll
+    for (int q = 0; q < QB; ++q) {
+        const int64_t row = row0 + q * 16 + (lane & 15);
+        const int64_t t = row < a.rays ? a.target[row] : a.ignore;
+        lse2[q] = row < a.rays ? a.lse2[row] : kInf;
+        up[q] = row < a.rays ? upstream_of(a, row, t) : 0.0f;
+        label[q] = (t >= 0 && t < a.labels ? (int)t : -0x40000000) - 4 * g;
+#pragma unroll
+        for (int m = 0; m < NM; ++m) out[q][m] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    for (int at = first; at < last; at += T::kRows) {
+        stage.store(tile);
+        if ((int)threadIdx.x < T::kRows) tile_bias[threadIdx.x] = stage_bias;
+        __syncthreads();
+        if (at + T::kRows < last) fetch(at + T::kRows);
+#pragma unroll
+        for (int pair = 0; pair < T::kBlocks; pair += 2) {
+            f4 p[2][QB];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const f4 b = *reinterpret_cast<const f4 *>(tile_bias + (pair + j) * 16 + 4 * g);
+#pragma unroll
+                for (int q = 0; q < QB; ++q) p[j][q] = b;
+                product<TY, NK, QB>(tile, pair + j, own, p[j]);
+#pragma unroll
+                for (int q = 0; q < QB; ++q)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float e = exp2_of(__builtin_fmaf(p[j][q][r], kLog2E, -lse2[q]));
+                        e -= label[q] - at == (pair + j) * 16 + r ? 1.0f : 0.0f;
+                        p[j][q][r] = e;
+                    }
+            }
+            if (at + T::kRows > last) {   // rows behind the table's end: their products are with zeros, but not of anything
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (at + (pair + j) * 16 + 4 * g + r >= last)
+#pragma unroll
+                            for (int q = 0; q < QB; ++q) p[j][q][r] = 0.0f;
+            }
+            accumulate<TY, NK, QB, NM>(tile, pair, p[0], p[1], out);
+        }
+        __syncthreads();
+    }
+    typedef typename TY::E E;
+    const bool four = (a.d & 3) == 0;
+#pragma unroll
+    for (int q = 0; q < QB; ++q) {
+        const int64_t row = row0 + q * 16 + (lane & 15);
+        if (row >= a.rays) continue;
+#pragma unroll
+        for (int m = 0; m < NM; ++m) {
+            f4 v = out[q][m] * up[q];
+            if (up[q] == 0.0f) v = f4{0.0f, 0.0f, 0.0f, 0.0f};   // (an ignored ray's channels may hold anything)
+            if (a.splits > 1) store_four(a.out_part + ((int64_t)split * a.rays + row) * a.d, m * 16 + 4 * g, a.d, v, four);
+            else store_four(reinterpret_cast<E *>(a.out) + row * a.d, m * 16 + 4 * g, a.d, v, four);
+        }
+    }
+}
+
+// dw and db: labels as own rows, the rays streamed.
+template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void k_label_dw(LabelArgs a) {
+    typedef TileShape<NK> T;
+    constexpr int NM = T::kBytes / TY::kSize / 16;
+    __shared__ alignas(16) char tile[T::kRows * T::kPitch];
+    __shared__ alignas(16) float tile_lse2[T::kRows], tile_up[T::kRows];
+    __shared__ alignas(16) int tile_label[T::kRows];
+    const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6;
+    const int split = blockIdx.x % a.splits;
+    const int row0 = (int)(blockIdx.x / a.splits) * (kWaves * 16 * QB) + wave * 16 * QB;   // (the host keeps labels + a tile below 2^31)
+    const int64_t first = (int64_t)split * a.per_split * T::kRows;
+    const int64_t last = min(a.rays, first + (int64_t)a.per_split * T::kRows);
+
+    Stage<TY, NK> stage;
+    float alive[T::kChunks];   // lse2 of the word's ray: +inf where it is ignored, whose channels may hold anything
+    float stage_lse2 = kInf, stage_up = 0.0f;
+    int stage_label = -1;
+    auto fetch = [&](int64_t at) {
+        stage.load([&](int i) { return row_of<TY, NK>(a.x, at + i, last, a.x_pitch); }, a.d, a.x_vec);
+#pragma unroll
+        for (int c = 0; c < T::kChunks; ++c) {
+            const int64_t row = at + ((int)threadIdx.x + c * kThreads) / (T::kBytes / 16);
+            alive[c] = row < last ? a.lse2[row] : kInf;
+        }
+        if ((int)threadIdx.x < T::kRows) {
+            const int64_t row = at + threadIdx.x, t = row < last ? a.target[row] : a.ignore;
+            stage_lse2 = row < last ? a.lse2[row] : kInf;
+            stage_up = row < last ? upstream_of(a, row, t) : 0.0f;
+            stage_label = t >= 0 && t < a.labels && t != a.ignore ? (int)t : -1;
+        }
+    };
+    fetch(first);
+    Own<TY, NK, QB> own;
+    own.load([&](int i) { return row_of<TY, NK>(a.w, row0 + i, a.labels, a.w_pitch); }, a.d, a.w_vec);
+    float bias[QB], db[QB];
+    f4 out[QB][NM];
+#pragma unroll
+    for (int q = 0; q < QB; ++q) {
+        const int v = row0 + q * 16 + (lane & 15);
+        bias[q] = a.bias && v < a.labels ? a.bias[v] : 0.0f;
+        db[q] = 0.0f;
+#pragma unroll
+        for (int m = 0; m < NM; ++m) out[q][m] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    for (int64_t at = first; at < last; at += T::kRows) {
+#pragma unroll
+        for (int c = 0; c < T::kChunks; ++c)
+            if (alive[c] == kInf) stage.word[c] = u4{0u, 0u, 0u, 0u};
+        stage.store(tile);
+        if ((int)threadIdx.x < T::kRows) tile_lse2[threadIdx.x] = stage_lse2, tile_up[threadIdx.x] = stage_up, tile_label[threadIdx.x] = stage_label;
+        __syncthreads();
+        if (at + T::kRows < last) fetch(at + T::kRows);
+#pragma unroll
+        for (int pair = 0; pair < T::kBlocks; pair += 2) {
+            f4 p[2][QB];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                for (int q = 0; q < QB; ++q) p[j][q] = f4{bias[q], bias[q], bias[q], bias[q]};
+                product<TY, NK, QB>(tile, pair + j, own, p[j]);
+                const int at4 = (pair + j) * 16 + 4 * g;
+                const f4 lse2 = *reinterpret_cast<const f4 *>(tile_lse2 + at4), up = *reinterpret_cast<const f4 *>(tile_up + at4);
+                const int4 label = *reinterpret_cast<const int4 *>(tile_label + at4);
+                const int labels[4] = {label.x, label.y, label.z, label.w};
+#pragma unroll
+                for (int q = 0; q < QB; ++q) {
+                    const int v = row0 + q * 16 + (lane & 15);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float e = exp2_of(__builtin_fmaf(p[j][q][r], kLog2E, -lse2[r]));
+                        e -= labels[r] == v ? 1.0f : 0.0f;
+                        e *= up[r];
+                        p[j][q][r] = e;
+                        db[q] += e;
+                    }
+                }
+            }
+            accumulate<TY, NK, QB, NM>(tile, pair, p[0], p[1], out);
+        }
+        __syncthreads();
+    }
+    typedef typename TY::E E;
+    const bool four = (a.d & 3) == 0;
+#pragma unroll
+    for (int q = 0; q < QB; ++q) {
+        const int v = row0 + q * 16 + (lane & 15);
+        const float b = sum_group(db[q]);
+        if (v >= a.labels) continue;
+        if (g == 0 && a.bias_out) (a.splits > 1 ? a.bias_part + (int64_t)split * a.labels : a.bias_out)[v] = b;
+#pragma unroll
+        for (int m = 0; m < NM; ++m) {
+            if (a.splits > 1) store_four(a.out_part + ((int64_t)split * a.labels + v) * a.d, m * 16 + 4 * g, a.d, out[q][m], four);
+            else store_four(reinterpret_cast<E *>(a.out) + (int64_t)v * a.d, m * 16 + 4 * g, a.d, out[q][m], four);
+        }
+    }
+}
+}  // namespace
+
+// ---- host -----------------------------------------------------------------------------------------------------------
+namespace {
+
+int check(const DstLabelParams *p) {
+    if (!p) return dst_op_fail(DST_E_INVALID, "params is null");
+    if (p->dtype != DST_DTYPE_F32 && p->dtype != DST_DTYPE_BF16 && p->dtype != DST_DTYPE_F16)
+        return dst_op_fail(DST_E_UNSUPPORTED, "dtype must be float32, bfloat16 or float16");
+    if (p->rays < 0 || p->rays > 0x7fffffff) return dst_op_fail(DST_E_INVALID, "rays must be in 0..2^31-1");
+    if (p->labels < 1 || p->labels > DST_MAX_LABELS) return dst_op_fail(DST_E_UNSUPPORTED, "labels must be in 1..%d", DST_MAX_LABELS);
+    if (p->channels < 1 || p->channels > DST_MAX_CHANNELS)
+        return dst_op_fail(DST_E_UNSUPPORTED, "channels must be in 1..%d", DST_MAX_CHANNELS);
+    if (p->features_stride < p->channels || p->weight_stride < p->channels)
+        return dst_op_fail(DST_E_INVALID, "rows of features and weight must not overlap");
+    if (p->reduction < DST_REDUCE_NONE || p->reduction > DST_REDUCE_MEAN) return dst_op_fail(DST_E_INVALID, "unknown reduction");
+    if ((p->rays > 0 && !p->features) || !p->weight) return dst_op_fail(DST_E_INVALID, "features and weight are required");
+    return DST_OK;
+}
+
+LabelArgs arguments(const DstLabelParams *p) {
+    LabelArgs a = {};
+    const int size = value_size(p->dtype);
+    a.x = p->features, a.w = p->weight, a.bias = p->bias, a.target = p->targets;
+    a.x_pitch = p->features_stride, a.w_pitch = p->weight_stride;
+    a.rays = p->rays, a.ignore = p->ignore_index, a.d = p->channels, a.labels = p->labels;
+    a.x_vec = words_align(p->features, p->features_stride, p->channels, size);
+    a.w_vec = words_align(p->weight, p->weight_stride, p->channels, size);
+    a.lse2 = p->lse;
+    a.splits = a.per_split = 1;
+    return a;
+}
+
+template <class TY, int NK> struct Shapes {   // own rows of a workgroup, rows of a tile
+    static constexpr int kForward = kWaves * 16 * forward_blocks<TY, NK>(), kBackward = kWaves * 16 * backward_blocks<TY, NK>();
+    static constexpr int kTile = TileShape<NK>::kRows;
+};
+
+// f(type, integral constant of NK) for the call's type and channels
+template <class TY, class F> int with_fragments(int nk, F f) {
+    switch (nk) {
+        case 1: return f(TY{}, std::integral_constant<int, 1>{});
+        case 2: return f(TY{}, std::integral_constant<int, 2>{});
+        case 4: return f(TY{}, std::integral_constant<int, 4>{});
+        case 8: return f(TY{}, std::integral_constant<int, 8>{});
+        default:
+            if constexpr (TY::kSize == 4) return f(TY{}, std::integral_constant<int, 16>{});
+            return dst_op_fail(DST_E_UNSUPPORTED, "channels must be in 1..%d", DST_MAX_CHANNELS);
+    }
+}
+template <class F> int with_type(const DstLabelParams *p, F f) {
+    const int nk = fragments_of(p->channels, p->dtype);
+    if (p->dtype == DST_DTYPE_F32) return with_fragments<F32>(nk, f);
+    return p->dtype == DST_DTYPE_BF16 ? with_fragments<BF16>(nk, f) : with_fragments<F16>(nk, f);
+}
+
+struct ForwardPlan {
+    Split split;
+    int64_t tiles, blocks;   // own tiles; blocks that leave a sum
+    uint64_t bytes;
+};
+template <class TY, int NK> ForwardPlan forward_plan(const DstLabelParams *p, bool best, char *base, LabelArgs *a) {
+    typedef Shapes<TY, NK> S;
+    ForwardPlan f;
+    f.tiles = div_up(p->rays, S::kForward);
+    f.split = split_tiles(f.tiles, div_up(p->labels, S::kTile));
+    f.blocks = f.split.splits > 1 ? div_up(p->rays, kThreads) : f.tiles;
+    Carve c = {base, 0};
+    LabelArgs unused = {};
+    if (!a) a = &unused;
+    a->splits = f.split.splits, a->per_split = f.split.per_split;
+    if (f.split.splits > 1) {
+        a->part = c.take<float2>((uint64_t)f.split.splits * p->rays);
+        if (best) a->best = c.take<int4>((uint64_t)f.split.splits * p->rays);
+        else a->target_logit = c.take<float>(p->rays);
+    }
+    if (best) {
+        a->bounds = c.take<float>(2 * kBoundBlocks);
+        a->near_count = c.take<uint32_t>(1);
+        a->near_list = c.take<uint32_t>(p->rays);
+    } else if (p->reduction != DST_REDUCE_NONE) {
+        a->sums = c.take<double>(f.blocks);
+        a->counts = c.take<uint32_t>(f.blocks);
+    }
+    f.bytes = c.used;
+    return f;
+}
+
+struct BackwardPlan {
+    Split split;
+    int64_t tiles;
+    uint64_t bytes;
+};
+// dx: the rays are the own rows; else the labels
+template <class TY, int NK> BackwardPlan backward_plan(const DstLabelParams *p, bool dx, char *base, LabelArgs *a) {
+    typedef Shapes<TY, NK> S;
+    const int64_t own = dx ? p->rays : p->labels, streamed = dx ? p->labels : p->rays;
+    BackwardPlan b;
+    b.tiles = div_up(own, S::kBackward);
+    b.split = split_tiles(b.tiles, div_up(streamed, S::kTile));
+    Carve c = {base, 0};
+    LabelArgs unused = {};
+    if (!a) a = &unused;
+    a->splits = b.split.splits, a->per_split = b.split.per_split;
+    if (b.split.splits > 1) {
+        a->out_part = c.take<float>((uint64_t)b.split.splits * own * p->channels);
+        if (!dx) a->bias_part = c.take<float>((uint64_t)b.split.splits * own);
+    }
+    b.bytes = c.used;
+    return b;
+}
+
+int check_workspace(const DstLabelParams *p, uint64_t need) {
+    if (need == 0) return DST_OK;
+    if (!p->workspace || p->workspace_bytes < need)
+        return dst_op_fail(DST_E_INVALID, "workspace of %llu bytes is needed", (unsigned long long)need);
+    if (reinterpret_cast<uintptr_t>(p->workspace) & 255u) return dst_op_fail(DST_E_INVALID, "workspace must be aligned to 256 bytes");
+    return DST_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+uint64_t dst_label_workspace_bytes(const DstLabelParams *p, int pass) {
+    if (check(p) != DST_OK) return 0;
+    uint64_t bytes = 0;
+    with_type(p, [&](auto ty, auto nk) {
+        typedef decltype(ty) TY;
+        constexpr int NK = decltype(nk)::value;
+        if (pass == DST_PASS_BACKWARD) {
+            const uint64_t x = p->grad_features ? backward_plan<TY, NK>(p, true, nullptr, nullptr).bytes : 0;
+            const uint64_t w = p->grad_weight || p->grad_bias ? backward_plan<TY, NK>(p, false, nullptr, nullptr).bytes : 0;
+            bytes = x > w ? x : w;
+        } else {
+            bytes = forward_plan<TY, NK>(p, pass == DST_PASS_BEST, nullptr, nullptr).bytes;
+        }
+        return DST_OK;
+    });
+    return bytes;
+}
+
+int dst_label_loss_forward(const DstLabelParams *p, void *stream) {
+    if (int rc = check(p)) return rc;
+    if (p->rays > 0 && (!p->targets || !p->lse)) return dst_op_fail(DST_E_INVALID, "targets and lse are required");
+    if (!p->loss && (p->rays > 0 || p->reduction != DST_REDUCE_NONE)) return dst_op_fail(DST_E_INVALID, "loss is required");
+    if (p->reduction != DST_REDUCE_NONE && !p->inverse) return dst_op_fail(DST_E_INVALID, "a reduced loss needs inverse");
+    return with_type(p, [&](auto ty, auto nk) {
+        typedef decltype(ty) TY;
+        constexpr int NK = decltype(nk)::value;
+        LabelArgs a = arguments(p);
+        const ForwardPlan f = forward_plan<TY, NK>(p, false, (char *)p->workspace, &a);
+        if (int rc = check_workspace(p, f.bytes)) return rc;
+        if (p->reduction == DST_REDUCE_NONE) a.rows = p->loss;
+        const hipStream_t s = (hipStream_t)stream;
+        if (f.tiles > 0) {
+            k_label_forward<TY, NK, forward_blocks<TY, NK>(), false><<<dim3((uint32_t)(f.tiles * a.splits)), kThreads, 0, s>>>(a);
+            DST_OP_LAUNCH("label loss");
+            if (a.splits > 1) {
+                k_label_join<false><<<dim3((uint32_t)f.blocks), kThreads, 0, s>>>(a);
+                DST_OP_LAUNCH("label loss, joining");
+            }
+        }
+        if (p->reduction != DST_REDUCE_NONE) {
+            k_label_mean<<<1, kThreads, 0, s>>>(a.sums, a.counts, (uint32_t)(f.tiles > 0 ? f.blocks : 0), p->reduction == DST_REDUCE_MEAN,
+                                               p->loss, p->inverse);
+            DST_OP_LAUNCH("label loss, summing");
+        }
+        return (int)DST_OK;
+    });
+}
+
+int dst_label_loss_backward(const DstLabelParams *p, void *stream) {
+    if (int rc = check(p)) return rc;
+    if (p->rays > 0 && (!p->targets || !p->lse || !p->upstream)) return dst_op_fail(DST_E_INVALID, "targets, lse and upstream are required");
+    if (p->reduction != DST_REDUCE_NONE && !p->inverse) return dst_op_fail(DST_E_INVALID, "a reduced loss needs inverse");
+    if (p->dtype == DST_DTYPE_F16) return dst_op_fail(DST_E_UNSUPPORTED, "gradients are of float32 and bfloat16 features");
+    if ((reinterpret_cast<uintptr_t>(p->grad_features) | reinterpret_cast<uintptr_t>(p->grad_weight)) & 15u)
+        return dst_op_fail(DST_E_INVALID, "gradients must be aligned to 16 bytes");
+    auto launch = [&](auto ty, auto nk) {
+        typedef decltype(ty) TY;
+        typedef typename TY::E E;
+        constexpr int NK = decltype(nk)::value, QB = backward_blocks<TY, NK>();
+        const hipStream_t s = (hipStream_t)stream;
+        for (int pass = 0; pass < 2; ++pass) {
+            const bool dx = pass == 0;
+            if (dx ? !p->grad_features || p->rays == 0 : !p->grad_weight && !p->grad_bias) continue;
+            LabelArgs a = arguments(p);
+            const BackwardPlan b = backward_plan<TY, NK>(p, dx, (char *)p->workspace, &a);
+            if (int rc = check_workspace(p, b.bytes)) return rc;
+            a.upstream = p->upstream, a.upstream_rows = p->reduction == DST_REDUCE_NONE;
+            a.inverse = a.upstream_rows ? nullptr : p->inverse;
+            a.out = dx ? p->grad_features : p->grad_weight, a.bias_out = p->grad_bias;
+            const dim3 grid((uint32_t)(b.tiles * a.splits));
+            if (dx) k_label_dx<TY, NK, QB><<<grid, kThreads, 0, s>>>(a);
+            else k_label_dw<TY, NK, QB><<<grid, kThreads, 0, s>>>(a);
+            DST_OP_LAUNCH("label gradient");
+            if (a.splits > 1) {
+                const int64_t n = (dx ? p->rays : (int64_t)p->labels) * p->channels;
+                if (a.out) k_sum_parts<E><<<dim3(sum_blocks(n)), 256, 0, s>>>(a.out_part, (E *)a.out, n, a.splits);
+                if (!dx && p->grad_bias) k_sum_parts<float><<<dim3(sum_blocks(p->labels)), 256, 0, s>>>(a.bias_part, p->grad_bias, p->labels, a.splits);
+                DST_OP_LAUNCH("label gradient, summing");
+            }
+        }
+        return (int)DST_OK;
+    };
+    const int nk = fragments_of(p->channels, p->dtype);
+    return p->dtype == DST_DTYPE_F32 ? with_fragments<F32>(nk, launch) : with_fragments<BF16>(nk, launch);
+}
+
+int dst_label_best(const DstLabelParams *p, void *stream) {
+    if (int rc = check(p)) return rc;
+    if (p->rays == 0) return DST_OK;
+    if (!p->best || !p->log_prob) return dst_op_fail(DST_E_INVALID, "best and log_prob are required");
+    return with_type(p, [&](auto ty, auto nk) {
+        typedef decltype(ty) TY;
+        constexpr int NK = decltype(nk)::value;
+        LabelArgs a = arguments(p);
+        const ForwardPlan f = forward_plan<TY, NK>(p, true, (char *)p->workspace, &a);
+        if (int rc = check_workspace(p, f.bytes)) return rc;
+        a.label = p->best, a.log_prob = p->log_prob;
+        const hipStream_t s = (hipStream_t)stream;
+        k_label_bounds<TY><<<kBoundBlocks, kThreads, 0, s>>>(a, const_cast<float *>(a.bounds));
+        k_label_forward<TY, NK, forward_blocks<TY, NK>(), true><<<dim3((uint32_t)(f.tiles * a.splits)), kThreads, 0, s>>>(a);
+        DST_OP_LAUNCH("best label");
+        if (a.splits > 1) k_label_join<true><<<dim3((uint32_t)f.blocks), kThreads, 0, s>>>(a);
+        // (as many workgroups as the device holds; each takes rays off the list until there are no more)
+        k_label_near<TY><<<dim3((uint32_t)(p->rays < 2048 ? p->rays : 2048)), kThreads, 0, s>>>(a);
+        DST_OP_LAUNCH("best label, near rays");
+        return (int)DST_OK;
+    });
+}
+
+}  // extern "C"

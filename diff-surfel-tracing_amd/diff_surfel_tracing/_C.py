@@ -57,6 +57,25 @@ class DstTraceInfo(C.Structure):
                 ("tiles_handed_over", C.c_uint64)]
 
 
+class DstLabelParams(C.Structure):
+    """Field-for-field mirror of `DstLabelParams` in include/dst_api.h."""
+    _fields_ = [("rays", C.c_int64), ("channels", C.c_int32), ("labels", C.c_int32), ("dtype", C.c_int32),
+                ("reduction", C.c_int32), ("features", _FP), ("features_stride", C.c_int64), ("weight", _FP),
+                ("weight_stride", C.c_int64), ("bias", _FP), ("targets", _FP), ("ignore_index", C.c_int64), ("loss", _FP),
+                ("lse", _FP), ("inverse", _FP), ("upstream", _FP), ("grad_features", _FP), ("grad_weight", _FP),
+                ("grad_bias", _FP), ("best", _FP), ("log_prob", _FP), ("workspace", _FP), ("workspace_bytes", C.c_uint64)]
+
+
+class DstAttendParams(C.Structure):
+    """Field-for-field mirror of `DstAttendParams` in include/dst_api.h."""
+    _fields_ = ([(n, C.c_int32) for n in ("batch", "queries", "memory", "heads", "kv_heads", "channels", "value_channels",
+                                          "dtype")]
+                + [("scale", C.c_float), ("reserved", C.c_int32), ("q", _FP), ("k", _FP), ("v", _FP)]
+                + [(n, C.c_int64 * 3) for n in ("q_strides", "k_strides", "v_strides")]
+                + [(n, _FP) for n in ("lengths", "out", "lse", "upstream", "grad_q", "grad_k", "grad_v", "workspace")]
+                + [("workspace_bytes", C.c_uint64)])
+
+
 HANDOVER_OFF, HANDOVER_AUTO, HANDOVER_ALWAYS = 0, 1, 2
 
 
@@ -64,7 +83,10 @@ EXPORTS = ("dst_create", "dst_destroy", "dst_build_accel", "dst_trace_forward", 
            "dst_last_error", "dst_accel_info", "dst_accel_download", "dst_version", "dst_sizeof_params",
            "dst_hit_record_layout", "dst_refit_accel_static", "dst_refit_from_surfels",
            "dst_det_workspace_words", "dst_trace_scratch_bytes",
-           "dst_trace_scratch_needed", "dst_pack_sh_half", "dst_trace_info", "dst_set_handover", "dst_det_out_of_range")
+           "dst_trace_scratch_needed", "dst_pack_sh_half", "dst_trace_info", "dst_set_handover", "dst_det_out_of_range",
+           "dst_label_workspace_bytes", "dst_label_loss_forward", "dst_label_loss_backward", "dst_label_best",
+           "dst_attend_workspace_bytes", "dst_attend_forward", "dst_attend_backward", "dst_op_error",
+           "dst_sizeof_label_params", "dst_sizeof_attend_params")
 
 _lib = None
 
@@ -107,6 +129,20 @@ def load_library():
     L.dst_hit_record_layout.restype = C.c_uint64
     L.dst_hit_record_layout.argtypes = [C.c_int32, C.c_int32, C.c_int32, C.c_uint32, C.POINTER(C.c_uint64),
                                         C.POINTER(C.c_uint32)]
+    for name in ("dst_label_workspace_bytes", "dst_attend_workspace_bytes"):
+        block = DstLabelParams if "label" in name else DstAttendParams
+        getattr(L, name).restype = C.c_uint64
+        getattr(L, name).argtypes = [C.POINTER(block), C.c_int]
+    for name in ("dst_label_loss_forward", "dst_label_loss_backward", "dst_label_best"):
+        getattr(L, name).argtypes = [C.POINTER(DstLabelParams), C.c_void_p]
+    for name in ("dst_attend_forward", "dst_attend_backward"):
+        getattr(L, name).argtypes = [C.POINTER(DstAttendParams), C.c_void_p]
+    L.dst_op_error.restype = C.c_char_p
+    L.dst_sizeof_label_params.restype = C.c_size_t
+    L.dst_sizeof_attend_params.restype = C.c_size_t
+    for name, block in (("label", DstLabelParams), ("attend", DstAttendParams)):
+        if getattr(L, "dst_sizeof_%s_params" % name)() != C.sizeof(block):
+            raise ImportError("diff_surfel_tracing: %s layout mismatch between _C.py and libdst.so" % block.__name__)
     if L.dst_sizeof_params() != C.sizeof(DstParams):
         raise ImportError("diff_surfel_tracing: DstParams layout mismatch between _C.py and libdst.so")
     _lib = L

@@ -2,7 +2,8 @@
 
 Public names, argument order, defaults and return tuples follow the reference package
 (reference diff_surfel_tracing/__init__.py:14-290):
-`SurfelTracer`, `SurfelTracingSettings`, `trace_surfels`, `_TraceSurfels`.  The work happens in
+`SurfelTracer`, `SurfelTracingSettings`, `trace_surfels`, `_TraceSurfels`.  Beside them, what a ray's channels are
+read with (see `features.py`): `label_loss`, `label_rays`, `attend_memory`.  The work happens in
 hand-written HIP kernels behind the C ABI of libdst.so (see `_C.py`); there is no fallback path.
 """
 import threading
@@ -13,8 +14,9 @@ import torch.nn as nn
 from torch.autograd import forward_ad
 
 from . import _C
+from .features import attend_memory, label_loss, label_rays
 
-__all__ = ["SurfelTracer", "SurfelTracingSettings", "trace_surfels"]
+__all__ = ["SurfelTracer", "SurfelTracingSettings", "trace_surfels", "label_loss", "label_rays", "attend_memory"]
 
 
 def cpu_deep_copy_tuple(input_tuple):

@@ -296,6 +296,91 @@ uint64_t dst_det_workspace_words(int32_t P, int32_t aux, int backward);
  * reference, whose SH coefficients are fp32 (optix_tracer/forward.cu:265-268). */
 int dst_pack_sh_half(const float *shs, uint16_t *out, uint64_t n_values, void *stream);
 
+/* ---- What a ray's channels are read with (no counterpart in the reference, which hands out_aux to its caller) --------
+ * Operators on the channels that traces return, or on what a caller makes of them: rows of up to DST_MAX_CHANNELS values,
+ * against a table of labels or a memory of another length, through a softmax whose matrix is never stored.
+ * They need no context: device pointers of the current device, all work on `stream`, nothing allocated, nothing waited for, nothing kept
+ * between calls (a call may be recorded into a graph and replayed; calls that overlap need workspaces of their own).  Status as above; dst_op_error() then describes the calling
+ * thread's last failure.  All sums are in fp32 or wider and have one order: the same inputs give the same bits. */
+#define DST_DTYPE_F32 0
+#define DST_DTYPE_BF16 1
+#define DST_DTYPE_F16 2             /* forward passes only: gradients of binary16 rows would need a scale of their own */
+#define DST_MAX_CHANNELS 256
+#define DST_MAX_LABELS 0x3fffffff
+#define DST_REDUCE_NONE 0
+#define DST_REDUCE_SUM 1
+#define DST_REDUCE_MEAN 2
+#define DST_PASS_FORWARD 0
+#define DST_PASS_BACKWARD 1
+#define DST_PASS_BEST 2
+
+/* Softmax cross entropy of rays against a table of labels: s = features . weight^T + bias, loss = log sum exp s - s[target],
+ * 0 where the target is ignore_index, NaN (and NaN gradients) where it is neither that nor in 0..labels-1. */
+typedef struct DstLabelParams {
+    int64_t rays;                 /* 0..2^31-1 */
+    int32_t channels, labels;     /* 1..DST_MAX_CHANNELS, 1..DST_MAX_LABELS */
+    int32_t dtype;                /* DST_DTYPE_* of features and weight and of their gradients */
+    int32_t reduction;            /* DST_REDUCE_*; the mean is over the rays that are not ignored (none: NaN) */
+    const void *features;         /* (rays, channels), features_stride values from ray to ray */
+    int64_t features_stride;
+    const void *weight;           /* (labels, channels), weight_stride values from label to label */
+    int64_t weight_stride;
+    const float *bias;            /* (labels) or NULL; -inf switches a label off */
+    const int64_t *targets;       /* (rays) */
+    int64_t ignore_index;
+    float *loss;                  /* forward: (rays) for DST_REDUCE_NONE, else one value */
+    float *lse;                   /* (rays): forward writes, backward reads (log2 of the sum of exponentials; +inf: ignored) */
+    float *inverse;               /* one value, unless DST_REDUCE_NONE: forward writes, backward reads */
+    const float *upstream;        /* backward: gradient of the loss, of its shape */
+    void *grad_features;          /* backward: (rays, channels), written whole; NULL: not wanted */
+    void *grad_weight;            /* (labels, channels); NULL: not wanted */
+    float *grad_bias;             /* (labels); NULL: not wanted */
+    int64_t *best;                /* best: (rays), the label of the largest s, the lowest of equal ones */
+    float *log_prob;              /* best: (rays), its log probability */
+    void *workspace;              /* dst_label_workspace_bytes(), aligned to 256 bytes; contents mean nothing */
+    uint64_t workspace_bytes;
+} DstLabelParams;
+
+/* Bytes of workspace for DST_PASS_FORWARD, _BACKWARD (by the gradients wanted) or _BEST; 0 also where the sizes are refused. */
+uint64_t dst_label_workspace_bytes(const DstLabelParams *params, int pass);
+int dst_label_loss_forward(const DstLabelParams *params, void *stream);
+int dst_label_loss_backward(const DstLabelParams *params, void *stream);
+/* The best label of every ray, as if the logits were formed in 64 bits (rays whose two best labels fp32 cannot tell
+ * apart are decided again in 64 bits).  A ray with NaN among its logits gets some label and log probability NaN. */
+int dst_label_best(const DstLabelParams *params, void *stream);
+
+/* Attention of queries to a memory of another length, no mask but each batch's length: for query head h of `heads`, which reads
+ * kv head h / (heads / kv_heads):  p = softmax_j(scale q . k_j) over j < lengths[batch],  out = sum_j p_j v_j.
+ * A length of 0 gives zeros and no gradient.  Keys and values behind the length are not used and may hold anything. */
+typedef struct DstAttendParams {
+    int32_t batch, queries, memory;   /* >= 0 */
+    int32_t heads, kv_heads;          /* heads a multiple of kv_heads */
+    int32_t channels, value_channels; /* 1..DST_MAX_CHANNELS */
+    int32_t dtype;                    /* DST_DTYPE_* of all rows */
+    float scale;
+    int32_t reserved;
+    const void *q, *k, *v;            /* rows of channels (value_channels) consecutive values; strides in values, by batch, */
+    int64_t q_strides[3], k_strides[3], v_strides[3];   /* row and head (0: shared) */
+    const int32_t *lengths;           /* (batch), clamped to 0..memory; NULL: memory everywhere */
+    void *out;                        /* (batch, queries, heads, value_channels), contiguous, as all that follow */
+    float *lse;                       /* (batch, kv_heads, queries * heads / kv_heads): forward writes (NULL: not wanted),
+                                       * backward reads (log2 of the sum of exponentials; +inf where there is no memory) */
+    const void *upstream;             /* backward: gradient of out, of its shape */
+    void *grad_q;                     /* (batch, queries, heads, channels) */
+    void *grad_k, *grad_v;            /* (batch, memory, kv_heads, ...): zeros behind the lengths; NULL (either, or grad_q): not wanted */
+    void *workspace;                  /* dst_attend_workspace_bytes(), aligned to 256 bytes */
+    uint64_t workspace_bytes;
+} DstAttendParams;
+
+uint64_t dst_attend_workspace_bytes(const DstAttendParams *params, int pass);   /* DST_PASS_FORWARD or _BACKWARD */
+int dst_attend_forward(const DstAttendParams *params, void *stream);
+int dst_attend_backward(const DstAttendParams *params, void *stream);
+
+/* Message of the calling thread's last failure of these operators (never NULL), and the sizes of their parameter blocks. */
+const char *dst_op_error(void);
+size_t dst_sizeof_label_params(void);
+size_t dst_sizeof_attend_params(void);
+
 /* Library version string, and sizeof(DstParams) as compiled (lets a foreign-language binding
  * verify its own struct layout before the first launch). */
 const char *dst_version(void);
