@@ -12,7 +12,7 @@
 
 #include "tiles.inc"
 
-#include "features.h"
+#include "operators.h"
 
 namespace {
 
@@ -195,7 +195,63 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     }
 }
 
-// The parts of a split forward pass: a thread for four channels of a row.
+// The parts of a split forward pass, a workgroup a row: for many parts of few rows (one ray that asks a long memory), which the
+// kernel below would go through one after another (8 rows of 256 parts: 5 us, 45 with that one).
+template <class E> __global__ __launch_bounds__(kThreads) void k_attend_join_row(AttendArgs a, int rows_per_part) {
+    __shared__ float weight[kMostSplits], wave_top[kWaves], wave_sum[kWaves];
+    __shared__ f4 sums[kThreads];
+    const int64_t at = blockIdx.x;
+    Place p;
+    p.kv = (int)(at / a.rows % a.kv_heads), p.batch = (int)(at / a.rows / a.kv_heads);
+    const int row = (int)(at % a.rows), tid = threadIdx.x;
+    const int length = a.lengths ? min(max(a.lengths[p.batch], 0), a.memory) : a.memory;
+    const int used = (length + rows_per_part - 1) / rows_per_part;   // (parts behind the length left no sums)
+    float top = -kInf;
+    for (int s = tid; s < used; s += kThreads) top = fmaxf(top, a.part[(int64_t)s * a.all_rows + at].x);
+    for (int step = 32; step > 0; step >>= 1) top = fmaxf(top, __shfl_xor(top, step));
+    if ((tid & 63) == 0) wave_top[tid >> 6] = top;
+    __syncthreads();
+    const float m = fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3])), use = finite_or_zero(m);
+    float l = 0.0f;
+    for (int s = tid; s < used; s += kThreads) {
+        const float2 ml = a.part[(int64_t)s * a.all_rows + at];
+        const float by = exp2_of(ml.x - use);
+        weight[s] = by;
+        l += ml.y * by;
+    }
+    for (int step = 32; step > 0; step >>= 1) l += __shfl_xor(l, step);
+    if ((tid & 63) == 0) wave_sum[tid >> 6] = l;
+    __syncthreads();
+    l = (wave_sum[0] + wave_sum[1]) + (wave_sum[2] + wave_sum[3]);
+    const int words = (a.dv + 3) / 4;   // at most 64
+    int wide = 1;
+    while (wide < words) wide *= 2;
+    const int word = tid & (wide - 1), lane = tid / wide, lanes = kThreads / wide;
+    const bool four = (a.dv & 3) == 0;
+    f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (word < words) {
+#pragma unroll 4
+        for (int s = lane; s < used; s += lanes) {
+            const float *from = a.out_part + ((int64_t)s * a.all_rows + at) * a.dv + 4 * word;
+            if (four) {
+                o += *reinterpret_cast<const f4 *>(from) * weight[s];
+            } else {
+                for (int i = 0; i < 4; ++i)
+                    if (4 * word + i < a.dv) o[i] += from[i] * weight[s];
+            }
+        }
+    }
+    sums[tid] = o;
+    for (int step = lanes / 2; step > 0; step >>= 1) {
+        __syncthreads();
+        if (lane < step) sums[tid] += sums[tid + step * wide];
+    }
+    if (tid == 0 && a.lse2) a.lse2[at] = length > 0 ? m + log2_of(l) : kInf;
+    if (lane == 0 && word < words)
+        store_four(reinterpret_cast<E *>(a.out) + out_row(a, p, row) * a.dv, 4 * word, a.dv, length > 0 ? sums[tid] * (1.0f / l) : sums[tid], four);
+}
+
+// The same, a thread for four channels of a row.
 template <class E> __global__ __launch_bounds__(kThreads) void k_attend_join(AttendArgs a, int rows_per_part) {
     const int words = (a.dv + 3) / 4;
     const int64_t id = (int64_t)blockIdx.x * kThreads + threadIdx.x, at = id / words;
@@ -488,8 +544,19 @@ template <class F> int with_type(const DstAttendParams *p, F f) {
     return p->dtype == DST_DTYPE_BF16 ? with_fragments<BF16>(fragments(p), f) : with_fragments<F16>(fragments(p), f);
 }
 
-// Few rows (one query and its heads): a wave with one block of them leaves the others nothing but to load.
-template <class TY, int NK> int forward_rows(const AttendArgs &a) { return kWaves * 16 * (a.rows <= kWaves * 16 ? 1 : forward_blocks<TY, NK>()); }
+// Own blocks of 16 rows a wave: one where the rows are few, by the rule that every pass has.
+int blocks_for(int most, int64_t rows, int64_t heads, int tile, int64_t streamed) {
+    return rows <= kWaves * 16 || few_rows(div_up(rows, kWaves * 16 * most) * heads, 1, div_up(streamed, tile)) ? 1 : most;
+}
+template <class TY, int NK> int forward_rows(const AttendArgs &a, int64_t heads) {
+    return kWaves * 16 * blocks_for(forward_blocks<TY, NK>(), a.rows, heads, TileShape<NK>::kRows, a.memory);
+}
+template <class TY, int NK> int dq_rows(const AttendArgs &a, int64_t heads) {
+    return kWaves * 16 * blocks_for(dq_blocks<TY, NK>(), a.rows, heads, TileShape<NK>::kRows, a.memory);
+}
+template <class TY, int NK> int dkv_rows(const AttendArgs &a, int64_t heads) {
+    return kWaves * 16 * blocks_for(dkv_blocks<TY, NK>(), a.memory, heads, TileShape<NK>::kRows, a.rows);
+}
 
 uint64_t plan_forward(AttendArgs &a, int own, int tile, int64_t heads, char *base) {
     a.tiles = (int)div_up(a.rows, own);
@@ -547,12 +614,12 @@ uint64_t dst_attend_workspace_bytes(const DstAttendParams *p, int pass) {
         const int64_t heads = (int64_t)p->batch * p->kv_heads;
         if (a.all_rows == 0 && pass == DST_PASS_FORWARD) return DST_OK;
         if (pass == DST_PASS_FORWARD) {
-            bytes = plan_forward(a, forward_rows<TY, NK>(a), TileShape<NK>::kRows, heads, nullptr);
+            bytes = plan_forward(a, forward_rows<TY, NK>(a, heads), TileShape<NK>::kRows, heads, nullptr);
         } else {
             a.dq = p->grad_q;
-            bytes = plan_dq(a, kWaves * 16 * dq_blocks<TY, NK>(), TileShape<NK>::kRows, heads, nullptr);
+            bytes = plan_dq(a, dq_rows<TY, NK>(a, heads), TileShape<NK>::kRows, heads, nullptr);
             if (p->grad_k || p->grad_v) {
-                const uint64_t more = plan_dkv(a, kWaves * 16 * dkv_blocks<TY, NK>(), TileShape<NK>::kRows, heads, nullptr);
+                const uint64_t more = plan_dkv(a, dkv_rows<TY, NK>(a, heads), TileShape<NK>::kRows, heads, nullptr);
                 bytes = more > bytes ? more : bytes;
             }
         }
@@ -570,16 +637,19 @@ int dst_attend_forward(const DstAttendParams *p, void *stream) {
         AttendArgs a = arguments(p);
         if (a.all_rows == 0) return (int)DST_OK;
         const int64_t heads = (int64_t)p->batch * p->kv_heads;
-        const uint64_t need = plan_forward(a, forward_rows<TY, NK>(a), TileShape<NK>::kRows, heads, (char *)p->workspace);
+        const int own = forward_rows<TY, NK>(a, heads);
+        const uint64_t need = plan_forward(a, own, TileShape<NK>::kRows, heads, (char *)p->workspace);
         if (int rc = check_workspace(p, need)) return rc;
         const hipStream_t s = (hipStream_t)stream;
         const dim3 grid((uint32_t)(a.tiles * heads * a.splits));
-        if (a.rows <= kWaves * 16) k_attend_forward<TY, NK, 1><<<grid, kThreads, 0, s>>>(a);
+        if (own == kWaves * 16) k_attend_forward<TY, NK, 1><<<grid, kThreads, 0, s>>>(a);
         else k_attend_forward<TY, NK, QB><<<grid, kThreads, 0, s>>>(a);
         DST_OP_LAUNCH("attention");
         if (a.splits > 1) {
             const int64_t words = a.all_rows * ((a.dv + 3) / 4);
-            k_attend_join<E><<<dim3((uint32_t)div_up(words, kThreads)), kThreads, 0, s>>>(a, a.per_split * TileShape<NK>::kRows);
+            const int part = a.per_split * TileShape<NK>::kRows;
+            if (a.splits >= 16) k_attend_join_row<E><<<dim3((uint32_t)a.all_rows), kThreads, 0, s>>>(a, part);
+            else k_attend_join<E><<<dim3((uint32_t)div_up(words, kThreads)), kThreads, 0, s>>>(a, part);
             DST_OP_LAUNCH("attention, joining");
         }
         return (int)DST_OK;
@@ -597,32 +667,35 @@ int dst_attend_backward(const DstAttendParams *p, void *stream) {
         typedef decltype(ty) TY;
         typedef typename TY::E E;
         constexpr int NK = decltype(nk)::value;
-        constexpr int tile = TileShape<NK>::kRows, dq_rows = kWaves * 16 * dq_blocks<TY, NK>(), dkv_rows = kWaves * 16 * dkv_blocks<TY, NK>();
+        constexpr int tile = TileShape<NK>::kRows;
         const hipStream_t s = (hipStream_t)stream;
         const int64_t heads = (int64_t)p->batch * p->kv_heads;
         AttendArgs a = arguments(p);
         a.up = p->upstream, a.dq = p->grad_q, a.dk = p->grad_k, a.dvalue = p->grad_v;
         if (a.all_rows > 0) {
-            const uint64_t need = plan_dq(a, dq_rows, tile, heads, (char *)p->workspace);
+            const int own = dq_rows<TY, NK>(a, heads);
+            const uint64_t need = plan_dq(a, own, tile, heads, (char *)p->workspace);
             if (int rc = check_workspace(p, need)) return rc;
-            k_attend_dq<TY, NK, dq_blocks<TY, NK>()><<<dim3((uint32_t)(a.tiles * heads * a.splits)), kThreads, 0, s>>>(a);
+            const dim3 grid((uint32_t)(a.tiles * heads * a.splits));
+            if (own == kWaves * 16) k_attend_dq<TY, NK, 1><<<grid, kThreads, 0, s>>>(a);
+            else k_attend_dq<TY, NK, dq_blocks<TY, NK>()><<<grid, kThreads, 0, s>>>(a);
             DST_OP_LAUNCH("attention gradient, queries");
             if (a.splits > 1) {
-                const int64_t n = a.all_rows * a.d;
-                k_sum_parts<E><<<dim3(sum_blocks(n)), 256, 0, s>>>(a.out_part, (E *)a.dq, n, a.splits);
+                sum_parts(a.out_part, (E *)a.dq, a.all_rows * a.d, nullptr, (E *)nullptr, 0, a.splits, s);
                 DST_OP_LAUNCH("attention gradient, summing");
             }
         }
         if ((a.dk || a.dvalue) && heads * a.memory > 0) {
-            const uint64_t need = plan_dkv(a, dkv_rows, tile, heads, (char *)p->workspace);
+            const int own = dkv_rows<TY, NK>(a, heads);
+            const uint64_t need = plan_dkv(a, own, tile, heads, (char *)p->workspace);
             if (int rc = check_workspace(p, need)) return rc;
             a.own_all = heads * a.memory;
-            k_attend_dkv<TY, NK, dkv_blocks<TY, NK>()><<<dim3((uint32_t)(a.tiles * heads * a.splits)), kThreads, 0, s>>>(a);
+            const dim3 grid((uint32_t)(a.tiles * heads * a.splits));
+            if (own == kWaves * 16) k_attend_dkv<TY, NK, 1><<<grid, kThreads, 0, s>>>(a);
+            else k_attend_dkv<TY, NK, dkv_blocks<TY, NK>()><<<grid, kThreads, 0, s>>>(a);
             DST_OP_LAUNCH("attention gradient, memory");
             if (a.splits > 1) {
-                const int64_t nk_ = a.own_all * a.d, nv = a.own_all * a.dv;
-                if (a.dk) k_sum_parts<E><<<dim3(sum_blocks(nk_)), 256, 0, s>>>(a.out_part, (E *)a.dk, nk_, a.splits);
-                if (a.dvalue) k_sum_parts<E><<<dim3(sum_blocks(nv)), 256, 0, s>>>(a.out_part2, (E *)a.dvalue, nv, a.splits);
+                sum_parts(a.out_part, (E *)a.dk, a.own_all * a.d, a.out_part2, (E *)a.dvalue, a.own_all * a.dv, a.splits, s);
                 DST_OP_LAUNCH("attention gradient, summing");
             }
         }

@@ -1,7 +1,7 @@
 // C ABI of libdst.so: context management, argument validation, launches.
 // Replaces the pybind module and host launcher of the reference (ext.cpp, trace_surfels.cpp).
 #include "dst_internal.h"
-#include "features.h"
+#include "operators.h"
 
 #include <cstdarg>
 #include <cstdio>

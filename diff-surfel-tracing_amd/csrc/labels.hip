@@ -12,7 +12,7 @@
 
 #include "tiles.inc"
 
-#include "features.h"
+#include "operators.h"
 
 namespace {
 
@@ -39,7 +39,8 @@ struct LabelArgs {
     int64_t *label;                 // (rays)
     float *log_prob;                // (rays)
     uint32_t *near_count;           // rays whose two best labels 32 bits cannot tell apart ...
-    uint32_t *near_list;            // ... and which
+    uint32_t *near_list;            // ... which ...
+    float *near_floor;              // ... and what a label's logit has to come to to be the best
     // backward
     const float *upstream;          // (rays) or one value
     const float *inverse;           // one value that multiplies a single upstream value, or nullptr
@@ -102,14 +103,24 @@ __device__ inline void block_sums(const LabelArgs &a, double sum, uint32_t count
 // The best label of a ray, or a place on the list of those that 32 bits cannot decide: a logit of d products is off by less
 // than (d + 16) 2^-22 times the norms (the tile product rounds at most once a product and once a block), twice that between
 // two; a ray without channels has none.
-__device__ inline void finish_best(const LabelArgs &a, int64_t row, Running r, float best, int label, float second, float norm) {
-    float wide = 0.0f, tall = 0.0f;
-    for (int i = 0; i < kBoundBlocks; ++i) wide = fmaxf(wide, a.bounds[2 * i]), tall = fmaxf(tall, a.bounds[2 * i + 1]);
+__device__ inline void finish_best(const LabelArgs &a, int64_t row, Running r, float best, int label, float second, float norm, float2 bound) {
+    const float wide = bound.x, tall = bound.y;
     const float off = norm > 0.0f ? 2.3841858e-7f * ((float)(a.d + 16) * norm * wide + 2.0f * tall) : 0.0f;
     a.label[row] = label == 0x7fffffff ? 0 : label;
     a.log_prob[row] = -log2_of(r.l) * kLn2;
-    if (best - second < 2.0f * off) a.near_list[atomicAdd(a.near_count, 1u)] = (uint32_t)row;
+    if (best - second < 2.0f * off) {
+        const uint32_t i = atomicAdd(a.near_count, 1u);
+        a.near_list[i] = (uint32_t)row;
+        a.near_floor[i] = best - 3.0f * off;   // (the best label's logit is best - off at least, and another sum of it off by as much)
+    }
 }
+// The largest norm and |bias| over the blocks that looked for them: every lane of a wave takes one.
+__device__ inline float2 table_bound(const LabelArgs &a) {
+    float2 b = reinterpret_cast<const float2 *>(a.bounds)[threadIdx.x & 63];
+    for (int step = 32; step > 0; step >>= 1) b.x = fmaxf(b.x, __shfl_xor(b.x, step)), b.y = fmaxf(b.y, __shfl_xor(b.y, step));
+    return b;
+}
+static_assert(kBoundBlocks == 64, "a lane each");
 
 // (best, label) of two lanes or parts: the larger, the lower label where they are equal; `second`: the largest of the others.
 __device__ inline void merge_best(float &best, int &label, float &second, float b, int l, float s) {
@@ -215,6 +226,8 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
 
     double sum = 0.0;
     uint32_t count = 0;
+    float2 bound = {0.0f, 0.0f};
+    if constexpr (BEST) bound = table_bound(a);
 #pragma unroll
     for (int q = 0; q < QB; ++q) {
         const int64_t row = row0 + q * 16 + (lane & 15);
@@ -233,7 +246,7 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
                     a.best[(int64_t)split * a.rays + row] = int4{__builtin_bit_cast(int, best[q]), label[q], __builtin_bit_cast(int, second[q]),
                                                                  __builtin_bit_cast(int, norm)};
                 } else {
-                    finish_best(a, row, r, best[q], label[q], second[q], norm);
+                    finish_best(a, row, r, best[q], label[q], second[q], norm, bound);
                 }
             }
         } else {
@@ -268,6 +281,8 @@ template <bool BEST> __global__ __launch_bounds__(kThreads) void k_label_join(La
     const int64_t row = (int64_t)blockIdx.x * kThreads + threadIdx.x;
     double sum = 0.0;
     uint32_t count = 0;
+    float2 bound = {0.0f, 0.0f};
+    if constexpr (BEST) bound = table_bound(a);
     if (row < a.rays) {
         Running r = {-kInf, 0.0f};
         float best = -kInf, second = -kInf, norm = 0.0f;
@@ -281,7 +296,7 @@ template <bool BEST> __global__ __launch_bounds__(kThreads) void k_label_join(La
                 norm = __builtin_bit_cast(float, b.w);
             }
         }
-        if constexpr (BEST) finish_best(a, row, r, best, label, second, norm);
+        if constexpr (BEST) finish_best(a, row, r, best, label, second, norm, bound);
         else finish_row(a, row, r, a.target_logit[row], sum, count);
     }
     if constexpr (!BEST) block_sums(a, sum, count, lds);
@@ -337,25 +352,39 @@ template <class TY> __global__ __launch_bounds__(kThreads) void k_label_bounds(L
     }
 }
 
-// The rays on the list, decided in 64 bits, a workgroup a ray.
+// The rays on the list, a workgroup each: every label's logit again in 32 bits, and in 64 where it can be the best.
 template <class TY> __global__ __launch_bounds__(kThreads) void k_label_near(LabelArgs a) {
-    __shared__ double x[256], top[kThreads];
+    constexpr int per = 16 / TY::kSize;
+    typedef typename TY::E E;
+    __shared__ alignas(16) float x[DST_MAX_CHANNELS];
+    __shared__ double top[kThreads];
     __shared__ int at[kThreads];
     const uint32_t n = *a.near_count;
     for (uint32_t i = blockIdx.x; i < n; i += gridDim.x) {
         const int64_t row = a.near_list[i];
-        const typename TY::E *xr = reinterpret_cast<const typename TY::E *>(a.x) + row * a.x_pitch;
+        const float floor = a.near_floor[i];
+        const E *xr = reinterpret_cast<const E *>(a.x) + row * a.x_pitch;
         __syncthreads();
-        if ((int)threadIdx.x < a.d) x[threadIdx.x] = (double)(float)xr[threadIdx.x];
+        x[threadIdx.x] = (int)threadIdx.x < a.d ? (float)xr[threadIdx.x] : 0.0f;
         __syncthreads();
         double best = -__builtin_huge_val();
         int label = 0x7fffffff;
         for (int v = threadIdx.x; v < a.labels; v += kThreads) {
-            const typename TY::E *w = reinterpret_cast<const typename TY::E *>(a.w) + (int64_t)v * a.w_pitch;
-            double s = 0.0;
-            for (int k = 0; k < a.d; ++k) s = __builtin_fma(x[k], (double)(float)w[k], s);
-            if (a.bias) s += (double)a.bias[v];
-            if (s > best) best = s, label = v;
+            const E *w = reinterpret_cast<const E *>(a.w) + (int64_t)v * a.w_pitch;
+            float s = a.bias ? a.bias[v] : 0.0f;
+#pragma unroll 4
+            for (int k = 0; k * per < a.d; ++k) {
+                E word[per];
+                const u4 bits = load_word<TY>(w, k, a.d, a.w_vec);
+                __builtin_memcpy(word, &bits, 16);
+#pragma unroll
+                for (int j = 0; j < per; ++j) s = __builtin_fmaf(x[k * per + j], (float)word[j], s);
+            }
+            if (!(s >= floor)) continue;
+            double exact = 0.0;
+            for (int k = 0; k < a.d; ++k) exact = __builtin_fma((double)x[k], (double)(float)w[k], exact);
+            if (a.bias) exact += (double)a.bias[v];
+            if (exact > best) best = exact, label = v;
         }
         top[threadIdx.x] = best, at[threadIdx.x] = label;
         for (int step = kThreads / 2; step > 0; step >>= 1) {
@@ -369,6 +398,7 @@ template <class TY> __global__ __launch_bounds__(kThreads) void k_label_near(Lab
         if (threadIdx.x == 0 && at[0] != 0x7fffffff) a.label[row] = at[0];
     }
 }
+static_assert(kThreads == DST_MAX_CHANNELS, "a thread a channel");
 
 // ---- backward -------------------------------------------------------------------------------------------------------
 // dx: rays as own rows, the table streamed.
@@ -491,13 +521,13 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     fetch(first);
     Own<TY, NK, QB> own;
     own.load([&](int i) { return row_of<TY, NK>(a.w, row0 + i, a.labels, a.w_pitch); }, a.d, a.w_vec);
-    float bias[QB], db[QB];
+    float bias[QB], db[QB], db_low[QB];   // (a sum over all rays: with what its additions lost)
     f4 out[QB][NM];
 #pragma unroll
     for (int q = 0; q < QB; ++q) {
         const int v = row0 + q * 16 + (lane & 15);
         bias[q] = a.bias && v < a.labels ? a.bias[v] : 0.0f;
-        db[q] = 0.0f;
+        db[q] = db_low[q] = 0.0f;
 #pragma unroll
         for (int m = 0; m < NM; ++m) out[q][m] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
@@ -530,9 +560,15 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
                         e -= labels[r] == v ? 1.0f : 0.0f;
                         e *= up[r];
                         p[j][q][r] = e;
-                        db[q] += e;
                     }
                 }
+            }
+#pragma unroll
+            for (int q = 0; q < QB; ++q) {
+                const f4 e = p[0][q] + p[1][q];
+                const float more = ((e[0] + e[1]) + (e[2] + e[3])) - db_low[q], to = db[q] + more;
+                db_low[q] = (to - db[q]) - more;
+                db[q] = to;
             }
             accumulate<TY, NK, QB, NM>(tile, pair, p[0], p[1], out);
         }
@@ -549,7 +585,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
 #pragma unroll
         for (int m = 0; m < NM; ++m) {
             if (a.splits > 1) store_four(a.out_part + ((int64_t)split * a.labels + v) * a.d, m * 16 + 4 * g, a.d, out[q][m], four);
-            else store_four(reinterpret_cast<E *>(a.out) + (int64_t)v * a.d, m * 16 + 4 * g, a.d, out[q][m], four);
+            else if (a.out) store_four(reinterpret_cast<E *>(a.out) + (int64_t)v * a.d, m * 16 + 4 * g, a.d, out[q][m], four);
         }
     }
 }
@@ -611,13 +647,15 @@ template <class F> int with_type(const DstLabelParams *p, F f) {
 
 struct ForwardPlan {
     Split split;
+    bool few;
     int64_t tiles, blocks;   // own tiles; blocks that leave a sum
     uint64_t bytes;
 };
 template <class TY, int NK> ForwardPlan forward_plan(const DstLabelParams *p, bool best, char *base, LabelArgs *a) {
     typedef Shapes<TY, NK> S;
     ForwardPlan f;
-    f.tiles = div_up(p->rays, S::kForward);
+    f.few = few_rows(p->rays, S::kForward, div_up(p->labels, S::kTile));
+    f.tiles = div_up(p->rays, f.few ? kWaves * 16 : S::kForward);
     f.split = split_tiles(f.tiles, div_up(p->labels, S::kTile));
     f.blocks = f.split.splits > 1 ? div_up(p->rays, kThreads) : f.tiles;
     Carve c = {base, 0};
@@ -633,6 +671,7 @@ template <class TY, int NK> ForwardPlan forward_plan(const DstLabelParams *p, bo
         a->bounds = c.take<float>(2 * kBoundBlocks);
         a->near_count = c.take<uint32_t>(1);
         a->near_list = c.take<uint32_t>(p->rays);
+        a->near_floor = c.take<float>(p->rays);
     } else if (p->reduction != DST_REDUCE_NONE) {
         a->sums = c.take<double>(f.blocks);
         a->counts = c.take<uint32_t>(f.blocks);
@@ -643,6 +682,7 @@ template <class TY, int NK> ForwardPlan forward_plan(const DstLabelParams *p, bo
 
 struct BackwardPlan {
     Split split;
+    bool few;
     int64_t tiles;
     uint64_t bytes;
 };
@@ -651,7 +691,8 @@ template <class TY, int NK> BackwardPlan backward_plan(const DstLabelParams *p, 
     typedef Shapes<TY, NK> S;
     const int64_t own = dx ? p->rays : p->labels, streamed = dx ? p->labels : p->rays;
     BackwardPlan b;
-    b.tiles = div_up(own, S::kBackward);
+    b.few = few_rows(own, S::kBackward, div_up(streamed, S::kTile));
+    b.tiles = div_up(own, b.few ? kWaves * 16 : S::kBackward);
     b.split = split_tiles(b.tiles, div_up(streamed, S::kTile));
     Carve c = {base, 0};
     LabelArgs unused = {};
@@ -709,7 +750,9 @@ int dst_label_loss_forward(const DstLabelParams *p, void *stream) {
         if (p->reduction == DST_REDUCE_NONE) a.rows = p->loss;
         const hipStream_t s = (hipStream_t)stream;
         if (f.tiles > 0) {
-            k_label_forward<TY, NK, forward_blocks<TY, NK>(), false><<<dim3((uint32_t)(f.tiles * a.splits)), kThreads, 0, s>>>(a);
+            const dim3 grid((uint32_t)(f.tiles * a.splits));
+            if (f.few) k_label_forward<TY, NK, 1, false><<<grid, kThreads, 0, s>>>(a);
+            else k_label_forward<TY, NK, forward_blocks<TY, NK>(), false><<<grid, kThreads, 0, s>>>(a);
             DST_OP_LAUNCH("label loss");
             if (a.splits > 1) {
                 k_label_join<false><<<dim3((uint32_t)f.blocks), kThreads, 0, s>>>(a);
@@ -747,13 +790,14 @@ int dst_label_loss_backward(const DstLabelParams *p, void *stream) {
             a.inverse = a.upstream_rows ? nullptr : p->inverse;
             a.out = dx ? p->grad_features : p->grad_weight, a.bias_out = p->grad_bias;
             const dim3 grid((uint32_t)(b.tiles * a.splits));
-            if (dx) k_label_dx<TY, NK, QB><<<grid, kThreads, 0, s>>>(a);
+            if (dx && b.few) k_label_dx<TY, NK, 1><<<grid, kThreads, 0, s>>>(a);
+            else if (dx) k_label_dx<TY, NK, QB><<<grid, kThreads, 0, s>>>(a);
+            else if (b.few) k_label_dw<TY, NK, 1><<<grid, kThreads, 0, s>>>(a);
             else k_label_dw<TY, NK, QB><<<grid, kThreads, 0, s>>>(a);
             DST_OP_LAUNCH("label gradient");
             if (a.splits > 1) {
                 const int64_t n = (dx ? p->rays : (int64_t)p->labels) * p->channels;
-                if (a.out) k_sum_parts<E><<<dim3(sum_blocks(n)), 256, 0, s>>>(a.out_part, (E *)a.out, n, a.splits);
-                if (!dx && p->grad_bias) k_sum_parts<float><<<dim3(sum_blocks(p->labels)), 256, 0, s>>>(a.bias_part, p->grad_bias, p->labels, a.splits);
+                sum_parts(a.out_part, (E *)a.out, n, a.bias_part, dx ? nullptr : p->grad_bias, p->labels, a.splits, s);
                 DST_OP_LAUNCH("label gradient, summing");
             }
         }
@@ -776,7 +820,9 @@ int dst_label_best(const DstLabelParams *p, void *stream) {
         a.label = p->best, a.log_prob = p->log_prob;
         const hipStream_t s = (hipStream_t)stream;
         k_label_bounds<TY><<<kBoundBlocks, kThreads, 0, s>>>(a, const_cast<float *>(a.bounds));
-        k_label_forward<TY, NK, forward_blocks<TY, NK>(), true><<<dim3((uint32_t)(f.tiles * a.splits)), kThreads, 0, s>>>(a);
+        const dim3 grid((uint32_t)(f.tiles * a.splits));
+        if (f.few) k_label_forward<TY, NK, 1, true><<<grid, kThreads, 0, s>>>(a);
+        else k_label_forward<TY, NK, forward_blocks<TY, NK>(), true><<<grid, kThreads, 0, s>>>(a);
         DST_OP_LAUNCH("best label");
         if (a.splits > 1) k_label_join<true><<<dim3((uint32_t)f.blocks), kThreads, 0, s>>>(a);
         // (as many workgroups as the device holds; each takes rays off the list until there are no more)
