@@ -10,19 +10,15 @@
 // rows are split over workgroups and joined by a closing kernel.
 #include <type_traits>
 
-#include "tiles.inc"
-
 #include "operators.h"
 
 namespace {
 
 struct AttendArgs {
-    const void *q, *k, *v;
-    int64_t qs[3], ks[3], vs[3];   // strides in values: batch, row, head
+    Rows q, k, v, o, up;           // o: out as the backward pass reads it; up: its gradient
     const int32_t *lengths;
     int32_t queries, memory, heads, kv_heads, group, rows;   // rows = queries * group
     int32_t d, dv;
-    int32_t q_vec, k_vec, v_vec, o_vec;
     int32_t splits, per_split;
     int32_t tiles;                 // of own rows, of one kv head of one batch
     float scale, c;                // c: what brings a product of rows to a score in units of log 2, but for what own rows carry
@@ -30,7 +26,6 @@ struct AttendArgs {
     int32_t flip;                  // 16-bit rows
     void *out;
     float *lse2, *delta;
-    const void *up;                // upstream gradient, contiguous like out
     void *dq, *dk, *dvalue;        // contiguous
     float2 *part;                  // (splits, batch * kv_heads * rows): maximum and sum
     float *out_part, *out_part2;   // (splits, ...) sums of a split pass
@@ -56,18 +51,10 @@ __device__ inline Place place_of(const AttendArgs &a) {
     return p;
 }
 
-template <class E> __device__ inline const E *query_row(const AttendArgs &a, const Place &p, int row) {
-    if (row >= a.rows) return nullptr;
-    const int query = a.group == 1 ? row : (int)((uint32_t)row / (uint32_t)a.group), head = p.kv * a.group + row - query * a.group;
-    return reinterpret_cast<const E *>(a.q) + p.batch * a.qs[0] + query * a.qs[1] + head * a.qs[2];
-}
-// Rows of out, its gradient and dq (contiguous: batch, query, head): the offset in rows.
+// Where a row of out and dq is written (contiguous: batch, query, head): the offset in rows.
 __device__ inline int64_t out_row(const AttendArgs &a, const Place &p, int row) {
     const int query = a.group == 1 ? row : (int)((uint32_t)row / (uint32_t)a.group), head = p.kv * a.group + row - query * a.group;
     return ((int64_t)p.batch * a.queries + query) * a.heads + head;
-}
-template <class E> __device__ inline const E *memory_row(const void *base, const int64_t (&s)[3], const Place &p, int row, int last) {
-    return row < last ? reinterpret_cast<const E *>(base) + p.batch * s[0] + row * s[1] + p.kv * s[2] : nullptr;
 }
 // Row of lse, delta and the parts
 __device__ inline int64_t stat_row(const AttendArgs &a, const Place &p, int row) { return ((int64_t)p.batch * a.kv_heads + p.kv) * a.rows + row; }
@@ -78,7 +65,7 @@ template <class TY, int NK, int QB> __device__ inline void carry_scale(Own<TY, N
 #pragma unroll
     for (int q = 0; q < QB; ++q)
 #pragma unroll
-        for (int k = 0; k < NK; ++k) {
+        for (int k = 0; k < fragments<NK>(); ++k) {
             if constexpr (TY::kSize == 4) own.f[q][k] = __builtin_bit_cast(u4, __builtin_bit_cast(f4, own.f[q][k]) * a.own_scale);
             else if (a.flip) own.f[q][k] ^= u4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
         }
@@ -92,22 +79,25 @@ constexpr float kSlack = 8.0f;
 template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void k_attend_forward(AttendArgs a) {
     typedef TileShape<NK> T;
     typedef typename TY::E E;
-    constexpr int NM = T::kBytes / TY::kSize / 16;
+    constexpr int NM = depth_blocks<TY, NK>();
     __shared__ alignas(16) char tile_k[T::kRows * T::kPitch], tile_v[T::kRows * T::kPitch];
+    __shared__ alignas(16) float tile_mask[T::kRows];   // 0, or -inf of a row behind the length, which takes it out of every sum
     const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6;
     const Place p = place_of(a);
     const int row0 = p.tile * (kWaves * 16 * QB) + wave * 16 * QB;
     const int first = p.split * a.per_split * T::kRows;
     const int last = min(p.length, first + a.per_split * T::kRows);
 
-    Stage<TY, NK> stage_k, stage_v;
+    Stage<NK> stage_k, stage_v;
+    stage_k.begin(a.k);
+    stage_v.begin(a.v);
     auto fetch = [&](int at) {
-        stage_k.load([&](int i) { return memory_row<E>(a.k, a.ks, p, at + i, last); }, a.d, a.k_vec);
-        stage_v.load([&](int i) { return memory_row<E>(a.v, a.vs, p, at + i, last); }, a.dv, a.v_vec);
+        stage_k.load(tile_base(a.k, at, p.batch, p.kv), last - at);
+        stage_v.load(tile_base(a.v, at, p.batch, p.kv), last - at);
     };
     if (first < last) fetch(first);
     Own<TY, NK, QB> own;
-    own.load([&](int i) { return query_row<E>(a, p, row0 + i); }, a.d, a.q_vec);
+    own.load(a.q, tile_base(a.q, row0, p.batch, p.kv), a.rows - row0);
     carry_scale(own, a);
     float m[QB], l[QB];
     f4 out[QB][NM];
@@ -120,6 +110,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     for (int at = first; at < last; at += T::kRows) {
         stage_k.store(tile_k);
         stage_v.store(tile_v);
+        if ((int)threadIdx.x < T::kRows) tile_mask[threadIdx.x] = at + (int)threadIdx.x < last ? 0.0f : -kInf;
         __syncthreads();
         if (at + T::kRows < last) fetch(at + T::kRows);
 #pragma unroll
@@ -127,18 +118,10 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
             f4 s[2][QB];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
+                const f4 mask = *reinterpret_cast<const f4 *>(tile_mask + (pair + j) * 16 + 4 * g);
 #pragma unroll
-                for (int q = 0; q < QB; ++q) s[j][q] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int q = 0; q < QB; ++q) s[j][q] = mask;
                 product<TY, NK, QB>(tile_k, pair + j, own, s[j]);
-            }
-            if (at + T::kRows > last) {
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (at + (pair + j) * 16 + 4 * g + r >= last)
-#pragma unroll
-                            for (int q = 0; q < QB; ++q) s[j][q][r] = -kInf;
             }
             float top[QB];
             bool raise = false;
@@ -294,7 +277,7 @@ template <class TY, int NK, int QB> __device__ inline void deltas(const Own<TY, 
     for (int q = 0; q < QB; ++q) {
         f4 s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int k = 0; k < NK; ++k) s = TY::mma(o.f[q][k], up.f[q][k], s);
+        for (int k = 0; k < fragments<NK>(); ++k) s = fragment_product<TY, NK>(o.f[q][k], up.f[q][k], s);
         const float mine = (l & 2) ? ((l & 1) ? s[3] : s[2]) : ((l & 1) ? s[1] : s[0]);
         delta[q] = sum_group(g == (l >> 2) ? mine : 0.0f);   // (the diagonal's one value)
     }
@@ -304,26 +287,29 @@ template <class TY, int NK, int QB> __device__ inline void deltas(const Own<TY, 
 template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void k_attend_dq(AttendArgs a) {
     typedef TileShape<NK> T;
     typedef typename TY::E E;
-    constexpr int NM = T::kBytes / TY::kSize / 16;
+    constexpr int NM = depth_blocks<TY, NK>();
     __shared__ alignas(16) char tile_k[T::kRows * T::kPitch], tile_v[T::kRows * T::kPitch];
+    __shared__ alignas(16) float tile_mask[T::kRows];   // 0, or -inf of a row behind the length, which takes it out of every sum
     const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6;
     const Place p = place_of(a);
     const int row0 = p.tile * (kWaves * 16 * QB) + wave * 16 * QB;
     const int first = p.split * a.per_split * T::kRows;
     const int last = a.dq ? min(p.length, first + a.per_split * T::kRows) : 0;
 
-    Stage<TY, NK> stage_k, stage_v;
+    Stage<NK> stage_k, stage_v;
+    stage_k.begin(a.k);
+    stage_v.begin(a.v);
     auto fetch = [&](int at) {
-        stage_k.load([&](int i) { return memory_row<E>(a.k, a.ks, p, at + i, last); }, a.d, a.k_vec);
-        stage_v.load([&](int i) { return memory_row<E>(a.v, a.vs, p, at + i, last); }, a.dv, a.v_vec);
+        stage_k.load(tile_base(a.k, at, p.batch, p.kv), last - at);
+        stage_v.load(tile_base(a.v, at, p.batch, p.kv), last - at);
     };
     if (first < last) fetch(first);
     Own<TY, NK, QB> own, up;
     float delta[QB], lse2[QB];
-    up.load([&](int i) { return row0 + i < a.rows ? reinterpret_cast<const E *>(a.up) + out_row(a, p, row0 + i) * a.dv : nullptr; }, a.dv, a.o_vec);
-    own.load([&](int i) { return row0 + i < a.rows ? reinterpret_cast<const E *>(a.out) + out_row(a, p, row0 + i) * a.dv : nullptr; }, a.dv, a.o_vec);
+    up.load(a.up, tile_base(a.up, row0, p.batch, p.kv), a.rows - row0);
+    own.load(a.o, tile_base(a.o, row0, p.batch, p.kv), a.rows - row0);
     deltas<TY, NK, QB>(own, up, delta);
-    own.load([&](int i) { return query_row<E>(a, p, row0 + i); }, a.d, a.q_vec);
+    own.load(a.q, tile_base(a.q, row0, p.batch, p.kv), a.rows - row0);
     carry_scale(own, a);
     f4 out[QB][NM];
 #pragma unroll
@@ -337,6 +323,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     for (int at = first; at < last; at += T::kRows) {
         stage_k.store(tile_k);
         stage_v.store(tile_v);
+        if ((int)threadIdx.x < T::kRows) tile_mask[threadIdx.x] = at + (int)threadIdx.x < last ? 0.0f : -kInf;
         __syncthreads();
         if (at + T::kRows < last) fetch(at + T::kRows);
 #pragma unroll
@@ -345,8 +332,9 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 f4 dp[QB];
+                const f4 mask = *reinterpret_cast<const f4 *>(tile_mask + (pair + j) * 16 + 4 * g);
 #pragma unroll
-                for (int q = 0; q < QB; ++q) s[j][q] = dp[q] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int q = 0; q < QB; ++q) s[j][q] = mask, dp[q] = f4{0.0f, 0.0f, 0.0f, 0.0f};
                 product<TY, NK, QB>(tile_k, pair + j, own, s[j]);
                 product<TY, NK, QB>(tile_v, pair + j, up, dp);
 #pragma unroll
@@ -354,15 +342,6 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
                         s[j][q][r] = exp2_of(__builtin_fmaf(s[j][q][r], a.c, -lse2[q])) * (dp[q][r] - delta[q]);
-            }
-            if (at + T::kRows > last) {   // rows behind the length: their products are with zeros, but not of anything
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (at + (pair + j) * 16 + 4 * g + r >= last)
-#pragma unroll
-                            for (int q = 0; q < QB; ++q) s[j][q][r] = 0.0f;
             }
             accumulate<TY, NK, QB, NM>(tile_k, pair, s[0], s[1], out);
         }
@@ -388,7 +367,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
 template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void k_attend_dkv(AttendArgs a) {
     typedef TileShape<NK> T;
     typedef typename TY::E E;
-    constexpr int NM = T::kBytes / TY::kSize / 16;
+    constexpr int NM = depth_blocks<TY, NK>();
     __shared__ alignas(16) char tile_q[T::kRows * T::kPitch], tile_o[T::kRows * T::kPitch];
     __shared__ alignas(16) float tile_lse2[T::kRows], tile_delta[T::kRows];
     const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6;
@@ -397,11 +376,13 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     const int first = p.split * a.per_split * T::kRows;
     const int last = tile0 < p.length ? min(a.rows, first + a.per_split * T::kRows) : 0;
 
-    Stage<TY, NK> stage_q, stage_o;
+    Stage<NK> stage_q, stage_o;
+    stage_q.begin(a.q);
+    stage_o.begin(a.up);
     float stage_lse2 = kInf, stage_delta = 0.0f;
     auto fetch = [&](int at) {
-        stage_q.load([&](int i) { return at + i < last ? query_row<E>(a, p, at + i) : nullptr; }, a.d, a.q_vec);
-        stage_o.load([&](int i) { return at + i < last ? reinterpret_cast<const E *>(a.up) + out_row(a, p, at + i) * a.dv : nullptr; }, a.dv, a.o_vec);
+        stage_q.load(tile_base(a.q, at, p.batch, p.kv), last - at);
+        stage_o.load(tile_base(a.up, at, p.batch, p.kv), last - at);
         if ((int)threadIdx.x < T::kRows) {
             const int row = at + threadIdx.x;
             stage_lse2 = row < last ? a.lse2[stat_row(a, p, row)] : kInf;
@@ -410,8 +391,8 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     };
     if (first < last) fetch(first);
     Own<TY, NK, QB> own_k, own_v;
-    own_k.load([&](int i) { return memory_row<E>(a.k, a.ks, p, row0 + i, p.length); }, a.d, a.k_vec);
-    own_v.load([&](int i) { return memory_row<E>(a.v, a.vs, p, row0 + i, p.length); }, a.dv, a.v_vec);
+    own_k.load(a.k, tile_base(a.k, row0, p.batch, p.kv), p.length - row0);
+    own_v.load(a.v, tile_base(a.v, row0, p.batch, p.kv), p.length - row0);
     carry_scale(own_k, a);
     f4 dk[QB][NM], dv[QB][NM];
 #pragma unroll
@@ -496,23 +477,12 @@ int check(const DstAttendParams *p) {
     return DST_OK;
 }
 
-bool strides_align(const void *p, const int64_t (&s)[3], int channels, int size) {
-    return words_align(p, s[0], channels, size) && words_align(p, s[1], channels, size) && words_align(p, s[2], channels, size);
-}
-
 AttendArgs arguments(const DstAttendParams *p) {
     AttendArgs a = {};
-    const int size = value_size(p->dtype);
-    a.q = p->q, a.k = p->k, a.v = p->v;
-    for (int i = 0; i < 3; ++i) a.qs[i] = p->q_strides[i], a.ks[i] = p->k_strides[i], a.vs[i] = p->v_strides[i];
     a.lengths = p->lengths;
     a.queries = p->queries, a.memory = p->memory, a.heads = p->heads, a.kv_heads = p->kv_heads;
     a.group = p->heads / p->kv_heads, a.rows = p->queries * a.group;
     a.d = p->channels, a.dv = p->value_channels;
-    a.q_vec = strides_align(p->q, p->q_strides, p->channels, size);
-    a.k_vec = strides_align(p->k, p->k_strides, p->channels, size);
-    a.v_vec = strides_align(p->v, p->v_strides, p->value_channels, size);
-    a.o_vec = words_align(p->out, 0, p->value_channels, size) && words_align(p->upstream, 0, p->value_channels, size);
     a.scale = p->scale, a.flip = p->scale < 0.0f;
     // (a scale of 0 stands for all scores equal: the smallest normal number says that of any score that is finite, and leaves
     // -inf what it is)
@@ -527,6 +497,8 @@ AttendArgs arguments(const DstAttendParams *p) {
 
 template <class TY, class F> int with_fragments(int nk, F f) {
     switch (nk) {
+        case 0:
+            if constexpr (TY::kSize == 4) return f(TY{}, std::integral_constant<int, 0>{});
         case 1: return f(TY{}, std::integral_constant<int, 1>{});
         case 2: return f(TY{}, std::integral_constant<int, 2>{});
         case 4: return f(TY{}, std::integral_constant<int, 4>{});
@@ -558,31 +530,57 @@ template <class TY, int NK> int dkv_rows(const AttendArgs &a, int64_t heads) {
     return kWaves * 16 * blocks_for(dkv_blocks<TY, NK>(), a.memory, heads, TileShape<NK>::kRows, a.rows);
 }
 
-uint64_t plan_forward(AttendArgs &a, int own, int tile, int64_t heads, char *base) {
+// The rows of all sets, copied into the workspace's front where the kernels cannot read them where they lie.
+struct Sets {
+    RowSet q, k, v, o, up;
+};
+template <int NK> Sets row_sets(const DstAttendParams *p, AttendArgs &a, bool backward, Carve &c) {
+    // (a group has to fit whole into the steps between a thread's words, and into the blocks of 16 own rows)
+    const int stride = TileShape<NK>::kStride < 16 ? TileShape<NK>::kStride : 16, group = a.group;
+    auto memory = [&](const void *t, const int64_t (&s)[3], int channels) {
+        return row_set(t, s[0], s[1], s[2], p->batch, p->kv_heads, 1, p->memory, channels, p->dtype, stride, c);
+    };
+    auto queries = [&](const void *t, int64_t batch, int64_t row, int64_t head, int channels) {
+        return row_set(t, batch, row, head, p->batch, p->kv_heads, group, a.rows, channels, p->dtype, stride, c);
+    };
+    const int64_t row = (int64_t)p->heads * p->value_channels;
+    Sets s = {};
+    s.q = queries(p->q, p->q_strides[0], p->q_strides[1], p->q_strides[2], p->channels);
+    s.k = memory(p->k, p->k_strides, p->channels);
+    s.v = memory(p->v, p->v_strides, p->value_channels);
+    if (backward) {
+        s.o = queries(p->out, p->queries * row, row, p->value_channels, p->value_channels);
+        s.up = queries(p->upstream, p->queries * row, row, p->value_channels, p->value_channels);
+    }
+    a.q = s.q.rows, a.k = s.k.rows, a.v = s.v.rows, a.o = s.o.rows, a.up = s.up.rows;
+    return s;
+}
+void prepare(const Sets &s, hipStream_t stream) {
+    for (const RowSet *r : {&s.q, &s.k, &s.v, &s.o, &s.up}) prepare(*r, stream);
+}
+
+uint64_t plan_forward(AttendArgs &a, int own, int tile, int64_t heads, Carve c) {
     a.tiles = (int)div_up(a.rows, own);
     const Split s = split_tiles(a.tiles * heads, div_up(a.memory, tile));
     a.splits = s.splits, a.per_split = s.per_split;
-    Carve c = {base, 0};
     if (a.splits > 1) {
         a.part = c.take<float2>((uint64_t)a.splits * a.all_rows);
         a.out_part = c.take<float>((uint64_t)a.splits * a.all_rows * a.dv);
     }
     return c.used;
 }
-uint64_t plan_dq(AttendArgs &a, int own, int tile, int64_t heads, char *base) {
+uint64_t plan_dq(AttendArgs &a, int own, int tile, int64_t heads, Carve c) {
     a.tiles = (int)div_up(a.rows, own);
     const Split s = a.dq ? split_tiles(a.tiles * heads, div_up(a.memory, tile)) : Split{1, 1};
     a.splits = s.splits, a.per_split = s.per_split;
-    Carve c = {base, 0};
     a.delta = c.take<float>(a.all_rows);
     if (a.splits > 1) a.out_part = c.take<float>((uint64_t)a.splits * a.all_rows * a.d);
     return c.used;
 }
-uint64_t plan_dkv(AttendArgs &a, int own, int tile, int64_t heads, char *base) {
+uint64_t plan_dkv(AttendArgs &a, int own, int tile, int64_t heads, Carve c) {
     a.tiles = (int)div_up(a.memory, own);
     const Split s = split_tiles(a.tiles * heads, div_up(a.rows, tile));
     a.splits = s.splits, a.per_split = s.per_split;
-    Carve c = {base, 0};
     a.delta = c.take<float>(a.all_rows);
     if (a.splits > 1) {
         const uint64_t rows = (uint64_t)a.splits * heads * a.memory;
@@ -613,13 +611,15 @@ uint64_t dst_attend_workspace_bytes(const DstAttendParams *p, int pass) {
         AttendArgs a = arguments(p);
         const int64_t heads = (int64_t)p->batch * p->kv_heads;
         if (a.all_rows == 0 && pass == DST_PASS_FORWARD) return DST_OK;
+        Carve c = {nullptr, 0};
+        row_sets<NK>(p, a, pass != DST_PASS_FORWARD, c);
         if (pass == DST_PASS_FORWARD) {
-            bytes = plan_forward(a, forward_rows<TY, NK>(a, heads), TileShape<NK>::kRows, heads, nullptr);
+            bytes = plan_forward(a, forward_rows<TY, NK>(a, heads), TileShape<NK>::kRows, heads, c);
         } else {
             a.dq = p->grad_q;
-            bytes = plan_dq(a, dq_rows<TY, NK>(a, heads), TileShape<NK>::kRows, heads, nullptr);
+            bytes = plan_dq(a, dq_rows<TY, NK>(a, heads), TileShape<NK>::kRows, heads, c);
             if (p->grad_k || p->grad_v) {
-                const uint64_t more = plan_dkv(a, dkv_rows<TY, NK>(a, heads), TileShape<NK>::kRows, heads, nullptr);
+                const uint64_t more = plan_dkv(a, dkv_rows<TY, NK>(a, heads), TileShape<NK>::kRows, heads, c);
                 bytes = more > bytes ? more : bytes;
             }
         }
@@ -638,9 +638,12 @@ int dst_attend_forward(const DstAttendParams *p, void *stream) {
         if (a.all_rows == 0) return (int)DST_OK;
         const int64_t heads = (int64_t)p->batch * p->kv_heads;
         const int own = forward_rows<TY, NK>(a, heads);
-        const uint64_t need = plan_forward(a, own, TileShape<NK>::kRows, heads, (char *)p->workspace);
+        Carve c = {(char *)p->workspace, 0};
+        const Sets sets = row_sets<NK>(p, a, false, c);
+        const uint64_t need = plan_forward(a, own, TileShape<NK>::kRows, heads, c);
         if (int rc = check_workspace(p, need)) return rc;
         const hipStream_t s = (hipStream_t)stream;
+        prepare(sets, s);
         const dim3 grid((uint32_t)(a.tiles * heads * a.splits));
         if (own == kWaves * 16) k_attend_forward<TY, NK, 1><<<grid, kThreads, 0, s>>>(a);
         else k_attend_forward<TY, NK, QB><<<grid, kThreads, 0, s>>>(a);
@@ -671,11 +674,14 @@ int dst_attend_backward(const DstAttendParams *p, void *stream) {
         const hipStream_t s = (hipStream_t)stream;
         const int64_t heads = (int64_t)p->batch * p->kv_heads;
         AttendArgs a = arguments(p);
-        a.up = p->upstream, a.dq = p->grad_q, a.dk = p->grad_k, a.dvalue = p->grad_v;
+        Carve c = {(char *)p->workspace, 0};
+        const Sets sets = row_sets<NK>(p, a, true, c);
+        a.dq = p->grad_q, a.dk = p->grad_k, a.dvalue = p->grad_v;
         if (a.all_rows > 0) {
             const int own = dq_rows<TY, NK>(a, heads);
-            const uint64_t need = plan_dq(a, own, tile, heads, (char *)p->workspace);
+            const uint64_t need = plan_dq(a, own, tile, heads, c);
             if (int rc = check_workspace(p, need)) return rc;
+            prepare(sets, s);
             const dim3 grid((uint32_t)(a.tiles * heads * a.splits));
             if (own == kWaves * 16) k_attend_dq<TY, NK, 1><<<grid, kThreads, 0, s>>>(a);
             else k_attend_dq<TY, NK, dq_blocks<TY, NK>()><<<grid, kThreads, 0, s>>>(a);
@@ -687,7 +693,7 @@ int dst_attend_backward(const DstAttendParams *p, void *stream) {
         }
         if ((a.dk || a.dvalue) && heads * a.memory > 0) {
             const int own = dkv_rows<TY, NK>(a, heads);
-            const uint64_t need = plan_dkv(a, own, tile, heads, (char *)p->workspace);
+            const uint64_t need = plan_dkv(a, own, tile, heads, c);
             if (int rc = check_workspace(p, need)) return rc;
             a.own_all = heads * a.memory;
             const dim3 grid((uint32_t)(a.tiles * heads * a.splits));

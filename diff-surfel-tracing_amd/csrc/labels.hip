@@ -10,21 +10,17 @@
 // adds the parts.
 #include <type_traits>
 
-#include "tiles.inc"
-
 #include "operators.h"
 
 namespace {
 
 // ---- launch parameters as the kernels take them -------------------------------------------------------------------
 struct LabelArgs {
-    const void *x, *w;
+    Rows x, w;
     const float *bias;              // (labels) or nullptr
     const int64_t *target;          // (rays)
-    int64_t x_pitch, w_pitch;       // values from one row to the next
     int64_t rays, ignore;
     int32_t d, labels;
-    int32_t x_vec, w_vec;           // rows can be read in 16-byte words
     int32_t splits, per_split;      // parts of the streamed rows; tiles of each
     // forward
     float2 *part;                   // (splits, rays): maximum and sum, in units of log 2
@@ -57,10 +53,6 @@ constexpr int kBoundBlocks = 64;
 template <class TY, int NK> constexpr int forward_blocks() { return NK <= 4 ? 4 : NK <= 8 ? 2 : 1; }
 template <class TY, int NK> constexpr int backward_blocks() {
     return NK * (TY::kSize == 2 ? 12 : 8) <= 32 ? 4 : NK * (TY::kSize == 2 ? 12 : 8) <= 96 ? 2 : 1;
-}
-
-template <class TY, int NK> __device__ inline const typename TY::E *row_of(const void *base, int64_t row, int64_t rows, int64_t pitch) {
-    return row < rows ? reinterpret_cast<const typename TY::E *>(base) + row * pitch : nullptr;
 }
 
 // The upstream gradient of a ray's loss: 0 where it is ignored, NaN where its label is none.
@@ -150,15 +142,16 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
     const int first = split * a.per_split * T::kRows;
     const int last = min(a.labels, (split + 1) * a.per_split * T::kRows);   // (the host keeps labels + a tile below 2^31)
 
-    Stage<TY, NK> stage;
-    float stage_bias = 0.0f;
+    Stage<NK> stage;
+    stage.begin(a.w);
+    float stage_bias = 0.0f;   // of a row behind the table's end: -inf, which takes it out of every sum
     auto fetch = [&](int at) {
-        stage.load([&](int i) { return row_of<TY, NK>(a.w, at + i, last, a.w_pitch); }, a.d, a.w_vec);
-        if ((int)threadIdx.x < T::kRows && a.bias) stage_bias = at + (int)threadIdx.x < last ? a.bias[at + threadIdx.x] : 0.0f;
+        stage.load(tile_base(a.w, at), last - at);
+        if ((int)threadIdx.x < T::kRows) stage_bias = at + (int)threadIdx.x >= last ? -kInf : a.bias ? a.bias[at + threadIdx.x] : 0.0f;
     };
     fetch(first);
     Own<TY, NK, QB> own;
-    own.load([&](int i) { return row_of<TY, NK>(a.x, row0 + i, a.rays, a.x_pitch); }, a.d, a.x_vec);
+    own.load(a.x, tile_base(a.x, row0), (int)min(a.rays - row0, (int64_t)(16 * QB)));
 
     Running run[QB];
     float best[QB], second[QB];
@@ -180,15 +173,6 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
 #pragma unroll
                 for (int q = 0; q < QB; ++q) s[j][q] = b;
                 product<TY, NK, QB>(tile, pair + j, own, s[j]);
-            }
-            if (at + T::kRows > last) {   // rows behind the table's end
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (at + (pair + j) * 16 + 4 * g + r >= last)
-#pragma unroll
-                            for (int q = 0; q < QB; ++q) s[j][q][r] = -kInf;
             }
 #pragma unroll
             for (int q = 0; q < QB; ++q) {
@@ -235,7 +219,7 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
         if constexpr (BEST) {
             float norm = 0.0f;
 #pragma unroll
-            for (int k = 0; k < NK; ++k) norm += dot_word<TY>(own.f[q][k], own.f[q][k]);
+            for (int k = 0; k < fragments<NK>(); ++k) norm += dot_word<TY>(own.f[q][k], own.f[q][k]);
             norm = sqrtf(sum_group(norm));
 #pragma unroll
             for (int step = 16; step <= 32; step <<= 1)
@@ -256,8 +240,8 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
                 const int64_t t = row < a.rays ? a.target[row] : -1;
                 const bool there = t >= 0 && t < a.labels;
 #pragma unroll
-                for (int k = 0; k < NK; ++k)
-                    if (there) logit += dot_word<TY>(own.f[q][k], load_word<TY>(row_of<TY, NK>(a.w, t, a.labels, a.w_pitch), k * 4 + g, a.d, a.w_vec));
+                for (int k = 0; k < fragments<NK>(); ++k)
+                    logit += dot_word<TY>(own.f[q][k], own_word<NK>(there ? tile_base(a.w, t) : nullptr, k, a.w.words));
                 logit = sum_group(logit);
                 if (there && a.bias) logit += a.bias[t];
             }
@@ -328,7 +312,7 @@ template <class TY> __global__ __launch_bounds__(kThreads) void k_label_bounds(L
     const int lane = threadIdx.x & 63;
     float wide = 0.0f, tall = 0.0f;
     for (int64_t v = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6); v < a.labels; v += (int64_t)kBoundBlocks * kWaves) {
-        const typename TY::E *w = reinterpret_cast<const typename TY::E *>(a.w) + v * a.w_pitch;
+        const typename TY::E *w = reinterpret_cast<const typename TY::E *>(tile_base(a.w, v));
         float n = 0.0f;
         for (int i = lane; i < a.d; i += 64) n = __builtin_fmaf((float)w[i], (float)w[i], n);
         for (int step = 32; step > 0; step >>= 1) n += __shfl_xor(n, step);
@@ -363,20 +347,19 @@ template <class TY> __global__ __launch_bounds__(kThreads) void k_label_near(Lab
     for (uint32_t i = blockIdx.x; i < n; i += gridDim.x) {
         const int64_t row = a.near_list[i];
         const float floor = a.near_floor[i];
-        const E *xr = reinterpret_cast<const E *>(a.x) + row * a.x_pitch;
+        const E *xr = reinterpret_cast<const E *>(tile_base(a.x, row));
         __syncthreads();
         x[threadIdx.x] = (int)threadIdx.x < a.d ? (float)xr[threadIdx.x] : 0.0f;
         __syncthreads();
         double best = -__builtin_huge_val();
         int label = 0x7fffffff;
         for (int v = threadIdx.x; v < a.labels; v += kThreads) {
-            const E *w = reinterpret_cast<const E *>(a.w) + (int64_t)v * a.w_pitch;
+            const E *w = reinterpret_cast<const E *>(tile_base(a.w, v));
             float s = a.bias ? a.bias[v] : 0.0f;
 #pragma unroll 4
-            for (int k = 0; k * per < a.d; ++k) {
+            for (int k = 0; k < a.w.words; ++k) {
                 E word[per];
-                const u4 bits = load_word<TY>(w, k, a.d, a.w_vec);
-                __builtin_memcpy(word, &bits, 16);
+                __builtin_memcpy(word, w + k * per, 16);
 #pragma unroll
                 for (int j = 0; j < per; ++j) s = __builtin_fmaf(x[k * per + j], (float)word[j], s);
             }
@@ -404,7 +387,7 @@ static_assert(kThreads == DST_MAX_CHANNELS, "a thread a channel");
 // dx: rays as own rows, the table streamed.
 template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void k_label_dx(LabelArgs a) {
     typedef TileShape<NK> T;
-    constexpr int NM = T::kBytes / TY::kSize / 16;
+    constexpr int NM = depth_blocks<TY, NK>();
     __shared__ alignas(16) char tile[T::kRows * T::kPitch];
     __shared__ alignas(16) float tile_bias[T::kRows];
     const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6;
@@ -413,15 +396,16 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     const int first = split * a.per_split * T::kRows;
     const int last = min(a.labels, (split + 1) * a.per_split * T::kRows);
 
-    Stage<TY, NK> stage;
-    float stage_bias = 0.0f;
+    Stage<NK> stage;
+    stage.begin(a.w);
+    float stage_bias = 0.0f;   // of a row behind the table's end: -inf, which takes it out of every sum
     auto fetch = [&](int at) {
-        stage.load([&](int i) { return row_of<TY, NK>(a.w, at + i, last, a.w_pitch); }, a.d, a.w_vec);
-        if ((int)threadIdx.x < T::kRows && a.bias) stage_bias = at + (int)threadIdx.x < last ? a.bias[at + threadIdx.x] : 0.0f;
+        stage.load(tile_base(a.w, at), last - at);
+        if ((int)threadIdx.x < T::kRows) stage_bias = at + (int)threadIdx.x >= last ? -kInf : a.bias ? a.bias[at + threadIdx.x] : 0.0f;
     };
     fetch(first);
     Own<TY, NK, QB> own;
-    own.load([&](int i) { return row_of<TY, NK>(a.x, row0 + i, a.rays, a.x_pitch); }, a.d, a.x_vec);
+    own.load(a.x, tile_base(a.x, row0), (int)min(a.rays - row0, (int64_t)(16 * QB)));
     float lse2[QB], up[QB];
     int label[QB];   // relative to the lane's first row of a tile
     f4 out[QB][NM];
@@ -458,15 +442,6 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
                         p[j][q][r] = e;
                     }
             }
-            if (at + T::kRows > last) {   // rows behind the table's end: their products are with zeros, but not of anything
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (at + (pair + j) * 16 + 4 * g + r >= last)
-#pragma unroll
-                            for (int q = 0; q < QB; ++q) p[j][q][r] = 0.0f;
-            }
             accumulate<TY, NK, QB, NM>(tile, pair, p[0], p[1], out);
         }
         __syncthreads();
@@ -490,27 +465,23 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
 // dw and db: labels as own rows, the rays streamed.
 template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void k_label_dw(LabelArgs a) {
     typedef TileShape<NK> T;
-    constexpr int NM = T::kBytes / TY::kSize / 16;
+    constexpr int NM = depth_blocks<TY, NK>();
     __shared__ alignas(16) char tile[T::kRows * T::kPitch];
-    __shared__ alignas(16) float tile_lse2[T::kRows], tile_up[T::kRows];
-    __shared__ alignas(16) int tile_label[T::kRows];
+    __shared__ alignas(16) float tile_lse2[2][T::kRows], tile_up[2][T::kRows];
+    __shared__ alignas(16) int tile_label[2][T::kRows];
     const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6;
     const int split = blockIdx.x % a.splits;
     const int row0 = (int)(blockIdx.x / a.splits) * (kWaves * 16 * QB) + wave * 16 * QB;   // (the host keeps labels + a tile below 2^31)
     const int64_t first = (int64_t)split * a.per_split * T::kRows;
     const int64_t last = min(a.rays, first + (int64_t)a.per_split * T::kRows);
 
-    Stage<TY, NK> stage;
-    float alive[T::kChunks];   // lse2 of the word's ray: +inf where it is ignored, whose channels may hold anything
+    Stage<NK> stage;
+    stage.begin(a.x);
+    // Of every ray: lse (+inf where it is ignored or behind the end, which makes its weights 0), upstream gradient, label. They are a tile
+    // ahead of the channels, which are read only of rays that are not ignored: those of the others may hold anything.
     float stage_lse2 = kInf, stage_up = 0.0f;
     int stage_label = -1;
-    auto fetch = [&](int64_t at) {
-        stage.load([&](int i) { return row_of<TY, NK>(a.x, at + i, last, a.x_pitch); }, a.d, a.x_vec);
-#pragma unroll
-        for (int c = 0; c < T::kChunks; ++c) {
-            const int64_t row = at + ((int)threadIdx.x + c * kThreads) / (T::kBytes / 16);
-            alive[c] = row < last ? a.lse2[row] : kInf;
-        }
+    auto fetch_stats = [&](int64_t at) {
         if ((int)threadIdx.x < T::kRows) {
             const int64_t row = at + threadIdx.x, t = row < last ? a.target[row] : a.ignore;
             stage_lse2 = row < last ? a.lse2[row] : kInf;
@@ -518,9 +489,19 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
             stage_label = t >= 0 && t < a.labels && t != a.ignore ? (int)t : -1;
         }
     };
-    fetch(first);
+    auto store_stats = [&](int at) {
+        if ((int)threadIdx.x < T::kRows) tile_lse2[at][threadIdx.x] = stage_lse2, tile_up[at][threadIdx.x] = stage_up, tile_label[at][threadIdx.x] = stage_label;
+    };
+    auto fetch = [&](int64_t at, int half) {
+        stage.load(tile_base(a.x, at), (int)min(last - at, (int64_t)T::kRows), [&](int r) { return tile_lse2[half][r & (T::kRows - 1)] != kInf; });
+    };
+    fetch_stats(first);
     Own<TY, NK, QB> own;
-    own.load([&](int i) { return row_of<TY, NK>(a.w, row0 + i, a.labels, a.w_pitch); }, a.d, a.w_vec);
+    own.load(a.w, tile_base(a.w, row0), min(a.labels - row0, 16 * QB));
+    store_stats(0);
+    __syncthreads();
+    if (first < last) fetch(first, 0);
+    fetch_stats(first + T::kRows);
     float bias[QB], db[QB], db_low[QB];   // (a sum over all rays: with what its additions lost)
     f4 out[QB][NM];
 #pragma unroll
@@ -531,14 +512,15 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
 #pragma unroll
         for (int m = 0; m < NM; ++m) out[q][m] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    for (int64_t at = first; at < last; at += T::kRows) {
-#pragma unroll
-        for (int c = 0; c < T::kChunks; ++c)
-            if (alive[c] == kInf) stage.word[c] = u4{0u, 0u, 0u, 0u};
+    int half = 0;
+    for (int64_t at = first; at < last; at += T::kRows, half ^= 1) {
         stage.store(tile);
-        if ((int)threadIdx.x < T::kRows) tile_lse2[threadIdx.x] = stage_lse2, tile_up[threadIdx.x] = stage_up, tile_label[threadIdx.x] = stage_label;
+        store_stats(half ^ 1);
         __syncthreads();
-        if (at + T::kRows < last) fetch(at + T::kRows);
+        if (at + T::kRows < last) {
+            fetch(at + T::kRows, half ^ 1);
+            fetch_stats(at + 2 * T::kRows);
+        }
 #pragma unroll
         for (int pair = 0; pair < T::kBlocks; pair += 2) {
             f4 p[2][QB];
@@ -548,8 +530,8 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
                 for (int q = 0; q < QB; ++q) p[j][q] = f4{bias[q], bias[q], bias[q], bias[q]};
                 product<TY, NK, QB>(tile, pair + j, own, p[j]);
                 const int at4 = (pair + j) * 16 + 4 * g;
-                const f4 lse2 = *reinterpret_cast<const f4 *>(tile_lse2 + at4), up = *reinterpret_cast<const f4 *>(tile_up + at4);
-                const int4 label = *reinterpret_cast<const int4 *>(tile_label + at4);
+                const f4 lse2 = *reinterpret_cast<const f4 *>(tile_lse2[half] + at4), up = *reinterpret_cast<const f4 *>(tile_up[half] + at4);
+                const int4 label = *reinterpret_cast<const int4 *>(tile_label[half] + at4);
                 const int labels[4] = {label.x, label.y, label.z, label.w};
 #pragma unroll
                 for (int q = 0; q < QB; ++q) {
@@ -611,15 +593,22 @@ int check(const DstLabelParams *p) {
 
 LabelArgs arguments(const DstLabelParams *p) {
     LabelArgs a = {};
-    const int size = value_size(p->dtype);
-    a.x = p->features, a.w = p->weight, a.bias = p->bias, a.target = p->targets;
-    a.x_pitch = p->features_stride, a.w_pitch = p->weight_stride;
+    a.bias = p->bias, a.target = p->targets;
     a.rays = p->rays, a.ignore = p->ignore_index, a.d = p->channels, a.labels = p->labels;
-    a.x_vec = words_align(p->features, p->features_stride, p->channels, size);
-    a.w_vec = words_align(p->weight, p->weight_stride, p->channels, size);
     a.lse2 = p->lse;
     a.splits = a.per_split = 1;
     return a;
+}
+
+// The rows of both sets, copied into the workspace's front where the kernels cannot read them where they lie.
+struct Sets {
+    RowSet x, w;
+};
+Sets row_sets(const DstLabelParams *p, Carve &c) {
+    Sets s;
+    s.x = row_set(p->features, 0, p->features_stride, 0, 1, 1, 1, p->rays, p->channels, p->dtype, 1, c);
+    s.w = row_set(p->weight, 0, p->weight_stride, 0, 1, 1, 1, p->labels, p->channels, p->dtype, 1, c);
+    return s;
 }
 
 template <class TY, int NK> struct Shapes {   // own rows of a workgroup, rows of a tile
@@ -630,6 +619,8 @@ template <class TY, int NK> struct Shapes {   // own rows of a workgroup, rows o
 // f(type, integral constant of NK) for the call's type and channels
 template <class TY, class F> int with_fragments(int nk, F f) {
     switch (nk) {
+        case 0:
+            if constexpr (TY::kSize == 4) return f(TY{}, std::integral_constant<int, 0>{});
         case 1: return f(TY{}, std::integral_constant<int, 1>{});
         case 2: return f(TY{}, std::integral_constant<int, 2>{});
         case 4: return f(TY{}, std::integral_constant<int, 4>{});
@@ -646,6 +637,7 @@ template <class F> int with_type(const DstLabelParams *p, F f) {
 }
 
 struct ForwardPlan {
+    Sets sets;
     Split split;
     bool few;
     int64_t tiles, blocks;   // own tiles; blocks that leave a sum
@@ -661,6 +653,8 @@ template <class TY, int NK> ForwardPlan forward_plan(const DstLabelParams *p, bo
     Carve c = {base, 0};
     LabelArgs unused = {};
     if (!a) a = &unused;
+    f.sets = row_sets(p, c);
+    a->x = f.sets.x.rows, a->w = f.sets.w.rows;
     a->splits = f.split.splits, a->per_split = f.split.per_split;
     if (f.split.splits > 1) {
         a->part = c.take<float2>((uint64_t)f.split.splits * p->rays);
@@ -681,6 +675,7 @@ template <class TY, int NK> ForwardPlan forward_plan(const DstLabelParams *p, bo
 }
 
 struct BackwardPlan {
+    Sets sets;
     Split split;
     bool few;
     int64_t tiles;
@@ -697,6 +692,8 @@ template <class TY, int NK> BackwardPlan backward_plan(const DstLabelParams *p, 
     Carve c = {base, 0};
     LabelArgs unused = {};
     if (!a) a = &unused;
+    b.sets = row_sets(p, c);
+    a->x = b.sets.x.rows, a->w = b.sets.w.rows;
     a->splits = b.split.splits, a->per_split = b.split.per_split;
     if (b.split.splits > 1) {
         a->out_part = c.take<float>((uint64_t)b.split.splits * own * p->channels);
@@ -750,6 +747,7 @@ int dst_label_loss_forward(const DstLabelParams *p, void *stream) {
         if (p->reduction == DST_REDUCE_NONE) a.rows = p->loss;
         const hipStream_t s = (hipStream_t)stream;
         if (f.tiles > 0) {
+            prepare(f.sets.x, s), prepare(f.sets.w, s);
             const dim3 grid((uint32_t)(f.tiles * a.splits));
             if (f.few) k_label_forward<TY, NK, 1, false><<<grid, kThreads, 0, s>>>(a);
             else k_label_forward<TY, NK, forward_blocks<TY, NK>(), false><<<grid, kThreads, 0, s>>>(a);
@@ -780,6 +778,7 @@ int dst_label_loss_backward(const DstLabelParams *p, void *stream) {
         typedef typename TY::E E;
         constexpr int NK = decltype(nk)::value, QB = backward_blocks<TY, NK>();
         const hipStream_t s = (hipStream_t)stream;
+        bool copied = false;
         for (int pass = 0; pass < 2; ++pass) {
             const bool dx = pass == 0;
             if (dx ? !p->grad_features || p->rays == 0 : !p->grad_weight && !p->grad_bias) continue;
@@ -790,6 +789,8 @@ int dst_label_loss_backward(const DstLabelParams *p, void *stream) {
             a.inverse = a.upstream_rows ? nullptr : p->inverse;
             a.out = dx ? p->grad_features : p->grad_weight, a.bias_out = p->grad_bias;
             const dim3 grid((uint32_t)(b.tiles * a.splits));
+            if (!copied) prepare(b.sets.x, s), prepare(b.sets.w, s);   // (both passes have the copies in the same place)
+            copied = true;
             if (dx && b.few) k_label_dx<TY, NK, 1><<<grid, kThreads, 0, s>>>(a);
             else if (dx) k_label_dx<TY, NK, QB><<<grid, kThreads, 0, s>>>(a);
             else if (b.few) k_label_dw<TY, NK, 1><<<grid, kThreads, 0, s>>>(a);
@@ -819,6 +820,7 @@ int dst_label_best(const DstLabelParams *p, void *stream) {
         if (int rc = check_workspace(p, f.bytes)) return rc;
         a.label = p->best, a.log_prob = p->log_prob;
         const hipStream_t s = (hipStream_t)stream;
+        prepare(f.sets.x, s), prepare(f.sets.w, s);
         k_label_bounds<TY><<<kBoundBlocks, kThreads, 0, s>>>(a, const_cast<float *>(a.bounds));
         const dim3 grid((uint32_t)(f.tiles * a.splits));
         if (f.few) k_label_forward<TY, NK, 1, true><<<grid, kThreads, 0, s>>>(a);
