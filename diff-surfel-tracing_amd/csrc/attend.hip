@@ -19,32 +19,31 @@ struct AttendArgs {
     const int32_t *lengths;
     int32_t queries, memory, heads, kv_heads, group, rows;   // rows = queries * group
     int32_t d, dv;
-    int32_t splits, per_split;
-    int32_t tiles;                 // of own rows, of one kv head of one batch
+    Cut cut;
+    int32_t own, tiles;            // own rows of a workgroup; tiles of them of one kv head of one batch
     float scale, c;                // c: what brings a product of rows to a score in units of log 2, but for what own rows carry
     float own_scale;               // 32-bit rows
     int32_t flip;                  // 16-bit rows
     void *out;
     float *lse2, *delta;
     void *dq, *dk, *dvalue;        // contiguous
-    float2 *part;                  // (splits, batch * kv_heads * rows): maximum and sum
-    float *out_part, *out_part2;   // (splits, ...) sums of a split pass
+    float2 *part;                  // of a part's rows: maximum and sum
+    float *out_part, *out_part2;   // of a part's rows: sums
     int64_t all_rows;              // batch * kv_heads * rows
-    int64_t own_all;               // dk, dv: batch * memory * kv_heads
 };
 
-// Own blocks of 16 rows a wave (registers: own rows and sums, see the use)
-template <class TY, int NK> constexpr int forward_blocks() { return NK <= 4 ? 4 : NK <= 8 ? 2 : 1; }
-template <class TY, int NK> constexpr int dq_blocks() { return NK <= 2 ? 4 : NK <= 4 ? 2 : 1; }
-template <class TY, int NK> constexpr int dkv_blocks() { return NK <= 2 ? (TY::kSize == 2 ? 2 : 4) : NK <= 4 ? 2 : 1; }
+// Own blocks of 16 rows a wave. More of them read a streamed tile fewer times from LDS, fewer leave registers for a second wave on a
+// SIMD, which counts for more: the waits of one are the other's work (16384 x 8192, 8 heads of 128, bf16: forward 802 us with 4
+// blocks, 685 with 2; dk and dv 1619 with 2, 1317 with 1).
+template <class TY, int NK> constexpr int forward_blocks() { return NK <= 8 ? 2 : 1; }
+template <class TY, int NK> constexpr int dq_blocks() { return NK <= 4 ? 2 : 1; }
+template <class TY, int NK> constexpr int dkv_blocks() { return NK <= 2 ? 2 : 1; }
 
-struct Place {   // which own tile, split, batch and kv head a workgroup has
-    int split, tile, batch, kv, length;
+struct Place {   // which own tile, batch and kv head a workgroup has
+    int tile, batch, kv, length;
 };
-__device__ inline Place place_of(const AttendArgs &a) {
+__device__ inline Place place_of(const AttendArgs &a, uint32_t i) {
     Place p;
-    uint32_t i = blockIdx.x;
-    p.split = i % (uint32_t)a.splits, i /= (uint32_t)a.splits;
     p.tile = i % (uint32_t)a.tiles, i /= (uint32_t)a.tiles;
     p.kv = i % (uint32_t)a.kv_heads, p.batch = i / (uint32_t)a.kv_heads;
     p.length = a.lengths ? min(max(a.lengths[p.batch], 0), a.memory) : a.memory;
@@ -83,10 +82,11 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     __shared__ alignas(16) char tile_k[T::kRows * T::kPitch], tile_v[T::kRows * T::kPitch];
     __shared__ alignas(16) float tile_mask[T::kRows];   // 0, or -inf of a row behind the length, which takes it out of every sum
     const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6;
-    const Place p = place_of(a);
+    const Turn turn = turn_of(a.cut);
+    const Place p = place_of(a, turn.tile);
     const int row0 = p.tile * (kWaves * 16 * QB) + wave * 16 * QB;
-    const int first = p.split * a.per_split * T::kRows;
-    const int last = min(p.length, first + a.per_split * T::kRows);
+    const int first = turn.split * a.cut.per_split * T::kRows;
+    const int last = turn.part ? min(p.length, first + a.cut.per_split * T::kRows) : p.length;
 
     Stage<NK> stage_k, stage_v;
     stage_k.begin(a.k);
@@ -162,8 +162,8 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
         const float sum = sum_group(l[q]);
         if (row >= a.rows) continue;
         const int64_t at = stat_row(a, p, row);
-        if (a.splits > 1) {
-            const int64_t part = (int64_t)p.split * a.all_rows + at;
+        if (turn.part) {
+            const int64_t part = part_row(a.cut, turn, kWaves * 16 * QB, wave * 16 * QB + q * 16 + (lane & 15));
             if (g == 0) a.part[part] = float2{m[q], sum};
             if (first < last)
 #pragma unroll
@@ -183,21 +183,22 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
 template <class E> __global__ __launch_bounds__(kThreads) void k_attend_join_row(AttendArgs a, int rows_per_part) {
     __shared__ float weight[kMostSplits], wave_top[kWaves], wave_sum[kWaves];
     __shared__ f4 sums[kThreads];
-    const int64_t at = blockIdx.x;
-    Place p;
-    p.kv = (int)(at / a.rows % a.kv_heads), p.batch = (int)(at / a.rows / a.kv_heads);
-    const int row = (int)(at % a.rows), tid = threadIdx.x;
-    const int length = a.lengths ? min(max(a.lengths[p.batch], 0), a.memory) : a.memory;
+    const int tile = blockIdx.x / a.own, tid = threadIdx.x;
+    const Place p = place_of(a, a.cut.whole + tile);
+    const int row = p.tile * a.own + (int)(blockIdx.x % a.own), length = p.length;
+    if (row >= a.rows) return;
+    const int64_t from = (int64_t)tile * a.cut.splits * a.own + blockIdx.x % a.own;   // the row's first part; the next: own rows on
+    const int64_t at = stat_row(a, p, row);
     const int used = (length + rows_per_part - 1) / rows_per_part;   // (parts behind the length left no sums)
     float top = -kInf;
-    for (int s = tid; s < used; s += kThreads) top = fmaxf(top, a.part[(int64_t)s * a.all_rows + at].x);
+    for (int s = tid; s < used; s += kThreads) top = fmaxf(top, a.part[from + (int64_t)s * a.own].x);
     for (int step = 32; step > 0; step >>= 1) top = fmaxf(top, __shfl_xor(top, step));
     if ((tid & 63) == 0) wave_top[tid >> 6] = top;
     __syncthreads();
     const float m = fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3])), use = finite_or_zero(m);
     float l = 0.0f;
     for (int s = tid; s < used; s += kThreads) {
-        const float2 ml = a.part[(int64_t)s * a.all_rows + at];
+        const float2 ml = a.part[from + (int64_t)s * a.own];
         const float by = exp2_of(ml.x - use);
         weight[s] = by;
         l += ml.y * by;
@@ -215,12 +216,12 @@ template <class E> __global__ __launch_bounds__(kThreads) void k_attend_join_row
     if (word < words) {
 #pragma unroll 4
         for (int s = lane; s < used; s += lanes) {
-            const float *from = a.out_part + ((int64_t)s * a.all_rows + at) * a.dv + 4 * word;
+            const float *part = a.out_part + (from + (int64_t)s * a.own) * a.dv + 4 * word;
             if (four) {
-                o += *reinterpret_cast<const f4 *>(from) * weight[s];
+                o += *reinterpret_cast<const f4 *>(part) * weight[s];
             } else {
                 for (int i = 0; i < 4; ++i)
-                    if (4 * word + i < a.dv) o[i] += from[i] * weight[s];
+                    if (4 * word + i < a.dv) o[i] += part[i] * weight[s];
             }
         }
     }
@@ -237,22 +238,22 @@ template <class E> __global__ __launch_bounds__(kThreads) void k_attend_join_row
 // The same, a thread for four channels of a row.
 template <class E> __global__ __launch_bounds__(kThreads) void k_attend_join(AttendArgs a, int rows_per_part) {
     const int words = (a.dv + 3) / 4;
-    const int64_t id = (int64_t)blockIdx.x * kThreads + threadIdx.x, at = id / words;
-    const int c = (int)(id - at * words) * 4;
-    if (at >= a.all_rows) return;
-    Place p;
-    p.kv = (int)(at / a.rows % a.kv_heads), p.batch = (int)(at / a.rows / a.kv_heads);
-    const int row = (int)(at % a.rows);
-    const int length = a.lengths ? min(max(a.lengths[p.batch], 0), a.memory) : a.memory;
+    const int64_t id = (int64_t)blockIdx.x * kThreads + threadIdx.x, i = id / words;
+    const int c = (int)(id - i * words) * 4, tile = (int)(i / a.own);
+    if (i >= a.cut.parted() * a.own) return;
+    const Place p = place_of(a, a.cut.whole + tile);
+    const int row = p.tile * a.own + (int)(i % a.own), length = p.length;
+    if (row >= a.rows) return;
+    const int64_t first = (int64_t)tile * a.cut.splits * a.own + i % a.own, at = stat_row(a, p, row);
     const int used = (length + rows_per_part - 1) / rows_per_part;   // (parts behind the length left no sums)
     float m = -kInf;
-    for (int s = 0; s < used; ++s) m = fmaxf(m, a.part[(int64_t)s * a.all_rows + at].x);
+    for (int s = 0; s < used; ++s) m = fmaxf(m, a.part[first + (int64_t)s * a.own].x);
     const float use = finite_or_zero(m);
     const bool four = (a.dv & 3) == 0;
     float l = 0.0f;
     f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int s = 0; s < used; ++s) {
-        const int64_t part = (int64_t)s * a.all_rows + at;
+        const int64_t part = first + (int64_t)s * a.own;
         const float2 ml = a.part[part];
         const float by = exp2_of(ml.x - use);
         l += ml.y * by;
@@ -291,10 +292,11 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     __shared__ alignas(16) char tile_k[T::kRows * T::kPitch], tile_v[T::kRows * T::kPitch];
     __shared__ alignas(16) float tile_mask[T::kRows];   // 0, or -inf of a row behind the length, which takes it out of every sum
     const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6;
-    const Place p = place_of(a);
+    const Turn turn = turn_of(a.cut);
+    const Place p = place_of(a, turn.tile);
     const int row0 = p.tile * (kWaves * 16 * QB) + wave * 16 * QB;
-    const int first = p.split * a.per_split * T::kRows;
-    const int last = a.dq ? min(p.length, first + a.per_split * T::kRows) : 0;
+    const int first = turn.split * a.cut.per_split * T::kRows;
+    const int last = !a.dq ? 0 : turn.part ? min(p.length, first + a.cut.per_split * T::kRows) : p.length;
 
     Stage<NK> stage_k, stage_v;
     stage_k.begin(a.k);
@@ -316,7 +318,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     for (int q = 0; q < QB; ++q) {
         const int row = row0 + q * 16 + (lane & 15);
         lse2[q] = row < a.rows ? a.lse2[stat_row(a, p, row)] : kInf;
-        if (row < a.rows && g == 0 && p.split == 0) a.delta[stat_row(a, p, row)] = delta[q];
+        if (row < a.rows && g == 0 && turn.split == 0) a.delta[stat_row(a, p, row)] = delta[q];
 #pragma unroll
         for (int i = 0; i < NM; ++i) out[q][i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
@@ -357,7 +359,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
 #pragma unroll
         for (int i = 0; i < NM; ++i) {
             const f4 v = out[q][i] * a.scale;
-            if (a.splits > 1) store_four(a.out_part + ((int64_t)p.split * a.all_rows + to) * a.d, i * 16 + 4 * g, a.d, v, four);
+            if (turn.part) store_four(a.out_part + part_row(a.cut, turn, kWaves * 16 * QB, wave * 16 * QB + q * 16 + (lane & 15)) * a.d, i * 16 + 4 * g, a.d, v, four);
             else store_four(reinterpret_cast<E *>(a.dq) + to * a.d, i * 16 + 4 * g, a.d, v, four);
         }
     }
@@ -371,10 +373,11 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     __shared__ alignas(16) char tile_q[T::kRows * T::kPitch], tile_o[T::kRows * T::kPitch];
     __shared__ alignas(16) float tile_lse2[T::kRows], tile_delta[T::kRows];
     const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6;
-    const Place p = place_of(a);
+    const Turn turn = turn_of(a.cut);
+    const Place p = place_of(a, turn.tile);
     const int tile0 = p.tile * (kWaves * 16 * QB), row0 = tile0 + wave * 16 * QB;
-    const int first = p.split * a.per_split * T::kRows;
-    const int last = tile0 < p.length ? min(a.rows, first + a.per_split * T::kRows) : 0;
+    const int first = turn.split * a.cut.per_split * T::kRows;
+    const int last = tile0 >= p.length ? 0 : turn.part ? min(a.rows, first + a.cut.per_split * T::kRows) : a.rows;
 
     Stage<NK> stage_q, stage_o;
     stage_q.begin(a.q);
@@ -438,11 +441,11 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
         if (row >= a.memory) continue;
         const int64_t to = ((int64_t)p.batch * a.memory + row) * a.kv_heads + p.kv;
         const bool there = row < p.length;   // (a row behind the length has products of zeros with anything)
-        const int64_t part = (int64_t)p.split * a.own_all + to;
+        const int64_t part = part_row(a.cut, turn, kWaves * 16 * QB, wave * 16 * QB + q * 16 + (lane & 15));
 #pragma unroll
         for (int i = 0; i < NM; ++i) {
             const f4 k = there ? dk[q][i] * a.scale : none, v = there ? dv[q][i] : none;
-            if (a.splits > 1) {
+            if (turn.part) {
                 store_four(a.out_part + part * a.d, i * 16 + 4 * g, a.d, k, four_k);
                 store_four(a.out_part2 + part * a.dv, i * 16 + 4 * g, a.dv, v, four_v);
             } else {
@@ -490,7 +493,6 @@ AttendArgs arguments(const DstAttendParams *p) {
     if (a.c < 1.1754944e-38f) a.c = 1.1754944e-38f;
     if (p->dtype == DST_DTYPE_F32) a.own_scale = a.flip ? -a.c : a.c, a.c = 1.0f;
     a.out = p->out, a.lse2 = p->lse;
-    a.splits = a.per_split = 1;
     a.all_rows = (int64_t)p->batch * p->kv_heads * a.rows;
     return a;
 }
@@ -514,20 +516,6 @@ int fragments(const DstAttendParams *p) {
 template <class F> int with_type(const DstAttendParams *p, F f) {
     if (p->dtype == DST_DTYPE_F32) return with_fragments<F32>(fragments(p), f);
     return p->dtype == DST_DTYPE_BF16 ? with_fragments<BF16>(fragments(p), f) : with_fragments<F16>(fragments(p), f);
-}
-
-// Own blocks of 16 rows a wave: one where the rows are few, by the rule that every pass has.
-int blocks_for(int most, int64_t rows, int64_t heads, int tile, int64_t streamed) {
-    return rows <= kWaves * 16 || few_rows(div_up(rows, kWaves * 16 * most) * heads, 1, div_up(streamed, tile)) ? 1 : most;
-}
-template <class TY, int NK> int forward_rows(const AttendArgs &a, int64_t heads) {
-    return kWaves * 16 * blocks_for(forward_blocks<TY, NK>(), a.rows, heads, TileShape<NK>::kRows, a.memory);
-}
-template <class TY, int NK> int dq_rows(const AttendArgs &a, int64_t heads) {
-    return kWaves * 16 * blocks_for(dq_blocks<TY, NK>(), a.rows, heads, TileShape<NK>::kRows, a.memory);
-}
-template <class TY, int NK> int dkv_rows(const AttendArgs &a, int64_t heads) {
-    return kWaves * 16 * blocks_for(dkv_blocks<TY, NK>(), a.memory, heads, TileShape<NK>::kRows, a.rows);
 }
 
 // The rows of all sets, copied into the workspace's front where the kernels cannot read them where they lie.
@@ -559,36 +547,76 @@ void prepare(const Sets &s, hipStream_t stream) {
     for (const RowSet *r : {&s.q, &s.k, &s.v, &s.o, &s.up}) prepare(*r, stream);
 }
 
-uint64_t plan_forward(AttendArgs &a, int own, int tile, int64_t heads, Carve c) {
-    a.tiles = (int)div_up(a.rows, own);
-    const Split s = split_tiles(a.tiles * heads, div_up(a.memory, tile));
-    a.splits = s.splits, a.per_split = s.per_split;
-    if (a.splits > 1) {
-        a.part = c.take<float2>((uint64_t)a.splits * a.all_rows);
-        a.out_part = c.take<float>((uint64_t)a.splits * a.all_rows * a.dv);
+// Cuts a pass's own tiles; whether its rows are few. `kernel(few)`: the pass's kernel; `own_bytes`: of a part's row.
+template <class TY, int NK, class K>
+bool plan_cut(AttendArgs &a, int most, int64_t own_rows, int64_t streamed_rows, int64_t heads, int products, double row_bytes, K kernel) {
+    constexpr int tile = TileShape<NK>::kRows, dtype = TY::kSize == 4 ? DST_DTYPE_F32 : DST_DTYPE_BF16;
+    const int64_t streamed = div_up(streamed_rows, tile);
+    const bool few = own_rows <= kWaves * 16 || few_rows(div_up(own_rows, kWaves * 16 * most) * heads, streamed);
+    a.own = kWaves * 16 * (few ? 1 : most);
+    a.tiles = (int)div_up(own_rows, a.own);
+    a.cut = cut_tiles(a.tiles * heads, streamed, slots_of(kernel(few)), tile_time(a.own, tile, TileShape<NK>::kBytes, dtype, products),
+                      a.own * row_bytes, a.lengths != nullptr);
+    return few;
+}
+uint64_t parted_rows(const AttendArgs &a) { return a.cut.splits > 1 ? (uint64_t)a.cut.parted() * a.own * a.cut.splits : 0; }
+
+struct Plan {
+    bool few;
+    uint64_t bytes;
+};
+template <class TY, int NK> Plan plan_forward(AttendArgs &a, int64_t heads, Carve c) {
+    Plan p;
+    p.few = plan_cut<TY, NK>(a, forward_blocks<TY, NK>(), a.rows, a.memory, heads, 2, a.dv * 4.0 + 8.0, [](bool few) {
+        return few ? (const void *)&k_attend_forward<TY, NK, 1> : (const void *)&k_attend_forward<TY, NK, forward_blocks<TY, NK>()>;
+    });
+    if (const uint64_t rows = parted_rows(a)) {
+        a.part = c.take<float2>(rows);
+        a.out_part = c.take<float>(rows * a.dv);
     }
-    return c.used;
+    p.bytes = c.used;
+    return p;
 }
-uint64_t plan_dq(AttendArgs &a, int own, int tile, int64_t heads, Carve c) {
-    a.tiles = (int)div_up(a.rows, own);
-    const Split s = a.dq ? split_tiles(a.tiles * heads, div_up(a.memory, tile)) : Split{1, 1};
-    a.splits = s.splits, a.per_split = s.per_split;
+template <class TY, int NK> Plan plan_dq(AttendArgs &a, int64_t heads, Carve c) {
+    Plan p;
+    p.few = plan_cut<TY, NK>(a, dq_blocks<TY, NK>(), a.rows, a.dq ? a.memory : 0, heads, 3, a.d * 4.0, [](bool few) {
+        return few ? (const void *)&k_attend_dq<TY, NK, 1> : (const void *)&k_attend_dq<TY, NK, dq_blocks<TY, NK>()>;
+    });
     a.delta = c.take<float>(a.all_rows);
-    if (a.splits > 1) a.out_part = c.take<float>((uint64_t)a.splits * a.all_rows * a.d);
-    return c.used;
+    if (const uint64_t rows = parted_rows(a)) a.out_part = c.take<float>(rows * a.d);
+    p.bytes = c.used;
+    return p;
 }
-uint64_t plan_dkv(AttendArgs &a, int own, int tile, int64_t heads, Carve c) {
-    a.tiles = (int)div_up(a.memory, own);
-    const Split s = split_tiles(a.tiles * heads, div_up(a.rows, tile));
-    a.splits = s.splits, a.per_split = s.per_split;
+template <class TY, int NK> Plan plan_dkv(AttendArgs &a, int64_t heads, Carve c) {
+    Plan p;
+    p.few = plan_cut<TY, NK>(a, dkv_blocks<TY, NK>(), a.memory, a.rows, heads, 4, (a.d + a.dv) * 4.0, [](bool few) {
+        return few ? (const void *)&k_attend_dkv<TY, NK, 1> : (const void *)&k_attend_dkv<TY, NK, dkv_blocks<TY, NK>()>;
+    });
     a.delta = c.take<float>(a.all_rows);
-    if (a.splits > 1) {
-        const uint64_t rows = (uint64_t)a.splits * heads * a.memory;
+    if (const uint64_t rows = parted_rows(a)) {
         a.out_part = c.take<float>(rows * a.d);
         a.out_part2 = c.take<float>(rows * a.dv);
     }
-    return c.used;
+    p.bytes = c.used;
+    return p;
 }
+
+// The output row of a parted row: of dq, of dk and dv
+struct QueryRow {
+    int whole, tiles, own, rows, kv_heads, group, queries;
+    __device__ int64_t operator()(int tile, int row) const {
+        const int t = whole + tile, r = t % tiles * own + row, head = t / tiles % kv_heads, batch = t / tiles / kv_heads;
+        if (r >= rows) return -1;
+        return ((int64_t)batch * queries + r / group) * (kv_heads * group) + head * group + r % group;
+    }
+};
+struct MemoryRow {
+    int whole, tiles, own, memory, kv_heads;
+    __device__ int64_t operator()(int tile, int row) const {
+        const int t = whole + tile, r = t % tiles * own + row, head = t / tiles % kv_heads, batch = t / tiles / kv_heads;
+        return r < memory ? ((int64_t)batch * memory + r) * kv_heads + head : -1;
+    }
+};
 
 int check_workspace(const DstAttendParams *p, uint64_t need) {
     if (need == 0) return DST_OK;
@@ -614,12 +642,12 @@ uint64_t dst_attend_workspace_bytes(const DstAttendParams *p, int pass) {
         Carve c = {nullptr, 0};
         row_sets<NK>(p, a, pass != DST_PASS_FORWARD, c);
         if (pass == DST_PASS_FORWARD) {
-            bytes = plan_forward(a, forward_rows<TY, NK>(a, heads), TileShape<NK>::kRows, heads, c);
+            bytes = plan_forward<TY, NK>(a, heads, c).bytes;
         } else {
             a.dq = p->grad_q;
-            bytes = plan_dq(a, dq_rows<TY, NK>(a, heads), TileShape<NK>::kRows, heads, c);
+            bytes = plan_dq<TY, NK>(a, heads, c).bytes;
             if (p->grad_k || p->grad_v) {
-                const uint64_t more = plan_dkv(a, dkv_rows<TY, NK>(a, heads), TileShape<NK>::kRows, heads, c);
+                const uint64_t more = plan_dkv<TY, NK>(a, heads, c).bytes;
                 bytes = more > bytes ? more : bytes;
             }
         }
@@ -637,22 +665,21 @@ int dst_attend_forward(const DstAttendParams *p, void *stream) {
         AttendArgs a = arguments(p);
         if (a.all_rows == 0) return (int)DST_OK;
         const int64_t heads = (int64_t)p->batch * p->kv_heads;
-        const int own = forward_rows<TY, NK>(a, heads);
         Carve c = {(char *)p->workspace, 0};
         const Sets sets = row_sets<NK>(p, a, false, c);
-        const uint64_t need = plan_forward(a, own, TileShape<NK>::kRows, heads, c);
-        if (int rc = check_workspace(p, need)) return rc;
+        const Plan plan = plan_forward<TY, NK>(a, heads, c);
+        if (int rc = check_workspace(p, plan.bytes)) return rc;
         const hipStream_t s = (hipStream_t)stream;
         prepare(sets, s);
-        const dim3 grid((uint32_t)(a.tiles * heads * a.splits));
-        if (own == kWaves * 16) k_attend_forward<TY, NK, 1><<<grid, kThreads, 0, s>>>(a);
+        const dim3 grid((uint32_t)a.cut.blocks());
+        if (plan.few) k_attend_forward<TY, NK, 1><<<grid, kThreads, 0, s>>>(a);
         else k_attend_forward<TY, NK, QB><<<grid, kThreads, 0, s>>>(a);
         DST_OP_LAUNCH("attention");
-        if (a.splits > 1) {
-            const int64_t words = a.all_rows * ((a.dv + 3) / 4);
-            const int part = a.per_split * TileShape<NK>::kRows;
-            if (a.splits >= 16) k_attend_join_row<E><<<dim3((uint32_t)a.all_rows), kThreads, 0, s>>>(a, part);
-            else k_attend_join<E><<<dim3((uint32_t)div_up(words, kThreads)), kThreads, 0, s>>>(a, part);
+        if (a.cut.splits > 1) {
+            const int64_t rows = a.cut.parted() * a.own;
+            const int part = a.cut.per_split * TileShape<NK>::kRows;
+            if (a.cut.splits >= 16) k_attend_join_row<E><<<dim3((uint32_t)rows), kThreads, 0, s>>>(a, part);
+            else k_attend_join<E><<<dim3((uint32_t)div_up(rows * ((a.dv + 3) / 4), kThreads)), kThreads, 0, s>>>(a, part);
             DST_OP_LAUNCH("attention, joining");
         }
         return (int)DST_OK;
@@ -670,7 +697,6 @@ int dst_attend_backward(const DstAttendParams *p, void *stream) {
         typedef decltype(ty) TY;
         typedef typename TY::E E;
         constexpr int NK = decltype(nk)::value;
-        constexpr int tile = TileShape<NK>::kRows;
         const hipStream_t s = (hipStream_t)stream;
         const int64_t heads = (int64_t)p->batch * p->kv_heads;
         AttendArgs a = arguments(p);
@@ -678,32 +704,27 @@ int dst_attend_backward(const DstAttendParams *p, void *stream) {
         const Sets sets = row_sets<NK>(p, a, true, c);
         a.dq = p->grad_q, a.dk = p->grad_k, a.dvalue = p->grad_v;
         if (a.all_rows > 0) {
-            const int own = dq_rows<TY, NK>(a, heads);
-            const uint64_t need = plan_dq(a, own, tile, heads, c);
-            if (int rc = check_workspace(p, need)) return rc;
+            const Plan plan = plan_dq<TY, NK>(a, heads, c);
+            if (int rc = check_workspace(p, plan.bytes)) return rc;
             prepare(sets, s);
-            const dim3 grid((uint32_t)(a.tiles * heads * a.splits));
-            if (own == kWaves * 16) k_attend_dq<TY, NK, 1><<<grid, kThreads, 0, s>>>(a);
+            const dim3 grid((uint32_t)a.cut.blocks());
+            if (plan.few) k_attend_dq<TY, NK, 1><<<grid, kThreads, 0, s>>>(a);
             else k_attend_dq<TY, NK, dq_blocks<TY, NK>()><<<grid, kThreads, 0, s>>>(a);
             DST_OP_LAUNCH("attention gradient, queries");
-            if (a.splits > 1) {
-                sum_parts(a.out_part, (E *)a.dq, a.all_rows * a.d, nullptr, (E *)nullptr, 0, a.splits, s);
-                DST_OP_LAUNCH("attention gradient, summing");
-            }
+            const QueryRow to = {a.cut.whole, a.tiles, a.own, a.rows, a.kv_heads, a.group, a.queries};
+            sum_parts(Parts<E>{a.out_part, (E *)a.dq, a.d}, Parts<E>{nullptr, nullptr, 1}, a.cut, a.own, to, s);
+            DST_OP_LAUNCH("attention gradient, summing");
         }
         if ((a.dk || a.dvalue) && heads * a.memory > 0) {
-            const int own = dkv_rows<TY, NK>(a, heads);
-            const uint64_t need = plan_dkv(a, own, tile, heads, c);
-            if (int rc = check_workspace(p, need)) return rc;
-            a.own_all = heads * a.memory;
-            const dim3 grid((uint32_t)(a.tiles * heads * a.splits));
-            if (own == kWaves * 16) k_attend_dkv<TY, NK, 1><<<grid, kThreads, 0, s>>>(a);
+            const Plan plan = plan_dkv<TY, NK>(a, heads, c);
+            if (int rc = check_workspace(p, plan.bytes)) return rc;
+            const dim3 grid((uint32_t)a.cut.blocks());
+            if (plan.few) k_attend_dkv<TY, NK, 1><<<grid, kThreads, 0, s>>>(a);
             else k_attend_dkv<TY, NK, dkv_blocks<TY, NK>()><<<grid, kThreads, 0, s>>>(a);
             DST_OP_LAUNCH("attention gradient, memory");
-            if (a.splits > 1) {
-                sum_parts(a.out_part, (E *)a.dk, a.own_all * a.d, a.out_part2, (E *)a.dvalue, a.own_all * a.dv, a.splits, s);
-                DST_OP_LAUNCH("attention gradient, summing");
-            }
+            const MemoryRow to = {a.cut.whole, a.tiles, a.own, a.memory, a.kv_heads};
+            sum_parts(Parts<E>{a.out_part, (E *)a.dk, a.d}, Parts<E>{a.out_part2, (E *)a.dvalue, a.dv}, a.cut, a.own, to, s);
+            DST_OP_LAUNCH("attention gradient, summing");
         }
         return (int)DST_OK;
     };

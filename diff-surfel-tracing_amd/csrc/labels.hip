@@ -21,17 +21,18 @@ struct LabelArgs {
     const int64_t *target;          // (rays)
     int64_t rays, ignore;
     int32_t d, labels;
-    int32_t splits, per_split;      // parts of the streamed rows; tiles of each
+    Cut cut;
+    int32_t own;                    // own rows of a workgroup
     // forward
-    float2 *part;                   // (splits, rays): maximum and sum, in units of log 2
-    float *target_logit;            // (rays): forward with splits
+    float2 *part;                   // of a part's rays: maximum and sum, in units of log 2
+    float *target_logit;            // of the parted rays
     float *lse2;                    // (rays): log2 of the sum of exponentials; +inf where the ray is ignored
     float *rows;                    // (rays) losses, or nullptr
     double *sums;                   // (blocks): sums of losses ...
     uint32_t *counts;               // ... and rays counted in them
     // the best label
     const float *bounds;            // (kBoundBlocks, 2): largest row norm of the table, largest |bias|
-    int4 *best;                     // (splits, rays): bits of the best logit, its label, bits of the second best, -
+    int4 *best;                     // of a part's rays: bits of the best logit, its label, bits of the second best, -
     int64_t *label;                 // (rays)
     float *log_prob;                // (rays)
     uint32_t *near_count;           // rays whose two best labels 32 bits cannot tell apart ...
@@ -42,18 +43,16 @@ struct LabelArgs {
     const float *inverse;           // one value that multiplies a single upstream value, or nullptr
     int32_t upstream_rows;
     void *out;                      // (rays, d) or (labels, d), of the inputs' type
-    float *out_part;                // (splits, rows, d) if splits > 1
-    float *bias_out, *bias_part;    // (labels); (splits, labels)
+    float *out_part;                // of a part's rows: d values
+    float *bias_out, *bias_part;    // (labels); of a part's rows
 };
 
 constexpr int kBoundBlocks = 64;
 
-// Own blocks of 16 rows of a wave: as many as the registers hold with a wave or two on a SIMD: the more, the fewer times a
-// streamed tile is read from LDS.
-template <class TY, int NK> constexpr int forward_blocks() { return NK <= 4 ? 4 : NK <= 8 ? 2 : 1; }
-template <class TY, int NK> constexpr int backward_blocks() {
-    return NK * (TY::kSize == 2 ? 12 : 8) <= 32 ? 4 : NK * (TY::kSize == 2 ? 12 : 8) <= 96 ? 2 : 1;
-}
+// Own blocks of 16 rows of a wave. More of them read a streamed tile fewer times from LDS, fewer leave registers for a second wave
+// on a SIMD, which counts for more (32768 rays x 32771 labels, 256 channels, bf16: dx 1661 us with 2 blocks, 1268 with 1).
+template <class TY, int NK> constexpr int forward_blocks() { return NK <= 1 ? 4 : NK <= 8 ? 2 : 1; }
+template <class TY, int NK> constexpr int backward_blocks() { return NK <= 1 ? (TY::kSize == 2 ? 2 : 4) : NK <= 4 ? 2 : 1; }
 
 // The upstream gradient of a ray's loss: 0 where it is ignored, NaN where its label is none.
 __device__ inline float upstream_of(const LabelArgs &a, int64_t row, int64_t t) {
@@ -79,7 +78,7 @@ __device__ inline void finish_row(const LabelArgs &a, int64_t row, Running r, fl
 }
 
 // The workgroup's sum of losses and count of rays, in an order of its own.
-__device__ inline void block_sums(const LabelArgs &a, double sum, uint32_t count, char *lds) {
+__device__ inline void block_sums(const LabelArgs &a, int at, double sum, uint32_t count, char *lds) {
     if (!a.sums) return;
     double *s = reinterpret_cast<double *>(lds);
     uint32_t *c = reinterpret_cast<uint32_t *>(lds + sizeof(double) * kThreads);
@@ -89,7 +88,7 @@ __device__ inline void block_sums(const LabelArgs &a, double sum, uint32_t count
         __syncthreads();
         if ((int)threadIdx.x < step) s[threadIdx.x] += s[threadIdx.x + step], c[threadIdx.x] += c[threadIdx.x + step];
     }
-    if (threadIdx.x == 0) a.sums[blockIdx.x] = s[0], a.counts[blockIdx.x] = c[0];
+    if (threadIdx.x == 0) a.sums[at] = s[0], a.counts[at] = c[0];
 }
 
 // The best label of a ray, or a place on the list of those that 32 bits cannot decide: a logit of d products is off by less
@@ -137,10 +136,10 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
     __shared__ alignas(16) char tile[T::kRows * T::kPitch > kThreads * 12 ? T::kRows * T::kPitch : kThreads * 12];
     __shared__ alignas(16) float tile_bias[T::kRows];
     const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6;
-    const int split = blockIdx.x % a.splits;
-    const int64_t row0 = (int64_t)(blockIdx.x / a.splits) * (kWaves * 16 * QB) + wave * 16 * QB;
-    const int first = split * a.per_split * T::kRows;
-    const int last = min(a.labels, (split + 1) * a.per_split * T::kRows);   // (the host keeps labels + a tile below 2^31)
+    const Turn turn = turn_of(a.cut);
+    const int64_t row0 = (int64_t)turn.tile * (kWaves * 16 * QB) + wave * 16 * QB;
+    const int first = turn.part ? turn.split * a.cut.per_split * T::kRows : 0;
+    const int last = turn.part ? min(a.labels, first + a.cut.per_split * T::kRows) : a.labels;   // (the host keeps labels below 2^30)
 
     Stage<NK> stage;
     stage.begin(a.w);
@@ -225,9 +224,10 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
             for (int step = 16; step <= 32; step <<= 1)
                 merge_best(best[q], label[q], second[q], __shfl_xor(best[q], step), __shfl_xor(label[q], step), __shfl_xor(second[q], step));
             if (row < a.rays && g == 0) {
-                if (a.splits > 1) {
-                    a.part[(int64_t)split * a.rays + row] = float2{r.m, r.l};
-                    a.best[(int64_t)split * a.rays + row] = int4{__builtin_bit_cast(int, best[q]), label[q], __builtin_bit_cast(int, second[q]),
+                if (turn.part) {
+                    const int64_t part = part_row(a.cut, turn, kWaves * 16 * QB, wave * 16 * QB + q * 16 + (lane & 15));
+                    a.part[part] = float2{r.m, r.l};
+                    a.best[part] = int4{__builtin_bit_cast(int, best[q]), label[q], __builtin_bit_cast(int, second[q]),
                                                                  __builtin_bit_cast(int, norm)};
                 } else {
                     finish_best(a, row, r, best[q], label[q], second[q], norm, bound);
@@ -236,7 +236,7 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
         } else {
             // the target's logit, from the own row in registers
             float logit = 0.0f;
-            if (split == 0) {
+            if (turn.split == 0) {
                 const int64_t t = row < a.rays ? a.target[row] : -1;
                 const bool there = t >= 0 && t < a.labels;
 #pragma unroll
@@ -246,9 +246,9 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
                 if (there && a.bias) logit += a.bias[t];
             }
             if (row < a.rays && g == 0) {
-                if (a.splits > 1) {
-                    a.part[(int64_t)split * a.rays + row] = float2{r.m, r.l};
-                    if (split == 0) a.target_logit[row] = logit;
+                if (turn.part) {
+                    a.part[part_row(a.cut, turn, kWaves * 16 * QB, wave * 16 * QB + q * 16 + (lane & 15))] = float2{r.m, r.l};
+                    if (turn.split == 0) a.target_logit[row - (int64_t)a.cut.whole * (kWaves * 16 * QB)] = logit;
                 } else {
                     finish_row(a, row, r, logit, sum, count);
                 }
@@ -256,13 +256,13 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
         }
     }
     if constexpr (!BEST)
-        if (a.splits == 1) block_sums(a, sum, count, tile);
+        if (!turn.part) block_sums(a, turn.tile, sum, count, tile);
 }
 
 // The parts of a split forward pass, a thread a ray.
 template <bool BEST> __global__ __launch_bounds__(kThreads) void k_label_join(LabelArgs a) {
     __shared__ alignas(16) char lds[kThreads * 12];
-    const int64_t row = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x, row = (int64_t)a.cut.whole * a.own + i;
     double sum = 0.0;
     uint32_t count = 0;
     float2 bound = {0.0f, 0.0f};
@@ -271,19 +271,20 @@ template <bool BEST> __global__ __launch_bounds__(kThreads) void k_label_join(La
         Running r = {-kInf, 0.0f};
         float best = -kInf, second = -kInf, norm = 0.0f;
         int label = 0x7fffffff;
-        for (int s = 0; s < a.splits; ++s) {
-            const float2 p = a.part[(int64_t)s * a.rays + row];
+        const int64_t from = i / a.own * a.cut.splits * a.own + i % a.own;
+        for (int s = 0; s < a.cut.splits; ++s) {
+            const float2 p = a.part[from + (int64_t)s * a.own];
             r = merge(r, Running{p.x, p.y});
             if constexpr (BEST) {
-                const int4 b = a.best[(int64_t)s * a.rays + row];
+                const int4 b = a.best[from + (int64_t)s * a.own];
                 merge_best(best, label, second, __builtin_bit_cast(float, b.x), b.y, __builtin_bit_cast(float, b.z));
                 norm = __builtin_bit_cast(float, b.w);
             }
         }
         if constexpr (BEST) finish_best(a, row, r, best, label, second, norm, bound);
-        else finish_row(a, row, r, a.target_logit[row], sum, count);
+        else finish_row(a, row, r, a.target_logit[i], sum, count);
     }
-    if constexpr (!BEST) block_sums(a, sum, count, lds);
+    if constexpr (!BEST) block_sums(a, a.cut.whole + blockIdx.x, sum, count, lds);
 }
 
 // The sum of the blocks' losses, or their mean over the rays counted (none counted: 0 / 0), and what an upstream gradient
@@ -391,10 +392,10 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     __shared__ alignas(16) char tile[T::kRows * T::kPitch];
     __shared__ alignas(16) float tile_bias[T::kRows];
     const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6;
-    const int split = blockIdx.x % a.splits;
-    const int64_t row0 = (int64_t)(blockIdx.x / a.splits) * (kWaves * 16 * QB) + wave * 16 * QB;
-    const int first = split * a.per_split * T::kRows;
-    const int last = min(a.labels, (split + 1) * a.per_split * T::kRows);
+    const Turn turn = turn_of(a.cut);
+    const int64_t row0 = (int64_t)turn.tile * (kWaves * 16 * QB) + wave * 16 * QB;
+    const int first = turn.part ? turn.split * a.cut.per_split * T::kRows : 0;
+    const int last = turn.part ? min(a.labels, first + a.cut.per_split * T::kRows) : a.labels;
 
     Stage<NK> stage;
     stage.begin(a.w);
@@ -456,7 +457,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
         for (int m = 0; m < NM; ++m) {
             f4 v = out[q][m] * up[q];
             if (up[q] == 0.0f) v = f4{0.0f, 0.0f, 0.0f, 0.0f};   // (an ignored ray's channels may hold anything)
-            if (a.splits > 1) store_four(a.out_part + ((int64_t)split * a.rays + row) * a.d, m * 16 + 4 * g, a.d, v, four);
+            if (turn.part) store_four(a.out_part + part_row(a.cut, turn, kWaves * 16 * QB, wave * 16 * QB + q * 16 + (lane & 15)) * a.d, m * 16 + 4 * g, a.d, v, four);
             else store_four(reinterpret_cast<E *>(a.out) + row * a.d, m * 16 + 4 * g, a.d, v, four);
         }
     }
@@ -470,10 +471,10 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     __shared__ alignas(16) float tile_lse2[2][T::kRows], tile_up[2][T::kRows];
     __shared__ alignas(16) int tile_label[2][T::kRows];
     const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6;
-    const int split = blockIdx.x % a.splits;
-    const int row0 = (int)(blockIdx.x / a.splits) * (kWaves * 16 * QB) + wave * 16 * QB;   // (the host keeps labels + a tile below 2^31)
-    const int64_t first = (int64_t)split * a.per_split * T::kRows;
-    const int64_t last = min(a.rays, first + (int64_t)a.per_split * T::kRows);
+    const Turn turn = turn_of(a.cut);
+    const int row0 = turn.tile * (kWaves * 16 * QB) + wave * 16 * QB;   // (the host keeps labels below 2^30)
+    const int64_t first = turn.part ? (int64_t)turn.split * a.cut.per_split * T::kRows : 0;
+    const int64_t last = turn.part ? min(a.rays, first + (int64_t)a.cut.per_split * T::kRows) : a.rays;
 
     Stage<NK> stage;
     stage.begin(a.x);
@@ -563,10 +564,11 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
         const int v = row0 + q * 16 + (lane & 15);
         const float b = sum_group(db[q]);
         if (v >= a.labels) continue;
-        if (g == 0 && a.bias_out) (a.splits > 1 ? a.bias_part + (int64_t)split * a.labels : a.bias_out)[v] = b;
+        const int64_t part = part_row(a.cut, turn, kWaves * 16 * QB, wave * 16 * QB + q * 16 + (lane & 15));
+        if (g == 0 && a.bias_out) *(turn.part ? a.bias_part + part : a.bias_out + v) = b;
 #pragma unroll
         for (int m = 0; m < NM; ++m) {
-            if (a.splits > 1) store_four(a.out_part + ((int64_t)split * a.labels + v) * a.d, m * 16 + 4 * g, a.d, out[q][m], four);
+            if (turn.part) store_four(a.out_part + part * a.d, m * 16 + 4 * g, a.d, out[q][m], four);
             else if (a.out) store_four(reinterpret_cast<E *>(a.out) + (int64_t)v * a.d, m * 16 + 4 * g, a.d, out[q][m], four);
         }
     }
@@ -596,7 +598,6 @@ LabelArgs arguments(const DstLabelParams *p) {
     a.bias = p->bias, a.target = p->targets;
     a.rays = p->rays, a.ignore = p->ignore_index, a.d = p->channels, a.labels = p->labels;
     a.lse2 = p->lse;
-    a.splits = a.per_split = 1;
     return a;
 }
 
@@ -638,37 +639,39 @@ template <class F> int with_type(const DstLabelParams *p, F f) {
 
 struct ForwardPlan {
     Sets sets;
-    Split split;
     bool few;
-    int64_t tiles, blocks;   // own tiles; blocks that leave a sum
+    uint32_t sums;    // blocks that leave a sum
     uint64_t bytes;
 };
-template <class TY, int NK> ForwardPlan forward_plan(const DstLabelParams *p, bool best, char *base, LabelArgs *a) {
+template <class TY, int NK, bool BEST> const void *forward_kernel(bool few) {
+    return few ? (const void *)&k_label_forward<TY, NK, 1, BEST> : (const void *)&k_label_forward<TY, NK, forward_blocks<TY, NK>(), BEST>;
+}
+template <class TY, int NK, bool BEST> ForwardPlan forward_plan(const DstLabelParams *p, LabelArgs &a, char *base) {
     typedef Shapes<TY, NK> S;
     ForwardPlan f;
-    f.few = few_rows(p->rays, S::kForward, div_up(p->labels, S::kTile));
-    f.tiles = div_up(p->rays, f.few ? kWaves * 16 : S::kForward);
-    f.split = split_tiles(f.tiles, div_up(p->labels, S::kTile));
-    f.blocks = f.split.splits > 1 ? div_up(p->rays, kThreads) : f.tiles;
+    const int64_t streamed = div_up(p->labels, S::kTile);
+    f.few = few_rows(div_up(p->rays, S::kForward), streamed);
+    a.own = f.few ? kWaves * 16 : S::kForward;
+    a.cut = cut_tiles(div_up(p->rays, a.own), streamed, slots_of(forward_kernel<TY, NK, BEST>(f.few)),
+                      tile_time(a.own, S::kTile, TileShape<NK>::kBytes, p->dtype, 1), a.own * (BEST ? 24.0 : 8.0));
+    const uint64_t rest = a.cut.splits > 1 ? (uint64_t)a.cut.parted() * a.own : 0, parts = rest * a.cut.splits;
+    f.sums = (uint32_t)(a.cut.splits > 1 ? a.cut.whole + div_up(rest, kThreads) : a.cut.tiles);
     Carve c = {base, 0};
-    LabelArgs unused = {};
-    if (!a) a = &unused;
     f.sets = row_sets(p, c);
-    a->x = f.sets.x.rows, a->w = f.sets.w.rows;
-    a->splits = f.split.splits, a->per_split = f.split.per_split;
-    if (f.split.splits > 1) {
-        a->part = c.take<float2>((uint64_t)f.split.splits * p->rays);
-        if (best) a->best = c.take<int4>((uint64_t)f.split.splits * p->rays);
-        else a->target_logit = c.take<float>(p->rays);
+    a.x = f.sets.x.rows, a.w = f.sets.w.rows;
+    if (parts) {
+        a.part = c.take<float2>(parts);
+        if (BEST) a.best = c.take<int4>(parts);
+        else a.target_logit = c.take<float>(rest);
     }
-    if (best) {
-        a->bounds = c.take<float>(2 * kBoundBlocks);
-        a->near_count = c.take<uint32_t>(1);
-        a->near_list = c.take<uint32_t>(p->rays);
-        a->near_floor = c.take<float>(p->rays);
+    if (BEST) {
+        a.bounds = c.take<float>(2 * kBoundBlocks);
+        a.near_count = c.take<uint32_t>(1);
+        a.near_list = c.take<uint32_t>(p->rays);
+        a.near_floor = c.take<float>(p->rays);
     } else if (p->reduction != DST_REDUCE_NONE) {
-        a->sums = c.take<double>(f.blocks);
-        a->counts = c.take<uint32_t>(f.blocks);
+        a.sums = c.take<double>(f.sums);
+        a.counts = c.take<uint32_t>(f.sums);
     }
     f.bytes = c.used;
     return f;
@@ -676,32 +679,43 @@ template <class TY, int NK> ForwardPlan forward_plan(const DstLabelParams *p, bo
 
 struct BackwardPlan {
     Sets sets;
-    Split split;
     bool few;
-    int64_t tiles;
     uint64_t bytes;
 };
-// dx: the rays are the own rows; else the labels
-template <class TY, int NK> BackwardPlan backward_plan(const DstLabelParams *p, bool dx, char *base, LabelArgs *a) {
+// DX: the rays are the own rows; else the labels
+template <class TY, int NK, bool DX> BackwardPlan backward_plan(const DstLabelParams *p, LabelArgs &a, char *base) {
     typedef Shapes<TY, NK> S;
-    const int64_t own = dx ? p->rays : p->labels, streamed = dx ? p->labels : p->rays;
+    constexpr int QB = backward_blocks<TY, NK>();
+    const int64_t own = DX ? p->rays : p->labels, streamed = div_up(DX ? p->labels : p->rays, S::kTile);
     BackwardPlan b;
-    b.few = few_rows(own, S::kBackward, div_up(streamed, S::kTile));
-    b.tiles = div_up(own, b.few ? kWaves * 16 : S::kBackward);
-    b.split = split_tiles(b.tiles, div_up(streamed, S::kTile));
+    b.few = few_rows(div_up(own, S::kBackward), streamed);
+    a.own = b.few ? kWaves * 16 : S::kBackward;
+    const void *kernel;
+    if constexpr (DX) kernel = b.few ? (const void *)&k_label_dx<TY, NK, 1> : (const void *)&k_label_dx<TY, NK, QB>;
+    else kernel = b.few ? (const void *)&k_label_dw<TY, NK, 1> : (const void *)&k_label_dw<TY, NK, QB>;
+    a.cut = cut_tiles(div_up(own, a.own), streamed, slots_of(kernel), tile_time(a.own, S::kTile, TileShape<NK>::kBytes, p->dtype, 2),
+                      a.own * (p->channels + 1) * 4.0);
+    const uint64_t parts = a.cut.splits > 1 ? (uint64_t)a.cut.parted() * a.own * a.cut.splits : 0;
     Carve c = {base, 0};
-    LabelArgs unused = {};
-    if (!a) a = &unused;
     b.sets = row_sets(p, c);
-    a->x = b.sets.x.rows, a->w = b.sets.w.rows;
-    a->splits = b.split.splits, a->per_split = b.split.per_split;
-    if (b.split.splits > 1) {
-        a->out_part = c.take<float>((uint64_t)b.split.splits * own * p->channels);
-        if (!dx) a->bias_part = c.take<float>((uint64_t)b.split.splits * own);
+    a.x = b.sets.x.rows, a.w = b.sets.w.rows;
+    if (parts) {
+        a.out_part = c.take<float>(parts * p->channels);
+        if (!DX) a.bias_part = c.take<float>(parts);
     }
     b.bytes = c.used;
     return b;
 }
+
+// The output row of a parted row
+struct LabelRow {
+    int64_t first, rows;
+    int own;
+    __device__ int64_t operator()(int tile, int row) const {
+        const int64_t r = first + (int64_t)tile * own + row;
+        return r < rows ? r : -1;
+    }
+};
 
 int check_workspace(const DstLabelParams *p, uint64_t need) {
     if (need == 0) return DST_OK;
@@ -721,12 +735,13 @@ uint64_t dst_label_workspace_bytes(const DstLabelParams *p, int pass) {
     with_type(p, [&](auto ty, auto nk) {
         typedef decltype(ty) TY;
         constexpr int NK = decltype(nk)::value;
+        LabelArgs a = {};
         if (pass == DST_PASS_BACKWARD) {
-            const uint64_t x = p->grad_features ? backward_plan<TY, NK>(p, true, nullptr, nullptr).bytes : 0;
-            const uint64_t w = p->grad_weight || p->grad_bias ? backward_plan<TY, NK>(p, false, nullptr, nullptr).bytes : 0;
+            const uint64_t x = p->grad_features ? backward_plan<TY, NK, true>(p, a, nullptr).bytes : 0;
+            const uint64_t w = p->grad_weight || p->grad_bias ? backward_plan<TY, NK, false>(p, a, nullptr).bytes : 0;
             bytes = x > w ? x : w;
         } else {
-            bytes = forward_plan<TY, NK>(p, pass == DST_PASS_BEST, nullptr, nullptr).bytes;
+            bytes = pass == DST_PASS_BEST ? forward_plan<TY, NK, true>(p, a, nullptr).bytes : forward_plan<TY, NK, false>(p, a, nullptr).bytes;
         }
         return DST_OK;
     });
@@ -742,23 +757,23 @@ int dst_label_loss_forward(const DstLabelParams *p, void *stream) {
         typedef decltype(ty) TY;
         constexpr int NK = decltype(nk)::value;
         LabelArgs a = arguments(p);
-        const ForwardPlan f = forward_plan<TY, NK>(p, false, (char *)p->workspace, &a);
+        const ForwardPlan f = forward_plan<TY, NK, false>(p, a, (char *)p->workspace);
         if (int rc = check_workspace(p, f.bytes)) return rc;
         if (p->reduction == DST_REDUCE_NONE) a.rows = p->loss;
         const hipStream_t s = (hipStream_t)stream;
-        if (f.tiles > 0) {
+        if (a.cut.tiles > 0) {
             prepare(f.sets.x, s), prepare(f.sets.w, s);
-            const dim3 grid((uint32_t)(f.tiles * a.splits));
+            const dim3 grid((uint32_t)a.cut.blocks());
             if (f.few) k_label_forward<TY, NK, 1, false><<<grid, kThreads, 0, s>>>(a);
             else k_label_forward<TY, NK, forward_blocks<TY, NK>(), false><<<grid, kThreads, 0, s>>>(a);
             DST_OP_LAUNCH("label loss");
-            if (a.splits > 1) {
-                k_label_join<false><<<dim3((uint32_t)f.blocks), kThreads, 0, s>>>(a);
+            if (a.cut.splits > 1) {
+                k_label_join<false><<<dim3(f.sums - (uint32_t)a.cut.whole), kThreads, 0, s>>>(a);
                 DST_OP_LAUNCH("label loss, joining");
             }
         }
         if (p->reduction != DST_REDUCE_NONE) {
-            k_label_mean<<<1, kThreads, 0, s>>>(a.sums, a.counts, (uint32_t)(f.tiles > 0 ? f.blocks : 0), p->reduction == DST_REDUCE_MEAN,
+            k_label_mean<<<1, kThreads, 0, s>>>(a.sums, a.counts, f.sums, p->reduction == DST_REDUCE_MEAN,
                                                p->loss, p->inverse);
             DST_OP_LAUNCH("label loss, summing");
         }
@@ -783,12 +798,12 @@ int dst_label_loss_backward(const DstLabelParams *p, void *stream) {
             const bool dx = pass == 0;
             if (dx ? !p->grad_features || p->rays == 0 : !p->grad_weight && !p->grad_bias) continue;
             LabelArgs a = arguments(p);
-            const BackwardPlan b = backward_plan<TY, NK>(p, dx, (char *)p->workspace, &a);
+            const BackwardPlan b = dx ? backward_plan<TY, NK, true>(p, a, (char *)p->workspace) : backward_plan<TY, NK, false>(p, a, (char *)p->workspace);
             if (int rc = check_workspace(p, b.bytes)) return rc;
             a.upstream = p->upstream, a.upstream_rows = p->reduction == DST_REDUCE_NONE;
             a.inverse = a.upstream_rows ? nullptr : p->inverse;
             a.out = dx ? p->grad_features : p->grad_weight, a.bias_out = p->grad_bias;
-            const dim3 grid((uint32_t)(b.tiles * a.splits));
+            const dim3 grid((uint32_t)a.cut.blocks());
             if (!copied) prepare(b.sets.x, s), prepare(b.sets.w, s);   // (both passes have the copies in the same place)
             copied = true;
             if (dx && b.few) k_label_dx<TY, NK, 1><<<grid, kThreads, 0, s>>>(a);
@@ -796,11 +811,9 @@ int dst_label_loss_backward(const DstLabelParams *p, void *stream) {
             else if (b.few) k_label_dw<TY, NK, 1><<<grid, kThreads, 0, s>>>(a);
             else k_label_dw<TY, NK, QB><<<grid, kThreads, 0, s>>>(a);
             DST_OP_LAUNCH("label gradient");
-            if (a.splits > 1) {
-                const int64_t n = (dx ? p->rays : (int64_t)p->labels) * p->channels;
-                sum_parts(a.out_part, (E *)a.out, n, a.bias_part, dx ? nullptr : p->grad_bias, p->labels, a.splits, s);
-                DST_OP_LAUNCH("label gradient, summing");
-            }
+            const LabelRow to = {(int64_t)a.cut.whole * a.own, dx ? p->rays : (int64_t)p->labels, a.own};
+            sum_parts(Parts<E>{a.out_part, (E *)a.out, p->channels}, Parts<float>{a.bias_part, dx ? nullptr : p->grad_bias, 1}, a.cut, a.own, to, s);
+            DST_OP_LAUNCH("label gradient, summing");
         }
         return (int)DST_OK;
     };
@@ -816,17 +829,17 @@ int dst_label_best(const DstLabelParams *p, void *stream) {
         typedef decltype(ty) TY;
         constexpr int NK = decltype(nk)::value;
         LabelArgs a = arguments(p);
-        const ForwardPlan f = forward_plan<TY, NK>(p, true, (char *)p->workspace, &a);
+        const ForwardPlan f = forward_plan<TY, NK, true>(p, a, (char *)p->workspace);
         if (int rc = check_workspace(p, f.bytes)) return rc;
         a.label = p->best, a.log_prob = p->log_prob;
         const hipStream_t s = (hipStream_t)stream;
         prepare(f.sets.x, s), prepare(f.sets.w, s);
         k_label_bounds<TY><<<kBoundBlocks, kThreads, 0, s>>>(a, const_cast<float *>(a.bounds));
-        const dim3 grid((uint32_t)(f.tiles * a.splits));
+        const dim3 grid((uint32_t)a.cut.blocks());
         if (f.few) k_label_forward<TY, NK, 1, true><<<grid, kThreads, 0, s>>>(a);
         else k_label_forward<TY, NK, forward_blocks<TY, NK>(), true><<<grid, kThreads, 0, s>>>(a);
         DST_OP_LAUNCH("best label");
-        if (a.splits > 1) k_label_join<true><<<dim3((uint32_t)f.blocks), kThreads, 0, s>>>(a);
+        if (a.cut.splits > 1) k_label_join<true><<<dim3(f.sums - (uint32_t)a.cut.whole), kThreads, 0, s>>>(a);
         // (as many workgroups as the device holds; each takes rays off the list until there are no more)
         k_label_near<TY><<<dim3((uint32_t)(p->rays < 2048 ? p->rays : 2048)), kThreads, 0, s>>>(a);
         DST_OP_LAUNCH("best label, near rays");

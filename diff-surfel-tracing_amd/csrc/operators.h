@@ -30,27 +30,73 @@ inline int fragments_of(int channels, int dtype) {
 inline int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline uint64_t align_up(uint64_t bytes) { return (bytes + 255u) & ~(uint64_t)255u; }
 
-// How many parts the streamed tiles are cut into. 256 compute units want about two workgroups each; every part costs a
-// write and a read of the own rows' sums, so a part has at least four tiles while there are any.
+// Who does what. A workgroup takes a tile of own rows against all streamed tiles; the device holds `slots` workgroups at once, and own
+// tiles that do not fill its last round (or are fewer than it holds) are cut into parts of the streamed tiles, whose sums a
+// closing kernel adds: 513 tiles on 512 places would take two rounds. Tiles below `whole` are not cut.
 constexpr int kMostSplits = 512;
-struct Split {
-    int splits, per_split;
+struct Cut {
+    int32_t tiles, whole, splits, per_split;   // per_split: streamed tiles of a part
+    __host__ __device__ int64_t parted() const { return tiles - whole; }
+    int64_t blocks() const { return whole + parted() * splits; }
 };
-inline Split split_tiles(int64_t own_tiles, int64_t stream_tiles) {
-    if (stream_tiles < 1) return Split{1, 1};
-    int64_t want = div_up(kMostSplits, own_tiles > 0 ? own_tiles : 1);
-    const int64_t most = stream_tiles >= 8 ? stream_tiles / 4 : 1;
-    if (want > most) want = most;
-    if (want < 1) want = 1;
-    const int64_t per = div_up(stream_tiles, want);
-    return Split{(int)div_up(stream_tiles, per), (int)per};
+struct Turn {   // a workgroup's
+    int tile, split;
+    bool part;
+};
+__device__ inline Turn turn_of(const Cut &c) {
+    const int b = (int)blockIdx.x - c.whole;
+    if (b < 0) return Turn{(int)blockIdx.x, 0, false};
+    return Turn{c.whole + b / c.splits, b % c.splits, c.splits > 1};
+}
+// Where a part's row lies among the parts: `own` rows a tile.
+__device__ inline int64_t part_row(const Cut &c, const Turn &t, int own, int row) {
+    return ((int64_t)(t.tile - c.whole) * c.splits + t.split) * own + row;
+}
+
+// `tile_us`: what a streamed tile takes a workgroup, about; `own_bytes`: what a part writes and the closing kernel reads. The parts are those
+// of the shortest time by this count: rounds of workgroups, each of its part's tiles and two tiles' worth of beginning and
+// end; then the closing kernel, 4 us and the parts' bytes at 4 TB/s.
+inline Cut cut_tiles(int64_t own_tiles, int64_t stream_tiles, int slots, double tile_us, double own_bytes, bool ragged = false) {
+    Cut c = {(int)own_tiles, (int)own_tiles, 1, (int)(stream_tiles > 0 ? stream_tiles : 1)};
+    // (of ragged rows about half is there: tiles that fill the places once even out by themselves, fewer are cut finer)
+    if (ragged && own_tiles >= slots) return c;
+    if (ragged) slots *= 2;
+    const int64_t rest = own_tiles % slots;
+    if (rest == 0 || stream_tiles < 4) return c;
+    double best = (stream_tiles + 2) * tile_us;
+    for (int rounds = 1; rounds <= 8; ++rounds) {
+        int64_t want = rounds * (int64_t)slots / rest;
+        if (want > kMostSplits) want = kMostSplits;
+        if (want > stream_tiles / 2) want = stream_tiles / 2;
+        if (want < 2) continue;
+        const int64_t per = div_up(stream_tiles, want), splits = div_up(stream_tiles, per);
+        const double us = div_up(rest * splits, slots) * (per + 2) * tile_us + 4.0 + 2.0 * rest * splits * own_bytes / 4e6;
+        if (splits > 1 && us < best) best = us, c.whole = (int)(own_tiles - rest), c.splits = (int)splits, c.per_split = (int)per;
+    }
+    return c;
+}
+// Workgroups of a kernel that the current device runs side by side: one or two on a compute unit. (A third hides some latency but has
+// no more of the matrix units: counted as a place of its own it made the parts smaller and the kernels 6 % slower.)
+inline int slots_of(const void *kernel) {
+    int each = 0, units = 0, device = 0;
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&each, kernel, 256, 0) != hipSuccess || each < 1 || hipGetDevice(&device) != hipSuccess ||
+        hipDeviceGetAttribute(&units, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || units < 1) {
+        (void)hipGetLastError();
+        return 512;
+    }
+    return (each < 2 ? each : 2) * units;
+}
+// What a streamed tile takes a workgroup, about: `products` of own x tile x depth at 40 % of a compute unit's rate, shared by two
+// workgroups, and the exponentials.
+inline double tile_time(int own, int tile, int depth_bytes, int dtype, int products) {
+    const double flops = 2.0 * own * tile * (depth_bytes / value_size(dtype)) * products;
+    return 2.0 * (flops / (dtype == DST_DTYPE_F32 ? 0.4e6 : 4e6) + own * tile * 1.6e-5);
 }
 
 // Whether the own rows are few: blocks of 16 * QB rows a wave would leave compute units without a workgroup, however the streamed
-// rows are split; one block of 16 a wave then makes more, shorter ones.
-inline bool few_rows(int64_t rows, int own, int64_t stream_tiles) {
-    const int64_t most = stream_tiles >= 8 ? stream_tiles / 4 : 1;
-    return div_up(rows, own) * most < 256;
+// rows are cut; one block of 16 a wave then makes more, shorter ones.
+inline bool few_rows(int64_t own_tiles, int64_t stream_tiles) {
+    return own_tiles * (stream_tiles >= 8 ? stream_tiles / 4 : 1) < 256;
 }
 
 // Pieces of a workspace, in order.
@@ -64,23 +110,32 @@ struct Carve {
     }
 };
 
-// out[i] = sum of part[s][i], always in the same order. Two arrays in one launch (the second may be empty): a launch costs more than
-// either sum. kLanes parts are added side by side where there are many (a few thousand sums of 450 parts: 6 us with 8 lanes,
-// 115 with one, whose loads wait for each other).
-template <class E, class E2, int kLanes>
-__global__ __launch_bounds__(256) void k_sum_parts(const float *part, E *out, int64_t n, const float *part2, E2 *out2, int64_t n2, int splits) {
+// The sums of parts, always in the same order. Two arrays of rows in one launch (a launch costs more than either sum): `width`
+// values a row, out[to(i)] of the i-th parted row; to(i) < 0: no such row. kLanes parts are added side by side where there are many
+// (a few thousand sums of 450 parts: 7 us with 8 lanes, 115 with one, whose loads wait for each other).
+template <class E> struct Parts {
+    const float *part;
+    E *out;       // nullptr: not wanted
+    int32_t width;
+};
+template <class E, class E2, int kLanes, class To>
+__global__ __launch_bounds__(256) void k_sum_parts(Parts<E> a, Parts<E2> b, Cut cut, int own, To to) {
     constexpr int kColumns = 256 / kLanes;
     __shared__ float lds[256];
     const int column = threadIdx.x % kColumns, lane = threadIdx.x / kColumns;
-    const int64_t blocks = (n + kColumns - 1) / kColumns, all = blocks + (n2 + kColumns - 1) / kColumns;
-    for (int64_t b = blockIdx.x; b < all; b += gridDim.x) {
-        const bool second = b >= blocks;
-        const int64_t i = (second ? b - blocks : b) * kColumns + column, size = second ? n2 : n;
-        const float *from = (second ? part2 : part) + i;
+    const uint32_t rows = (uint32_t)cut.parted() * own;
+    const uint32_t n = a.out ? rows * a.width : 0u, n2 = b.out ? rows * b.width : 0u;
+    const uint32_t blocks = (n + kColumns - 1) / kColumns, all = blocks + (n2 + kColumns - 1) / kColumns;
+    for (uint32_t at = blockIdx.x; at < all; at += gridDim.x) {
+        const bool second = at >= blocks;
+        const uint32_t i = (second ? at - blocks : at) * kColumns + column, width = second ? b.width : a.width;
+        const uint32_t row = i / width, tile = row / (uint32_t)own, size = own * width;
+        const bool there = i < (second ? n2 : n);
+        const float *from = (second ? b.part : a.part) + (uint64_t)tile * cut.splits * size + (i - tile * size);
         float s = 0.0f;
-        if (i < size)
+        if (there)
 #pragma unroll 4
-            for (int k = lane; k < splits; k += kLanes) s += from[(int64_t)k * size];
+            for (int k = lane; k < cut.splits; k += kLanes) s += from[(uint64_t)k * size];
         if constexpr (kLanes > 1) {
             __syncthreads();
             lds[threadIdx.x] = s;
@@ -89,22 +144,20 @@ __global__ __launch_bounds__(256) void k_sum_parts(const float *part, E *out, in
 #pragma unroll
             for (int k = 1; k < kLanes; ++k) s += lds[k * kColumns + column];
         }
-        if (i < size) {
-            if (second) out2[i] = (E2)s;
-            else out[i] = (E)s;
-        }
+        if (!there) continue;
+        const int64_t where = to((int)tile, (int)(row - tile * own));
+        if (where < 0) continue;
+        if (second) b.out[where * width + (i - row * width)] = (E2)s;
+        else a.out[where * width + (i - row * width)] = (E)s;
     }
 }
-template <class E, class E2>
-inline void sum_parts(const float *part, E *out, int64_t n, const float *part2, E2 *out2, int64_t n2, int splits, hipStream_t s) {
-    if (!out) n = 0;
-    if (!out2) n2 = 0;
-    if (n + n2 == 0) return;
-    const int columns = splits >= 16 ? 32 : 256;
-    const int64_t blocks = div_up(n, columns) + div_up(n2, columns);
+template <class E, class E2, class To> inline void sum_parts(Parts<E> a, Parts<E2> b, const Cut &cut, int own, To to, hipStream_t s) {
+    if (cut.splits < 2 || (!a.out && !b.out)) return;
+    const int columns = cut.splits >= 16 ? 32 : 256;
+    const int64_t rows = cut.parted() * own, blocks = div_up(a.out ? rows * a.width : 0, columns) + div_up(b.out ? rows * b.width : 0, columns);
     const dim3 grid((uint32_t)(blocks < 8192 ? blocks : 8192));
-    if (splits >= 16) k_sum_parts<E, E2, 8><<<grid, 256, 0, s>>>(part, out, n, part2, out2, n2, splits);
-    else k_sum_parts<E, E2, 1><<<grid, 256, 0, s>>>(part, out, n, part2, out2, n2, splits);
+    if (cut.splits >= 16) k_sum_parts<E, E2, 8><<<grid, 256, 0, s>>>(a, b, cut, own, to);
+    else k_sum_parts<E, E2, 1><<<grid, 256, 0, s>>>(a, b, cut, own, to);
 }
 
 // Rows that the kernels cannot read where they lie, copied: (batches, heads, rows) of whole words, zeros behind the channels.
