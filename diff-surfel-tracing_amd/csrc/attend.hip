@@ -81,7 +81,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     constexpr int NM = depth_blocks<TY, NK>();
     __shared__ alignas(16) char tile_k[T::kRows * T::kPitch], tile_v[T::kRows * T::kPitch];
     __shared__ alignas(16) float tile_mask[T::kRows];   // 0, or -inf of a row behind the length, which takes it out of every sum
-    const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, g = lane >> 4, wave = wave_number();
     const Turn turn = turn_of(a.cut);
     const Place p = place_of(a, turn.tile);
     const int row0 = p.tile * (kWaves * 16 * QB) + wave * 16 * QB;
@@ -89,15 +89,15 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     const int last = turn.part ? min(p.length, first + a.cut.per_split * T::kRows) : p.length;
 
     Stage<NK> stage_k, stage_v;
-    stage_k.begin(a.k);
-    stage_v.begin(a.v);
+    stage_k.begin(a.k, tile_base(a.k, first, p.batch, p.kv));
+    stage_v.begin(a.v, tile_base(a.v, first, p.batch, p.kv));
     auto fetch = [&](int at) {
-        stage_k.load(tile_base(a.k, at, p.batch, p.kv), last - at);
-        stage_v.load(tile_base(a.v, at, p.batch, p.kv), last - at);
+        stage_k.load(last - at);
+        stage_v.load(last - at);
     };
     if (first < last) fetch(first);
     Own<TY, NK, QB> own;
-    own.load(a.q, tile_base(a.q, row0, p.batch, p.kv), a.rows - row0);
+    own.load(a.q, tile_base<true>(a.q, row0, p.batch, p.kv), a.rows - row0);
     carry_scale(own, a);
     float m[QB], l[QB];
     f4 out[QB][NM];
@@ -128,13 +128,13 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
 #pragma unroll
             for (int q = 0; q < QB; ++q) {
                 const f4 u = s[0][q], v = s[1][q];
-                top[q] = a.c * fmaxf(fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])), fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
+                top[q] = a.c * larger(largest(u), largest(v));
                 raise |= top[q] > m[q] + kSlack;
             }
             if (__any(raise)) {
 #pragma unroll
                 for (int q = 0; q < QB; ++q) {
-                    const float to = fmaxf(m[q], max_group(top[q])), by = exp2_of(m[q] - finite_or_zero(to));
+                    const float to = larger(m[q], max_group(top[q])), by = exp2_of(m[q] - finite_or_zero(to));
                     m[q] = to;
                     l[q] *= by;
 #pragma unroll
@@ -291,7 +291,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     constexpr int NM = depth_blocks<TY, NK>();
     __shared__ alignas(16) char tile_k[T::kRows * T::kPitch], tile_v[T::kRows * T::kPitch];
     __shared__ alignas(16) float tile_mask[T::kRows];   // 0, or -inf of a row behind the length, which takes it out of every sum
-    const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, g = lane >> 4, wave = wave_number();
     const Turn turn = turn_of(a.cut);
     const Place p = place_of(a, turn.tile);
     const int row0 = p.tile * (kWaves * 16 * QB) + wave * 16 * QB;
@@ -299,19 +299,19 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     const int last = !a.dq ? 0 : turn.part ? min(p.length, first + a.cut.per_split * T::kRows) : p.length;
 
     Stage<NK> stage_k, stage_v;
-    stage_k.begin(a.k);
-    stage_v.begin(a.v);
+    stage_k.begin(a.k, tile_base(a.k, first, p.batch, p.kv));
+    stage_v.begin(a.v, tile_base(a.v, first, p.batch, p.kv));
     auto fetch = [&](int at) {
-        stage_k.load(tile_base(a.k, at, p.batch, p.kv), last - at);
-        stage_v.load(tile_base(a.v, at, p.batch, p.kv), last - at);
+        stage_k.load(last - at);
+        stage_v.load(last - at);
     };
     if (first < last) fetch(first);
     Own<TY, NK, QB> own, up;
     float delta[QB], lse2[QB];
-    up.load(a.up, tile_base(a.up, row0, p.batch, p.kv), a.rows - row0);
-    own.load(a.o, tile_base(a.o, row0, p.batch, p.kv), a.rows - row0);
+    up.load(a.up, tile_base<true>(a.up, row0, p.batch, p.kv), a.rows - row0);
+    own.load(a.o, tile_base<true>(a.o, row0, p.batch, p.kv), a.rows - row0);
     deltas<TY, NK, QB>(own, up, delta);
-    own.load(a.q, tile_base(a.q, row0, p.batch, p.kv), a.rows - row0);
+    own.load(a.q, tile_base<true>(a.q, row0, p.batch, p.kv), a.rows - row0);
     carry_scale(own, a);
     f4 out[QB][NM];
 #pragma unroll
@@ -372,7 +372,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     constexpr int NM = depth_blocks<TY, NK>();
     __shared__ alignas(16) char tile_q[T::kRows * T::kPitch], tile_o[T::kRows * T::kPitch];
     __shared__ alignas(16) float tile_lse2[T::kRows], tile_delta[T::kRows];
-    const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, g = lane >> 4, wave = wave_number();
     const Turn turn = turn_of(a.cut);
     const Place p = place_of(a, turn.tile);
     const int tile0 = p.tile * (kWaves * 16 * QB), row0 = tile0 + wave * 16 * QB;
@@ -380,12 +380,12 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     const int last = tile0 >= p.length ? 0 : turn.part ? min(a.rows, first + a.cut.per_split * T::kRows) : a.rows;
 
     Stage<NK> stage_q, stage_o;
-    stage_q.begin(a.q);
-    stage_o.begin(a.up);
+    stage_q.begin(a.q, tile_base<true>(a.q, first, p.batch, p.kv));
+    stage_o.begin(a.up, tile_base<true>(a.up, first, p.batch, p.kv));
     float stage_lse2 = kInf, stage_delta = 0.0f;
     auto fetch = [&](int at) {
-        stage_q.load(tile_base(a.q, at, p.batch, p.kv), last - at);
-        stage_o.load(tile_base(a.up, at, p.batch, p.kv), last - at);
+        stage_q.load(last - at);
+        stage_o.load(last - at);
         if ((int)threadIdx.x < T::kRows) {
             const int row = at + threadIdx.x;
             stage_lse2 = row < last ? a.lse2[stat_row(a, p, row)] : kInf;

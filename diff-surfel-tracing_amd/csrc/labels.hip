@@ -54,12 +54,13 @@ constexpr int kBoundBlocks = 64;
 template <class TY, int NK> constexpr int forward_blocks() { return NK <= 1 ? 4 : NK <= 8 ? 2 : 1; }
 template <class TY, int NK> constexpr int backward_blocks() { return NK <= 1 ? (TY::kSize == 2 ? 2 : 4) : NK <= 4 ? 2 : 1; }
 
+// The one value that the rays share
+__device__ inline float upstream_value(const LabelArgs &a) { return a.upstream[0] * a.inverse[0]; }
 // The upstream gradient of a ray's loss: 0 where it is ignored, NaN where its label is none.
 __device__ inline float upstream_of(const LabelArgs &a, int64_t row, int64_t t) {
     if (t == a.ignore) return 0.0f;
     if (t < 0 || t >= a.labels) return __builtin_nanf("");
-    const float u = a.upstream[a.upstream_rows ? row : 0];
-    return a.inverse ? u * a.inverse[0] : u;
+    return a.upstream_rows ? a.upstream[row] : upstream_value(a);
 }
 
 // ---- forward --------------------------------------------------------------------------------------------------------
@@ -135,17 +136,17 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
     typedef TileShape<NK> T;
     __shared__ alignas(16) char tile[T::kRows * T::kPitch > kThreads * 12 ? T::kRows * T::kPitch : kThreads * 12];
     __shared__ alignas(16) float tile_bias[T::kRows];
-    const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, g = lane >> 4, wave = wave_number();
     const Turn turn = turn_of(a.cut);
     const int64_t row0 = (int64_t)turn.tile * (kWaves * 16 * QB) + wave * 16 * QB;
     const int first = turn.part ? turn.split * a.cut.per_split * T::kRows : 0;
     const int last = turn.part ? min(a.labels, first + a.cut.per_split * T::kRows) : a.labels;   // (the host keeps labels below 2^30)
 
     Stage<NK> stage;
-    stage.begin(a.w);
+    stage.begin(a.w, tile_base(a.w, first));
     float stage_bias = 0.0f;   // of a row behind the table's end: -inf, which takes it out of every sum
     auto fetch = [&](int at) {
-        stage.load(tile_base(a.w, at), last - at);
+        stage.load(last - at);
         if ((int)threadIdx.x < T::kRows) stage_bias = at + (int)threadIdx.x >= last ? -kInf : a.bias ? a.bias[at + threadIdx.x] : 0.0f;
     };
     fetch(first);
@@ -163,8 +164,13 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
         if ((int)threadIdx.x < T::kRows) tile_bias[threadIdx.x] = stage_bias;
         __syncthreads();
         if (at + T::kRows < last) fetch(at + T::kRows);
+        float before[QB];   // the best up to this tile
+        int place[QB];      // of the best in this tile, less 4 g
+#pragma unroll
+        for (int q = 0; q < QB; ++q) before[q] = best[q], place[q] = 0;
 #pragma unroll
         for (int pair = 0; pair < T::kBlocks; pair += 2) {
+            if (NK <= 2 && at + pair * 16 >= last) break;   // (short rows: the work on a logit is most of all work)
             f4 s[2][QB];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
@@ -183,14 +189,12 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
                         for (int r = 0; r < 4; ++r) {
                             const float v = s[j][q][r];
                             second[q] = __builtin_amdgcn_fmed3f(v, best[q], second[q]);
-                            label[q] = v > best[q] ? at + (pair + j) * 16 + 4 * g + r : label[q];
-                            best[q] = fmaxf(best[q], v);
+                            place[q] = v > best[q] ? (pair + j) * 16 + r : place[q];
+                            best[q] = larger(best[q], v);
                         }
                     top = best[q] * kLog2E;
                 } else {
-                    const f4 u = s[0][q], v = s[1][q];
-                    top = fmaxf(fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])), fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]))) * kLog2E;
-                    top = fmaxf(top, run[q].m);
+                    top = larger(larger(largest(s[0][q]), largest(s[1][q])) * kLog2E, run[q].m);
                 }
                 // (eight at a time, added in pairs: the running sum sees an eighth of the additions)
                 const float use = finite_or_zero(top);
@@ -204,6 +208,9 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
                 run[q].m = top;
             }
         }
+        if constexpr (BEST)
+#pragma unroll
+            for (int q = 0; q < QB; ++q) label[q] = best[q] > before[q] ? at + 4 * g + place[q] : label[q];
         __syncthreads();
     }
 
@@ -391,17 +398,17 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     constexpr int NM = depth_blocks<TY, NK>();
     __shared__ alignas(16) char tile[T::kRows * T::kPitch];
     __shared__ alignas(16) float tile_bias[T::kRows];
-    const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, g = lane >> 4, wave = wave_number();
     const Turn turn = turn_of(a.cut);
     const int64_t row0 = (int64_t)turn.tile * (kWaves * 16 * QB) + wave * 16 * QB;
     const int first = turn.part ? turn.split * a.cut.per_split * T::kRows : 0;
     const int last = turn.part ? min(a.labels, first + a.cut.per_split * T::kRows) : a.labels;
 
     Stage<NK> stage;
-    stage.begin(a.w);
+    stage.begin(a.w, tile_base(a.w, first));
     float stage_bias = 0.0f;   // of a row behind the table's end: -inf, which takes it out of every sum
     auto fetch = [&](int at) {
-        stage.load(tile_base(a.w, at), last - at);
+        stage.load(last - at);
         if ((int)threadIdx.x < T::kRows) stage_bias = at + (int)threadIdx.x >= last ? -kInf : a.bias ? a.bias[at + threadIdx.x] : 0.0f;
     };
     fetch(first);
@@ -439,7 +446,8 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         float e = exp2_of(__builtin_fmaf(p[j][q][r], kLog2E, -lse2[q]));
-                        e -= label[q] - at == (pair + j) * 16 + r ? 1.0f : 0.0f;
+                        // (of 32-bit rows the label's row is taken off the sum at the end; 16 bits would lose p - 1 where p is near 1)
+                        if constexpr (TY::kSize == 2) e -= label[q] - at == (pair + j) * 16 + r ? 1.0f : 0.0f;
                         p[j][q][r] = e;
                     }
             }
@@ -449,12 +457,20 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     }
     typedef typename TY::E E;
     const bool four = (a.d & 3) == 0;
+    typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
 #pragma unroll
     for (int q = 0; q < QB; ++q) {
         const int64_t row = row0 + q * 16 + (lane & 15);
         if (row >= a.rays) continue;
+        const int64_t t = a.target[row];
+        const bool label_here = TY::kSize == 4 && t >= first && t < last;   // (of a part: its labels' alone)
+        const float *label_row = reinterpret_cast<const float *>(tile_base(a.w, label_here ? t : 0));
 #pragma unroll
         for (int m = 0; m < NM; ++m) {
+            if (label_here) {
+                const int at = m * 16 + 4 * g;
+                if (at < 4 * a.w.words) out[q][m] -= *reinterpret_cast<const f4u *>(label_row + at);
+            }
             f4 v = out[q][m] * up[q];
             if (up[q] == 0.0f) v = f4{0.0f, 0.0f, 0.0f, 0.0f};   // (an ignored ray's channels may hold anything)
             if (turn.part) store_four(a.out_part + part_row(a.cut, turn, kWaves * 16 * QB, wave * 16 * QB + q * 16 + (lane & 15)) * a.d, m * 16 + 4 * g, a.d, v, four);
@@ -464,20 +480,21 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
 }
 
 // dw and db: labels as own rows, the rays streamed.
-template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void k_label_dw(LabelArgs a) {
+// ONE: the rays share one upstream gradient, which multiplies the sums at the end; else each ray's weights have its own.
+template <class TY, int NK, int QB, bool ONE> __global__ __launch_bounds__(kThreads) void k_label_dw(LabelArgs a) {
     typedef TileShape<NK> T;
     constexpr int NM = depth_blocks<TY, NK>();
     __shared__ alignas(16) char tile[T::kRows * T::kPitch];
     __shared__ alignas(16) float tile_lse2[2][T::kRows], tile_up[2][T::kRows];
     __shared__ alignas(16) int tile_label[2][T::kRows];
-    const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, g = lane >> 4, wave = wave_number();
     const Turn turn = turn_of(a.cut);
     const int row0 = turn.tile * (kWaves * 16 * QB) + wave * 16 * QB;   // (the host keeps labels below 2^30)
     const int64_t first = turn.part ? (int64_t)turn.split * a.cut.per_split * T::kRows : 0;
     const int64_t last = turn.part ? min(a.rays, first + (int64_t)a.cut.per_split * T::kRows) : a.rays;
 
     Stage<NK> stage;
-    stage.begin(a.x);
+    stage.begin(a.x, tile_base(a.x, first));
     // Of every ray: lse (+inf where it is ignored or behind the end, which makes its weights 0), upstream gradient, label. They are a tile
     // ahead of the channels, which are read only of rays that are not ignored: those of the others may hold anything.
     float stage_lse2 = kInf, stage_up = 0.0f;
@@ -486,7 +503,8 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
         if ((int)threadIdx.x < T::kRows) {
             const int64_t row = at + threadIdx.x, t = row < last ? a.target[row] : a.ignore;
             stage_lse2 = row < last ? a.lse2[row] : kInf;
-            stage_up = row < last ? upstream_of(a, row, t) : 0.0f;
+            if (!ONE) stage_up = row < last ? upstream_of(a, row, t) : 0.0f;
+            else if (t != a.ignore && (t < 0 || t >= a.labels)) stage_lse2 = __builtin_nanf("");
             stage_label = t >= 0 && t < a.labels && t != a.ignore ? (int)t : -1;
         }
     };
@@ -494,7 +512,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
         if ((int)threadIdx.x < T::kRows) tile_lse2[at][threadIdx.x] = stage_lse2, tile_up[at][threadIdx.x] = stage_up, tile_label[at][threadIdx.x] = stage_label;
     };
     auto fetch = [&](int64_t at, int half) {
-        stage.load(tile_base(a.x, at), (int)min(last - at, (int64_t)T::kRows), [&](int r) { return tile_lse2[half][r & (T::kRows - 1)] != kInf; });
+        stage.load((int)min(last - at, (int64_t)T::kRows), [&](int r) { return tile_lse2[half][r & (T::kRows - 1)] != kInf; });
     };
     fetch_stats(first);
     Own<TY, NK, QB> own;
@@ -541,7 +559,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
                     for (int r = 0; r < 4; ++r) {
                         float e = exp2_of(__builtin_fmaf(p[j][q][r], kLog2E, -lse2[r]));
                         e -= labels[r] == v ? 1.0f : 0.0f;
-                        e *= up[r];
+                        if constexpr (!ONE) e *= up[r];
                         p[j][q][r] = e;
                     }
                 }
@@ -562,14 +580,15 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
 #pragma unroll
     for (int q = 0; q < QB; ++q) {
         const int v = row0 + q * 16 + (lane & 15);
-        const float b = sum_group(db[q]);
+        const float by = ONE ? (a.rays > 0 ? upstream_value(a) : 0.0f) : 1.0f;
+        const float b = sum_group(db[q]) * by;
         if (v >= a.labels) continue;
         const int64_t part = part_row(a.cut, turn, kWaves * 16 * QB, wave * 16 * QB + q * 16 + (lane & 15));
         if (g == 0 && a.bias_out) *(turn.part ? a.bias_part + part : a.bias_out + v) = b;
 #pragma unroll
         for (int m = 0; m < NM; ++m) {
-            if (turn.part) store_four(a.out_part + part * a.d, m * 16 + 4 * g, a.d, out[q][m], four);
-            else if (a.out) store_four(reinterpret_cast<E *>(a.out) + (int64_t)v * a.d, m * 16 + 4 * g, a.d, out[q][m], four);
+            if (turn.part) store_four(a.out_part + part * a.d, m * 16 + 4 * g, a.d, out[q][m] * by, four);
+            else if (a.out) store_four(reinterpret_cast<E *>(a.out) + (int64_t)v * a.d, m * 16 + 4 * g, a.d, out[q][m] * by, four);
         }
     }
 }
@@ -692,7 +711,8 @@ template <class TY, int NK, bool DX> BackwardPlan backward_plan(const DstLabelPa
     a.own = b.few ? kWaves * 16 : S::kBackward;
     const void *kernel;
     if constexpr (DX) kernel = b.few ? (const void *)&k_label_dx<TY, NK, 1> : (const void *)&k_label_dx<TY, NK, QB>;
-    else kernel = b.few ? (const void *)&k_label_dw<TY, NK, 1> : (const void *)&k_label_dw<TY, NK, QB>;
+    else if (p->reduction == DST_REDUCE_NONE) kernel = b.few ? (const void *)&k_label_dw<TY, NK, 1, false> : (const void *)&k_label_dw<TY, NK, QB, false>;
+    else kernel = b.few ? (const void *)&k_label_dw<TY, NK, 1, true> : (const void *)&k_label_dw<TY, NK, QB, true>;
     a.cut = cut_tiles(div_up(own, a.own), streamed, slots_of(kernel), tile_time(a.own, S::kTile, TileShape<NK>::kBytes, p->dtype, 2),
                       a.own * (p->channels + 1) * 4.0);
     const uint64_t parts = a.cut.splits > 1 ? (uint64_t)a.cut.parted() * a.own * a.cut.splits : 0;
@@ -808,8 +828,10 @@ int dst_label_loss_backward(const DstLabelParams *p, void *stream) {
             copied = true;
             if (dx && b.few) k_label_dx<TY, NK, 1><<<grid, kThreads, 0, s>>>(a);
             else if (dx) k_label_dx<TY, NK, QB><<<grid, kThreads, 0, s>>>(a);
-            else if (b.few) k_label_dw<TY, NK, 1><<<grid, kThreads, 0, s>>>(a);
-            else k_label_dw<TY, NK, QB><<<grid, kThreads, 0, s>>>(a);
+            else if (b.few && a.upstream_rows) k_label_dw<TY, NK, 1, false><<<grid, kThreads, 0, s>>>(a);
+            else if (b.few) k_label_dw<TY, NK, 1, true><<<grid, kThreads, 0, s>>>(a);
+            else if (a.upstream_rows) k_label_dw<TY, NK, QB, false><<<grid, kThreads, 0, s>>>(a);
+            else k_label_dw<TY, NK, QB, true><<<grid, kThreads, 0, s>>>(a);
             DST_OP_LAUNCH("label gradient");
             const LabelRow to = {(int64_t)a.cut.whole * a.own, dx ? p->rays : (int64_t)p->labels, a.own};
             sum_parts(Parts<E>{a.out_part, (E *)a.out, p->channels}, Parts<float>{a.bias_part, dx ? nullptr : p->grad_bias, 1}, a.cut, a.own, to, s);
