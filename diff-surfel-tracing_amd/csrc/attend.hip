@@ -35,9 +35,9 @@ struct AttendArgs {
 // Own blocks of 16 rows a wave. More of them read a streamed tile fewer times from LDS, fewer leave registers for a second wave on a
 // SIMD, which counts for more: the waits of one are the other's work (16384 x 8192, 8 heads of 128, bf16: forward 802 us with 4
 // blocks, 685 with 2; dk and dv 1619 with 2, 1317 with 1).
-template <class TY, int NK> constexpr int forward_blocks() { return NK <= 8 ? 2 : 1; }
-template <class TY, int NK> constexpr int dq_blocks() { return NK <= 4 ? 2 : 1; }
-template <class TY, int NK> constexpr int dkv_blocks() { return NK <= 2 ? 2 : 1; }
+template <class TY, int NK> constexpr int forward_blocks() { return NK * TY::kPlanes <= 8 ? 2 : 1; }
+template <class TY, int NK> constexpr int dq_blocks() { return NK * TY::kPlanes <= 6 ? 2 : 1; }
+template <class TY, int NK> constexpr int dkv_blocks() { return NK * TY::kPlanes <= 3 ? 2 : 1; }
 
 struct Place {   // which own tile, batch and kv head a workgroup has
     int tile, batch, kv, length;
@@ -58,16 +58,25 @@ __device__ inline int64_t out_row(const AttendArgs &a, const Place &p, int row) 
 // Row of lse, delta and the parts
 __device__ inline int64_t stat_row(const AttendArgs &a, const Place &p, int row) { return ((int64_t)p.batch * a.kv_heads + p.kv) * a.rows + row; }
 
-// What own rows carry of the scores' factor: of 32-bit rows all of it (then the scores come out in units of log 2, and a row with
-// one weight gets exactly 1: score less maximum is 0), of 16-bit rows the sign.
+// What own rows carry of the scores' factor: rows in 32 bits all of it, rows of 16 bits or planes the sign. Either way a row with one
+// weight of 32 bits gets exactly 1: its score less the maximum, which is the score, is 0 (the product with c is rounded first).
 template <class TY, int NK, int QB> __device__ inline void carry_scale(Own<TY, NK, QB> &own, const AttendArgs &a) {
 #pragma unroll
     for (int q = 0; q < QB; ++q)
 #pragma unroll
-        for (int k = 0; k < fragments<NK>(); ++k) {
-            if constexpr (TY::kSize == 4) own.f[q][k] = __builtin_bit_cast(u4, __builtin_bit_cast(f4, own.f[q][k]) * a.own_scale);
-            else if (a.flip) own.f[q][k] ^= u4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
-        }
+        for (int k = 0; k < fragments<NK>(); ++k)
+#pragma unroll
+            for (int p = 0; p < TY::kPlanes; ++p) {
+                u4 &w = own.f[q][k].w[p];
+                if constexpr (TY::kDepth == 16) w = __builtin_bit_cast(u4, __builtin_bit_cast(f4, w) * a.own_scale);
+                else if (a.flip) w ^= u4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
+            }
+}
+// The weight of a product of rows, `less` its row's maximum or lse.
+template <class TY> __device__ inline float weight_of(const AttendArgs &a, float s, float less) {
+    if constexpr (TY::kRounds) return exp2_of(__builtin_fmaf(s, a.c, -less));
+    else if constexpr (TY::kPlanes == 3) return exp2_of(s * a.c - less);
+    else return exp2_of(s - less);
 }
 
 // ---- forward --------------------------------------------------------------------------------------------------------
@@ -76,10 +85,10 @@ template <class TY, int NK, int QB> __device__ inline void carry_scale(Own<TY, N
 constexpr float kSlack = 8.0f;
 
 template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void k_attend_forward(AttendArgs a) {
-    typedef TileShape<NK> T;
+    typedef Shape<TY, NK> T;
     typedef typename TY::E E;
     constexpr int NM = depth_blocks<TY, NK>();
-    __shared__ alignas(16) char tile_k[T::kRows * T::kPitch], tile_v[T::kRows * T::kPitch];
+    __shared__ alignas(16) char tile_k[T::kTile], tile_v[T::kTile];
     __shared__ alignas(16) float tile_mask[T::kRows];   // 0, or -inf of a row behind the length, which takes it out of every sum
     const int lane = threadIdx.x & 63, g = lane >> 4, wave = wave_number();
     const Turn turn = turn_of(a.cut);
@@ -88,7 +97,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     const int first = turn.split * a.cut.per_split * T::kRows;
     const int last = turn.part ? min(p.length, first + a.cut.per_split * T::kRows) : p.length;
 
-    Stage<NK> stage_k, stage_v;
+    Stage<TY, NK> stage_k, stage_v;
     stage_k.begin(a.k, tile_base(a.k, first, p.batch, p.kv));
     stage_v.begin(a.v, tile_base(a.v, first, p.batch, p.kv));
     auto fetch = [&](int at) {
@@ -147,7 +156,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[j][q][r] = exp2_of(__builtin_fmaf(s[j][q][r], a.c, -use));
+                    for (int r = 0; r < 4; ++r) s[j][q][r] = weight_of<TY>(a, s[j][q][r], use);
                 const f4 u = s[0][q], v = s[1][q];
                 l[q] += ((u[0] + u[1]) + (u[2] + u[3])) + ((v[0] + v[1]) + (v[2] + v[3]));
             }
@@ -286,10 +295,10 @@ template <class TY, int NK, int QB> __device__ inline void deltas(const Own<TY, 
 
 // dq, and delta for the other kernel: queries as own rows, the memory streamed.
 template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void k_attend_dq(AttendArgs a) {
-    typedef TileShape<NK> T;
+    typedef Shape<TY, NK> T;
     typedef typename TY::E E;
     constexpr int NM = depth_blocks<TY, NK>();
-    __shared__ alignas(16) char tile_k[T::kRows * T::kPitch], tile_v[T::kRows * T::kPitch];
+    __shared__ alignas(16) char tile_k[T::kTile], tile_v[T::kTile];
     __shared__ alignas(16) float tile_mask[T::kRows];   // 0, or -inf of a row behind the length, which takes it out of every sum
     const int lane = threadIdx.x & 63, g = lane >> 4, wave = wave_number();
     const Turn turn = turn_of(a.cut);
@@ -298,7 +307,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     const int first = turn.split * a.cut.per_split * T::kRows;
     const int last = !a.dq ? 0 : turn.part ? min(p.length, first + a.cut.per_split * T::kRows) : p.length;
 
-    Stage<NK> stage_k, stage_v;
+    Stage<TY, NK> stage_k, stage_v;
     stage_k.begin(a.k, tile_base(a.k, first, p.batch, p.kv));
     stage_v.begin(a.v, tile_base(a.v, first, p.batch, p.kv));
     auto fetch = [&](int at) {
@@ -343,7 +352,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
                 for (int q = 0; q < QB; ++q)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        s[j][q][r] = exp2_of(__builtin_fmaf(s[j][q][r], a.c, -lse2[q])) * (dp[q][r] - delta[q]);
+                        s[j][q][r] = weight_of<TY>(a, s[j][q][r], lse2[q]) * (dp[q][r] - delta[q]);
             }
             accumulate<TY, NK, QB, NM>(tile_k, pair, s[0], s[1], out);
         }
@@ -367,10 +376,10 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
 
 // dk and dv: the memory's rows as own rows, the queries streamed.
 template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void k_attend_dkv(AttendArgs a) {
-    typedef TileShape<NK> T;
+    typedef Shape<TY, NK> T;
     typedef typename TY::E E;
     constexpr int NM = depth_blocks<TY, NK>();
-    __shared__ alignas(16) char tile_q[T::kRows * T::kPitch], tile_o[T::kRows * T::kPitch];
+    __shared__ alignas(16) char tile_q[T::kTile], tile_o[T::kTile];
     __shared__ alignas(16) float tile_lse2[T::kRows], tile_delta[T::kRows];
     const int lane = threadIdx.x & 63, g = lane >> 4, wave = wave_number();
     const Turn turn = turn_of(a.cut);
@@ -379,7 +388,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     const int first = turn.split * a.cut.per_split * T::kRows;
     const int last = tile0 >= p.length ? 0 : turn.part ? min(a.rows, first + a.cut.per_split * T::kRows) : a.rows;
 
-    Stage<NK> stage_q, stage_o;
+    Stage<TY, NK> stage_q, stage_o;
     stage_q.begin(a.q, tile_base<true>(a.q, first, p.batch, p.kv));
     stage_o.begin(a.up, tile_base<true>(a.up, first, p.batch, p.kv));
     float stage_lse2 = kInf, stage_delta = 0.0f;
@@ -415,15 +424,15 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
             for (int j = 0; j < 2; ++j) {
 #pragma unroll
                 for (int q = 0; q < QB; ++q) s[j][q] = dp[j][q] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-                product<TY, NK, QB>(tile_q, pair + j, own_k, s[j]);
-                product<TY, NK, QB>(tile_o, pair + j, own_v, dp[j]);
+                product<TY, NK, QB, true>(tile_q, pair + j, own_k, s[j]);
+                product<TY, NK, QB, true>(tile_o, pair + j, own_v, dp[j]);
                 const int at4 = (pair + j) * 16 + 4 * g;
                 const f4 lse2 = *reinterpret_cast<const f4 *>(tile_lse2 + at4), delta = *reinterpret_cast<const f4 *>(tile_delta + at4);
 #pragma unroll
                 for (int q = 0; q < QB; ++q)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float e = exp2_of(__builtin_fmaf(s[j][q][r], a.c, -lse2[r]));
+                        const float e = weight_of<TY>(a, s[j][q][r], lse2[r]);
                         s[j][q][r] = e;
                         dp[j][q][r] = e * (dp[j][q][r] - delta[r]);
                     }
@@ -480,6 +489,8 @@ int check(const DstAttendParams *p) {
     return DST_OK;
 }
 
+int longest(const DstAttendParams *p) { return p->channels > p->value_channels ? p->channels : p->value_channels; }
+
 AttendArgs arguments(const DstAttendParams *p) {
     AttendArgs a = {};
     a.lengths = p->lengths;
@@ -491,45 +502,31 @@ AttendArgs arguments(const DstAttendParams *p) {
     // -inf what it is)
     a.c = __builtin_fabsf(p->scale) * kLog2E;
     if (a.c < 1.1754944e-38f) a.c = 1.1754944e-38f;
-    if (p->dtype == DST_DTYPE_F32) a.own_scale = a.flip ? -a.c : a.c, a.c = 1.0f;
+    if (p->dtype == DST_DTYPE_F32 && longest(p) <= kLongest32) a.own_scale = a.flip ? -a.c : a.c, a.c = 1.0f;
     a.out = p->out, a.lse2 = p->lse;
     a.all_rows = (int64_t)p->batch * p->kv_heads * a.rows;
     return a;
 }
 
-template <class TY, class F> int with_fragments(int nk, F f) {
-    switch (nk) {
-        case 0:
-            if constexpr (TY::kSize == 4) return f(TY{}, std::integral_constant<int, 0>{});
-        case 1: return f(TY{}, std::integral_constant<int, 1>{});
-        case 2: return f(TY{}, std::integral_constant<int, 2>{});
-        case 4: return f(TY{}, std::integral_constant<int, 4>{});
-        case 8: return f(TY{}, std::integral_constant<int, 8>{});
-        default:
-            if constexpr (TY::kSize == 4) return f(TY{}, std::integral_constant<int, 16>{});
-            return dst_op_fail(DST_E_UNSUPPORTED, "channels must be in 1..%d", DST_MAX_CHANNELS);
-    }
-}
-int fragments(const DstAttendParams *p) {
-    return fragments_of(p->channels > p->value_channels ? p->channels : p->value_channels, p->dtype);
-}
+// f(type, integral constant of the fragments) for the call's type and channels
 template <class F> int with_type(const DstAttendParams *p, F f) {
-    if (p->dtype == DST_DTYPE_F32) return with_fragments<F32>(fragments(p), f);
-    return p->dtype == DST_DTYPE_BF16 ? with_fragments<BF16>(fragments(p), f) : with_fragments<F16>(fragments(p), f);
+    const int nk = fragments_of(longest(p), p->dtype);
+    if (p->dtype == DST_DTYPE_F32) return with_floats(longest(p), f);
+    return p->dtype == DST_DTYPE_BF16 ? with_fragments<BF16>(nk, f) : with_fragments<F16>(nk, f);
 }
 
 // The rows of all sets, copied into the workspace's front where the kernels cannot read them where they lie.
 struct Sets {
     RowSet q, k, v, o, up;
 };
-template <int NK> Sets row_sets(const DstAttendParams *p, AttendArgs &a, bool backward, Carve &c) {
+template <class TY, int NK> Sets row_sets(const DstAttendParams *p, AttendArgs &a, bool backward, Carve &c) {
     // (a group has to fit whole into the steps between a thread's words, and into the blocks of 16 own rows)
-    const int stride = TileShape<NK>::kStride < 16 ? TileShape<NK>::kStride : 16, group = a.group;
+    const int stride = Shape<TY, NK>::kStride < 16 ? Shape<TY, NK>::kStride : 16, group = a.group;
     auto memory = [&](const void *t, const int64_t (&s)[3], int channels) {
-        return row_set(t, s[0], s[1], s[2], p->batch, p->kv_heads, 1, p->memory, channels, p->dtype, stride, c);
+        return row_set<TY>(t, s[0], s[1], s[2], p->batch, p->kv_heads, 1, p->memory, channels, stride, c);
     };
     auto queries = [&](const void *t, int64_t batch, int64_t row, int64_t head, int channels) {
-        return row_set(t, batch, row, head, p->batch, p->kv_heads, group, a.rows, channels, p->dtype, stride, c);
+        return row_set<TY>(t, batch, row, head, p->batch, p->kv_heads, group, a.rows, channels, stride, c);
     };
     const int64_t row = (int64_t)p->heads * p->value_channels;
     Sets s = {};
@@ -550,12 +547,12 @@ void prepare(const Sets &s, hipStream_t stream) {
 // Cuts a pass's own tiles; whether its rows are few. `kernel(few)`: the pass's kernel; `own_bytes`: of a part's row.
 template <class TY, int NK, class K>
 bool plan_cut(AttendArgs &a, int most, int64_t own_rows, int64_t streamed_rows, int64_t heads, int products, double row_bytes, K kernel) {
-    constexpr int tile = TileShape<NK>::kRows, dtype = TY::kSize == 4 ? DST_DTYPE_F32 : DST_DTYPE_BF16;
+    constexpr int tile = Shape<TY, NK>::kRows;
     const int64_t streamed = div_up(streamed_rows, tile);
     const bool few = own_rows <= kWaves * 16 || few_rows(div_up(own_rows, kWaves * 16 * most) * heads, streamed);
     a.own = kWaves * 16 * (few ? 1 : most);
     a.tiles = (int)div_up(own_rows, a.own);
-    a.cut = cut_tiles(a.tiles * heads, streamed, slots_of(kernel(few)), tile_time(a.own, tile, TileShape<NK>::kBytes, dtype, products),
+    a.cut = cut_tiles(a.tiles * heads, streamed, slots_of(kernel(few)), tile_time<TY, NK>(a.own, products),
                       a.own * row_bytes, a.lengths != nullptr);
     return few;
 }
@@ -640,7 +637,7 @@ uint64_t dst_attend_workspace_bytes(const DstAttendParams *p, int pass) {
         const int64_t heads = (int64_t)p->batch * p->kv_heads;
         if (a.all_rows == 0 && pass == DST_PASS_FORWARD) return DST_OK;
         Carve c = {nullptr, 0};
-        row_sets<NK>(p, a, pass != DST_PASS_FORWARD, c);
+        row_sets<TY, NK>(p, a, pass != DST_PASS_FORWARD, c);
         if (pass == DST_PASS_FORWARD) {
             bytes = plan_forward<TY, NK>(a, heads, c).bytes;
         } else {
@@ -666,7 +663,7 @@ int dst_attend_forward(const DstAttendParams *p, void *stream) {
         if (a.all_rows == 0) return (int)DST_OK;
         const int64_t heads = (int64_t)p->batch * p->kv_heads;
         Carve c = {(char *)p->workspace, 0};
-        const Sets sets = row_sets<NK>(p, a, false, c);
+        const Sets sets = row_sets<TY, NK>(p, a, false, c);
         const Plan plan = plan_forward<TY, NK>(a, heads, c);
         if (int rc = check_workspace(p, plan.bytes)) return rc;
         const hipStream_t s = (hipStream_t)stream;
@@ -677,7 +674,7 @@ int dst_attend_forward(const DstAttendParams *p, void *stream) {
         DST_OP_LAUNCH("attention");
         if (a.cut.splits > 1) {
             const int64_t rows = a.cut.parted() * a.own;
-            const int part = a.cut.per_split * TileShape<NK>::kRows;
+            const int part = a.cut.per_split * Shape<TY, NK>::kRows;
             if (a.cut.splits >= 16) k_attend_join_row<E><<<dim3((uint32_t)rows), kThreads, 0, s>>>(a, part);
             else k_attend_join<E><<<dim3((uint32_t)div_up(rows * ((a.dv + 3) / 4), kThreads)), kThreads, 0, s>>>(a, part);
             DST_OP_LAUNCH("attention, joining");
@@ -701,7 +698,7 @@ int dst_attend_backward(const DstAttendParams *p, void *stream) {
         const int64_t heads = (int64_t)p->batch * p->kv_heads;
         AttendArgs a = arguments(p);
         Carve c = {(char *)p->workspace, 0};
-        const Sets sets = row_sets<NK>(p, a, true, c);
+        const Sets sets = row_sets<TY, NK>(p, a, true, c);
         a.dq = p->grad_q, a.dk = p->grad_k, a.dvalue = p->grad_v;
         if (a.all_rows > 0) {
             const Plan plan = plan_dq<TY, NK>(a, heads, c);
@@ -728,7 +725,7 @@ int dst_attend_backward(const DstAttendParams *p, void *stream) {
         }
         return (int)DST_OK;
     };
-    return p->dtype == DST_DTYPE_F32 ? with_fragments<F32>(fragments(p), launch) : with_fragments<BF16>(fragments(p), launch);
+    return p->dtype == DST_DTYPE_F32 ? with_floats(longest(p), launch) : with_fragments<BF16>(fragments_of(longest(p), p->dtype), launch);
 }
 
 }  // extern "C"

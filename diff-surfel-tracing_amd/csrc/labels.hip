@@ -51,8 +51,8 @@ constexpr int kBoundBlocks = 64;
 
 // Own blocks of 16 rows of a wave. More of them read a streamed tile fewer times from LDS, fewer leave registers for a second wave
 // on a SIMD, which counts for more (32768 rays x 32771 labels, 256 channels, bf16: dx 1661 us with 2 blocks, 1268 with 1).
-template <class TY, int NK> constexpr int forward_blocks() { return NK <= 1 ? 4 : NK <= 8 ? 2 : 1; }
-template <class TY, int NK> constexpr int backward_blocks() { return NK <= 1 ? (TY::kSize == 2 ? 2 : 4) : NK <= 4 ? 2 : 1; }
+template <class TY, int NK> constexpr int forward_blocks() { return NK <= 1 ? 4 : NK * TY::kPlanes <= 12 ? 2 : 1; }
+template <class TY, int NK> constexpr int backward_blocks() { return NK <= 1 ? (TY::kDepth == 32 ? 2 : 4) : NK * TY::kPlanes <= 6 ? 2 : 1; }
 
 // The one value that the rays share
 __device__ inline float upstream_value(const LabelArgs &a) { return a.upstream[0] * a.inverse[0]; }
@@ -122,19 +122,10 @@ __device__ inline void merge_best(float &best, int &label, float &second, float 
     label = theirs ? l : label;
 }
 
-template <class TY> __device__ inline float dot_word(u4 a, u4 b) {
-    typename TY::E x[16 / TY::kSize], y[16 / TY::kSize];
-    __builtin_memcpy(x, &a, 16), __builtin_memcpy(y, &b, 16);
-    float s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 16 / TY::kSize; ++i) s = __builtin_fmaf((float)x[i], (float)y[i], s);
-    return s;
-}
-
 // Rays as own rows, the table streamed. BEST: the best label instead of the loss.
 template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThreads) void k_label_forward(LabelArgs a) {
-    typedef TileShape<NK> T;
-    __shared__ alignas(16) char tile[T::kRows * T::kPitch > kThreads * 12 ? T::kRows * T::kPitch : kThreads * 12];
+    typedef Shape<TY, NK> T;
+    __shared__ alignas(16) char tile[T::kTile > kThreads * 12 ? T::kTile : kThreads * 12];
     __shared__ alignas(16) float tile_bias[T::kRows];
     const int lane = threadIdx.x & 63, g = lane >> 4, wave = wave_number();
     const Turn turn = turn_of(a.cut);
@@ -142,7 +133,7 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
     const int first = turn.part ? turn.split * a.cut.per_split * T::kRows : 0;
     const int last = turn.part ? min(a.labels, first + a.cut.per_split * T::kRows) : a.labels;   // (the host keeps labels below 2^30)
 
-    Stage<NK> stage;
+    Stage<TY, NK> stage;
     stage.begin(a.w, tile_base(a.w, first));
     float stage_bias = 0.0f;   // of a row behind the table's end: -inf, which takes it out of every sum
     auto fetch = [&](int at) {
@@ -225,7 +216,7 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
         if constexpr (BEST) {
             float norm = 0.0f;
 #pragma unroll
-            for (int k = 0; k < fragments<NK>(); ++k) norm += dot_word<TY>(own.f[q][k], own.f[q][k]);
+            for (int k = 0; k < fragments<NK>(); ++k) norm += fragment_dot<TY>(own.f[q][k], own.f[q][k]);
             norm = sqrtf(sum_group(norm));
 #pragma unroll
             for (int step = 16; step <= 32; step <<= 1)
@@ -248,7 +239,7 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
                 const bool there = t >= 0 && t < a.labels;
 #pragma unroll
                 for (int k = 0; k < fragments<NK>(); ++k)
-                    logit += dot_word<TY>(own.f[q][k], own_word<NK>(there ? tile_base(a.w, t) : nullptr, k, a.w.words));
+                    logit += fragment_dot<TY>(own.f[q][k], own_word<TY, NK>(there ? tile_base(a.w, t) : nullptr, k, a.w.words));
                 logit = sum_group(logit);
                 if (there && a.bias) logit += a.bias[t];
             }
@@ -320,9 +311,12 @@ template <class TY> __global__ __launch_bounds__(kThreads) void k_label_bounds(L
     const int lane = threadIdx.x & 63;
     float wide = 0.0f, tall = 0.0f;
     for (int64_t v = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6); v < a.labels; v += (int64_t)kBoundBlocks * kWaves) {
-        const typename TY::E *w = reinterpret_cast<const typename TY::E *>(tile_base(a.w, v));
         float n = 0.0f;
-        for (int i = lane; i < a.d; i += 64) n = __builtin_fmaf((float)w[i], (float)w[i], n);
+        for (int k = lane; k < a.w.words; k += 64) {
+            float w[kWordValues<TY>];
+            row_values<TY>(tile_base(a.w, v), k, a.w.words, w);
+            for (int j = 0; j < kWordValues<TY>; ++j) n = __builtin_fmaf(w[j], w[j], n);
+        }
         for (int step = 32; step > 0; step >>= 1) n += __shfl_xor(n, step);
         wide = fmaxf(wide, n);
         if (a.bias) {   // (a label switched off by an infinite bias bounds nothing)
@@ -346,8 +340,7 @@ template <class TY> __global__ __launch_bounds__(kThreads) void k_label_bounds(L
 
 // The rays on the list, a workgroup each: every label's logit again in 32 bits, and in 64 where it can be the best.
 template <class TY> __global__ __launch_bounds__(kThreads) void k_label_near(LabelArgs a) {
-    constexpr int per = 16 / TY::kSize;
-    typedef typename TY::E E;
+    constexpr int per = kWordValues<TY>;
     __shared__ alignas(16) float x[DST_MAX_CHANNELS];
     __shared__ double top[kThreads];
     __shared__ int at[kThreads];
@@ -355,25 +348,32 @@ template <class TY> __global__ __launch_bounds__(kThreads) void k_label_near(Lab
     for (uint32_t i = blockIdx.x; i < n; i += gridDim.x) {
         const int64_t row = a.near_list[i];
         const float floor = a.near_floor[i];
-        const E *xr = reinterpret_cast<const E *>(tile_base(a.x, row));
         __syncthreads();
-        x[threadIdx.x] = (int)threadIdx.x < a.d ? (float)xr[threadIdx.x] : 0.0f;
+        if ((int)threadIdx.x < a.x.words) {
+            float v[per];
+            row_values<TY>(tile_base(a.x, row), threadIdx.x, a.x.words, v);
+            for (int j = 0; j < per; ++j) x[threadIdx.x * per + j] = v[j];
+        }
         __syncthreads();
         double best = -__builtin_huge_val();
         int label = 0x7fffffff;
         for (int v = threadIdx.x; v < a.labels; v += kThreads) {
-            const E *w = reinterpret_cast<const E *>(tile_base(a.w, v));
+            const char *w = tile_base(a.w, v);
             float s = a.bias ? a.bias[v] : 0.0f;
 #pragma unroll 4
             for (int k = 0; k < a.w.words; ++k) {
-                E word[per];
-                __builtin_memcpy(word, w + k * per, 16);
+                float word[per];
+                row_values<TY>(w, k, a.w.words, word);
 #pragma unroll
-                for (int j = 0; j < per; ++j) s = __builtin_fmaf(x[k * per + j], (float)word[j], s);
+                for (int j = 0; j < per; ++j) s = __builtin_fmaf(x[k * per + j], word[j], s);
             }
             if (!(s >= floor)) continue;
             double exact = 0.0;
-            for (int k = 0; k < a.d; ++k) exact = __builtin_fma((double)x[k], (double)(float)w[k], exact);
+            for (int k = 0; k < a.w.words; ++k) {
+                float word[per];
+                row_values<TY>(w, k, a.w.words, word);
+                for (int j = 0; j < per; ++j) exact = __builtin_fma((double)x[k * per + j], (double)word[j], exact);
+            }
             if (a.bias) exact += (double)a.bias[v];
             if (exact > best) best = exact, label = v;
         }
@@ -389,14 +389,12 @@ template <class TY> __global__ __launch_bounds__(kThreads) void k_label_near(Lab
         if (threadIdx.x == 0 && at[0] != 0x7fffffff) a.label[row] = at[0];
     }
 }
-static_assert(kThreads == DST_MAX_CHANNELS, "a thread a channel");
-
 // ---- backward -------------------------------------------------------------------------------------------------------
 // dx: rays as own rows, the table streamed.
 template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void k_label_dx(LabelArgs a) {
-    typedef TileShape<NK> T;
+    typedef Shape<TY, NK> T;
     constexpr int NM = depth_blocks<TY, NK>();
-    __shared__ alignas(16) char tile[T::kRows * T::kPitch];
+    __shared__ alignas(16) char tile[T::kTile];
     __shared__ alignas(16) float tile_bias[T::kRows];
     const int lane = threadIdx.x & 63, g = lane >> 4, wave = wave_number();
     const Turn turn = turn_of(a.cut);
@@ -404,7 +402,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     const int first = turn.part ? turn.split * a.cut.per_split * T::kRows : 0;
     const int last = turn.part ? min(a.labels, first + a.cut.per_split * T::kRows) : a.labels;
 
-    Stage<NK> stage;
+    Stage<TY, NK> stage;
     stage.begin(a.w, tile_base(a.w, first));
     float stage_bias = 0.0f;   // of a row behind the table's end: -inf, which takes it out of every sum
     auto fetch = [&](int at) {
@@ -447,7 +445,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
                     for (int r = 0; r < 4; ++r) {
                         float e = exp2_of(__builtin_fmaf(p[j][q][r], kLog2E, -lse2[q]));
                         // (of 32-bit rows the label's row is taken off the sum at the end; 16 bits would lose p - 1 where p is near 1)
-                        if constexpr (TY::kSize == 2) e -= label[q] - at == (pair + j) * 16 + r ? 1.0f : 0.0f;
+                        if constexpr (TY::kRounds) e -= label[q] - at == (pair + j) * 16 + r ? 1.0f : 0.0f;
                         p[j][q][r] = e;
                     }
             }
@@ -457,20 +455,17 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     }
     typedef typename TY::E E;
     const bool four = (a.d & 3) == 0;
-    typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
 #pragma unroll
     for (int q = 0; q < QB; ++q) {
         const int64_t row = row0 + q * 16 + (lane & 15);
         if (row >= a.rays) continue;
         const int64_t t = a.target[row];
-        const bool label_here = TY::kSize == 4 && t >= first && t < last;   // (of a part: its labels' alone)
-        const float *label_row = reinterpret_cast<const float *>(tile_base(a.w, label_here ? t : 0));
+        const bool label_here = !TY::kRounds && t >= first && t < last;   // (of a part: its labels' alone)
+        const char *label_row = tile_base(a.w, label_here ? t : 0);
 #pragma unroll
         for (int m = 0; m < NM; ++m) {
-            if (label_here) {
-                const int at = m * 16 + 4 * g;
-                if (at < 4 * a.w.words) out[q][m] -= *reinterpret_cast<const f4u *>(label_row + at);
-            }
+            if constexpr (!TY::kRounds)
+                if (label_here) out[q][m] -= row_four<TY>(label_row, m * 16 + 4 * g, a.w.words);
             f4 v = out[q][m] * up[q];
             if (up[q] == 0.0f) v = f4{0.0f, 0.0f, 0.0f, 0.0f};   // (an ignored ray's channels may hold anything)
             if (turn.part) store_four(a.out_part + part_row(a.cut, turn, kWaves * 16 * QB, wave * 16 * QB + q * 16 + (lane & 15)) * a.d, m * 16 + 4 * g, a.d, v, four);
@@ -482,9 +477,9 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
 // dw and db: labels as own rows, the rays streamed.
 // ONE: the rays share one upstream gradient, which multiplies the sums at the end; else each ray's weights have its own.
 template <class TY, int NK, int QB, bool ONE> __global__ __launch_bounds__(kThreads) void k_label_dw(LabelArgs a) {
-    typedef TileShape<NK> T;
+    typedef Shape<TY, NK> T;
     constexpr int NM = depth_blocks<TY, NK>();
-    __shared__ alignas(16) char tile[T::kRows * T::kPitch];
+    __shared__ alignas(16) char tile[T::kTile];
     __shared__ alignas(16) float tile_lse2[2][T::kRows], tile_up[2][T::kRows];
     __shared__ alignas(16) int tile_label[2][T::kRows];
     const int lane = threadIdx.x & 63, g = lane >> 4, wave = wave_number();
@@ -493,7 +488,7 @@ template <class TY, int NK, int QB, bool ONE> __global__ __launch_bounds__(kThre
     const int64_t first = turn.part ? (int64_t)turn.split * a.cut.per_split * T::kRows : 0;
     const int64_t last = turn.part ? min(a.rays, first + (int64_t)a.cut.per_split * T::kRows) : a.rays;
 
-    Stage<NK> stage;
+    Stage<TY, NK> stage;
     stage.begin(a.x, tile_base(a.x, first));
     // Of every ray: lse (+inf where it is ignored or behind the end, which makes its weights 0), upstream gradient, label. They are a tile
     // ahead of the channels, which are read only of rays that are not ignored: those of the others may hold anything.
@@ -624,35 +619,22 @@ LabelArgs arguments(const DstLabelParams *p) {
 struct Sets {
     RowSet x, w;
 };
-Sets row_sets(const DstLabelParams *p, Carve &c) {
+template <class TY> Sets row_sets(const DstLabelParams *p, Carve &c) {
     Sets s;
-    s.x = row_set(p->features, 0, p->features_stride, 0, 1, 1, 1, p->rays, p->channels, p->dtype, 1, c);
-    s.w = row_set(p->weight, 0, p->weight_stride, 0, 1, 1, 1, p->labels, p->channels, p->dtype, 1, c);
+    s.x = row_set<TY>(p->features, 0, p->features_stride, 0, 1, 1, 1, p->rays, p->channels, 1, c);
+    s.w = row_set<TY>(p->weight, 0, p->weight_stride, 0, 1, 1, 1, p->labels, p->channels, 1, c);
     return s;
 }
 
 template <class TY, int NK> struct Shapes {   // own rows of a workgroup, rows of a tile
     static constexpr int kForward = kWaves * 16 * forward_blocks<TY, NK>(), kBackward = kWaves * 16 * backward_blocks<TY, NK>();
-    static constexpr int kTile = TileShape<NK>::kRows;
+    static constexpr int kTile = Shape<TY, NK>::kRows;
 };
 
-// f(type, integral constant of NK) for the call's type and channels
-template <class TY, class F> int with_fragments(int nk, F f) {
-    switch (nk) {
-        case 0:
-            if constexpr (TY::kSize == 4) return f(TY{}, std::integral_constant<int, 0>{});
-        case 1: return f(TY{}, std::integral_constant<int, 1>{});
-        case 2: return f(TY{}, std::integral_constant<int, 2>{});
-        case 4: return f(TY{}, std::integral_constant<int, 4>{});
-        case 8: return f(TY{}, std::integral_constant<int, 8>{});
-        default:
-            if constexpr (TY::kSize == 4) return f(TY{}, std::integral_constant<int, 16>{});
-            return dst_op_fail(DST_E_UNSUPPORTED, "channels must be in 1..%d", DST_MAX_CHANNELS);
-    }
-}
+// f(type, integral constant of the fragments) for the call's type and channels
 template <class F> int with_type(const DstLabelParams *p, F f) {
     const int nk = fragments_of(p->channels, p->dtype);
-    if (p->dtype == DST_DTYPE_F32) return with_fragments<F32>(nk, f);
+    if (p->dtype == DST_DTYPE_F32) return with_floats(p->channels, f);
     return p->dtype == DST_DTYPE_BF16 ? with_fragments<BF16>(nk, f) : with_fragments<F16>(nk, f);
 }
 
@@ -672,11 +654,11 @@ template <class TY, int NK, bool BEST> ForwardPlan forward_plan(const DstLabelPa
     f.few = few_rows(div_up(p->rays, S::kForward), streamed);
     a.own = f.few ? kWaves * 16 : S::kForward;
     a.cut = cut_tiles(div_up(p->rays, a.own), streamed, slots_of(forward_kernel<TY, NK, BEST>(f.few)),
-                      tile_time(a.own, S::kTile, TileShape<NK>::kBytes, p->dtype, 1), a.own * (BEST ? 24.0 : 8.0));
+                      tile_time<TY, NK>(a.own, 1), a.own * (BEST ? 24.0 : 8.0));
     const uint64_t rest = a.cut.splits > 1 ? (uint64_t)a.cut.parted() * a.own : 0, parts = rest * a.cut.splits;
     f.sums = (uint32_t)(a.cut.splits > 1 ? a.cut.whole + div_up(rest, kThreads) : a.cut.tiles);
     Carve c = {base, 0};
-    f.sets = row_sets(p, c);
+    f.sets = row_sets<TY>(p, c);
     a.x = f.sets.x.rows, a.w = f.sets.w.rows;
     if (parts) {
         a.part = c.take<float2>(parts);
@@ -713,11 +695,11 @@ template <class TY, int NK, bool DX> BackwardPlan backward_plan(const DstLabelPa
     if constexpr (DX) kernel = b.few ? (const void *)&k_label_dx<TY, NK, 1> : (const void *)&k_label_dx<TY, NK, QB>;
     else if (p->reduction == DST_REDUCE_NONE) kernel = b.few ? (const void *)&k_label_dw<TY, NK, 1, false> : (const void *)&k_label_dw<TY, NK, QB, false>;
     else kernel = b.few ? (const void *)&k_label_dw<TY, NK, 1, true> : (const void *)&k_label_dw<TY, NK, QB, true>;
-    a.cut = cut_tiles(div_up(own, a.own), streamed, slots_of(kernel), tile_time(a.own, S::kTile, TileShape<NK>::kBytes, p->dtype, 2),
+    a.cut = cut_tiles(div_up(own, a.own), streamed, slots_of(kernel), tile_time<TY, NK>(a.own, 2),
                       a.own * (p->channels + 1) * 4.0);
     const uint64_t parts = a.cut.splits > 1 ? (uint64_t)a.cut.parted() * a.own * a.cut.splits : 0;
     Carve c = {base, 0};
-    b.sets = row_sets(p, c);
+    b.sets = row_sets<TY>(p, c);
     a.x = b.sets.x.rows, a.w = b.sets.w.rows;
     if (parts) {
         a.out_part = c.take<float>(parts * p->channels);
@@ -839,8 +821,7 @@ int dst_label_loss_backward(const DstLabelParams *p, void *stream) {
         }
         return (int)DST_OK;
     };
-    const int nk = fragments_of(p->channels, p->dtype);
-    return p->dtype == DST_DTYPE_F32 ? with_fragments<F32>(nk, launch) : with_fragments<BF16>(nk, launch);
+    return p->dtype == DST_DTYPE_F32 ? with_floats(p->channels, launch) : with_fragments<BF16>(fragments_of(p->channels, p->dtype), launch);
 }
 
 int dst_label_best(const DstLabelParams *p, void *stream) {

@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "dst_api.h"
 #include "tiles.inc"
 
@@ -19,13 +21,31 @@ int dst_op_fail(int code, const char *format, ...) __attribute__((format(printf,
 namespace {
 
 inline int value_size(int dtype) { return dtype == DST_DTYPE_F32 ? 4 : 2; }
-// 64-byte fragments of a row, as the kernels are instantiated: 0 (half a one), 1, 2, 4, 8 or 16
+// 32-bit rows longer than this are split into planes of 16 bits (tiles.inc).
+constexpr int kLongest32 = 16;
+// 64-byte fragments of a row (of its planes, where it is split), as the kernels are instantiated: 0 (half a one), 1, 2, 4 or 8
 inline int fragments_of(int channels, int dtype) {
-    const int bytes = channels * value_size(dtype);
-    if (dtype == DST_DTYPE_F32 && bytes <= 32) return 0;
+    if (dtype == DST_DTYPE_F32 && channels <= kLongest32) return channels <= 8 ? 0 : 1;
     int nk = 1;
-    while (nk * 64 < bytes) nk *= 2;
+    while (nk * 32 < channels) nk *= 2;
     return nk;
+}
+// f(type, integral constant of the fragments) of a call
+template <class TY, class F> int with_fragments(int nk, F f) {
+    if constexpr (std::is_same_v<TY, F32>) {
+        return nk == 0 ? f(TY{}, std::integral_constant<int, 0>{}) : f(TY{}, std::integral_constant<int, 1>{});
+    } else {
+        switch (nk) {
+            case 1: return f(TY{}, std::integral_constant<int, 1>{});
+            case 2: return f(TY{}, std::integral_constant<int, 2>{});
+            case 4: return f(TY{}, std::integral_constant<int, 4>{});
+            default: return f(TY{}, std::integral_constant<int, 8>{});
+        }
+    }
+}
+template <class F> int with_floats(int channels, F f) {
+    const int nk = fragments_of(channels, DST_DTYPE_F32);
+    return channels <= kLongest32 ? with_fragments<F32>(nk, f) : with_fragments<Split32>(nk, f);
 }
 inline int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline uint64_t align_up(uint64_t bytes) { return (bytes + 255u) & ~(uint64_t)255u; }
@@ -88,9 +108,9 @@ inline int slots_of(const void *kernel) {
 }
 // What a streamed tile takes a workgroup, about: `products` of own x tile x depth at 40 % of a compute unit's rate, shared by two
 // workgroups, and the exponentials.
-inline double tile_time(int own, int tile, int depth_bytes, int dtype, int products) {
-    const double flops = 2.0 * own * tile * (depth_bytes / value_size(dtype)) * products;
-    return 2.0 * (flops / (dtype == DST_DTYPE_F32 ? 0.4e6 : 4e6) + own * tile * 1.6e-5);
+template <class TY, int NK> double tile_time(int own, int products) {
+    const double flops = 2.0 * own * Shape<TY, NK>::kRows * (NK ? NK * TY::kDepth : 8) * products;
+    return 2.0 * (flops / (TY::kPlanes == 3 ? 0.7e6 : TY::kRounds ? 4e6 : 0.4e6) + own * Shape<TY, NK>::kRows * 1.6e-5);
 }
 
 // Whether the own rows are few: blocks of 16 * QB rows a wave would leave compute units without a workgroup, however the streamed
@@ -160,11 +180,12 @@ template <class E, class E2, class To> inline void sum_parts(Parts<E> a, Parts<E
     else k_sum_parts<E, E2, 1><<<grid, 256, 0, s>>>(a, b, cut, own, to);
 }
 
-// Rows that the kernels cannot read where they lie, copied: (batches, heads, rows) of whole words, zeros behind the channels.
+// Rows that the kernels cannot read where they lie, copied: (batches, heads, rows) of whole words, zeros behind the channels; 32-bit
+// values split into planes where `split`.
 struct RowCopy {
     const char *from;
     int64_t batch, row, in_group;   // bytes; a head is `group` steps of in_group
-    int32_t heads, group, size, channels, words;
+    int32_t heads, group, size, channels, words, split;
     int64_t rows, all_words;
     uint4 *to;
 };
@@ -174,6 +195,20 @@ __global__ __launch_bounds__(256) void k_copy_rows(RowCopy c) {
     const int64_t at = i / c.words, r = at % c.rows, head = at / c.rows % c.heads, batch = at / c.rows / c.heads;
     const int w = (int)(i - at * c.words);
     const char *from = c.from + batch * c.batch + r / c.group * c.row + (head * c.group + r % c.group) * c.in_group;
+    if (c.split) {
+        f4 v[2] = {};
+        for (int h = 0; h < 2; ++h) {
+            const float *p = reinterpret_cast<const float *>(from) + 8 * w + 4 * h;
+            if (8 * w + 4 * h + 4 <= c.channels) __builtin_memcpy(&v[h], p, 16);
+            else
+                for (int k = 0; k < 4; ++k)
+                    if (8 * w + 4 * h + k < c.channels) v[h][k] = p[k];
+        }
+        u4 planes[3];
+        Split32::pack(v[0], v[1], planes);
+        for (int p = 0; p < 3; ++p) reinterpret_cast<u4 *>(c.to)[(at * 3 + p) * c.words + w] = planes[p];
+        return;
+    }
     uint32_t word[4] = {0u, 0u, 0u, 0u};
     if (c.size == 4) {
         for (int k = 0; k < 4; ++k)
@@ -192,18 +227,20 @@ struct RowSet {
     RowCopy copy;
     bool copied;
 };
-inline RowSet row_set(const void *p, int64_t batch, int64_t row, int64_t head, int64_t batches, int heads, int group, int64_t n, int channels,
-                      int dtype, int stride, Carve &c) {
-    const int size = value_size(dtype), words = (channels * size + 15) / 16;
+template <class TY>
+RowSet row_set(const void *p, int64_t batch, int64_t row, int64_t head, int64_t batches, int heads, int group, int64_t n, int channels, int stride, Carve &c) {
+    constexpr bool split = TY::kPlanes == 3;
+    const int size = sizeof(typename TY::E), words = split ? (channels + 7) / 8 : (channels * size + 15) / 16;
     RowSet s = {};
-    s.rows = Rows{(const char *)p, batch * size, head * size * group, row * size, (int32_t)(head * size), group, words};
+    s.rows = Rows{(const char *)p, batch * size, head * size * group, row * size, head * size > 0x7fffffff ? 0 : (int32_t)(head * size), group, words};
     const int64_t widest = (256 / group + 1) * s.rows.row + (int64_t)group * head * size + 4096;   // within 256 rows
-    s.copied = (channels * size) % 16 != 0 || (reinterpret_cast<uintptr_t>(p) & 3u) != 0 || (batch * size) % 4 != 0 || (row * size) % 4 != 0 ||
-               (head * size) % 4 != 0 || stride % group != 0 || widest > 0x7fffffff || head * size > 0x7fffffff;
+    s.copied = split || (channels * size) % 16 != 0 || (reinterpret_cast<uintptr_t>(p) & 3u) != 0 || (batch * size) % 4 != 0 ||
+               (row * size) % 4 != 0 || (head * size) % 4 != 0 || stride % group != 0 || widest > 0x7fffffff || head * size > 0x7fffffff;
     if (s.copied) {
-        const int64_t all = batches * heads * n * words;
-        s.copy = RowCopy{(const char *)p, batch * size, row * size, head * size, heads, group, size, channels, words, n, all, c.take<uint4>(all)};
-        s.rows = Rows{(const char *)s.copy.to, (int64_t)heads * n * words * 16, n * words * 16, words * 16, 0, 1, words};
+        const int64_t all = batches * heads * n * words, line = words * TY::kPlanes * 16;
+        s.copy = RowCopy{(const char *)p, batch * size, row * size, head * size, heads, group, size, channels, words, split, n, all,
+                         c.take<uint4>(all * TY::kPlanes)};
+        s.rows = Rows{(const char *)s.copy.to, (int64_t)heads * n * line, n * line, line, 0, 1, words};
     }
     return s;
 }
