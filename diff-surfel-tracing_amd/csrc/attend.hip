@@ -116,6 +116,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
 #pragma unroll
         for (int i = 0; i < NM; ++i) out[q][i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
+    rows_are_here(own);
     for (int at = first; at < last; at += T::kRows) {
         stage_k.store(tile_k);
         stage_v.store(tile_v);
@@ -124,6 +125,8 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
         if (at + T::kRows < last) fetch(at + T::kRows);
 #pragma unroll
         for (int pair = 0; pair < T::kBlocks; pair += 2) {
+            if constexpr (TY::kRounds)
+                if (pair == 0) loads_between_products();
             f4 s[2][QB];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
@@ -189,14 +192,14 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
 
 // The parts of a split forward pass, a workgroup a row: for many parts of few rows (one ray that asks a long memory), which the
 // kernel below would go through one after another (8 rows of 256 parts: 5 us, 45 with that one).
-template <class E> __global__ __launch_bounds__(kThreads) void k_attend_join_row(AttendArgs a, int rows_per_part) {
+template <class E> __global__ __launch_bounds__(kThreads) void k_attend_join_row(AttendArgs a, int rows_per_part, int rows_per_tile) {
     __shared__ float weight[kMostSplits], wave_top[kWaves], wave_sum[kWaves];
     __shared__ f4 sums[kThreads];
-    const int tile = blockIdx.x / a.own, tid = threadIdx.x;
+    const int tile = blockIdx.x / rows_per_tile, r = blockIdx.x % rows_per_tile, tid = threadIdx.x;
     const Place p = place_of(a, a.cut.whole + tile);
-    const int row = p.tile * a.own + (int)(blockIdx.x % a.own), length = p.length;
+    const int row = p.tile * a.own + r, length = p.length;
     if (row >= a.rows) return;
-    const int64_t from = (int64_t)tile * a.cut.splits * a.own + blockIdx.x % a.own;   // the row's first part; the next: own rows on
+    const int64_t from = (int64_t)tile * a.cut.splits * a.own + r;   // the row's first part; the next: own rows on
     const int64_t at = stat_row(a, p, row);
     const int used = (length + rows_per_part - 1) / rows_per_part;   // (parts behind the length left no sums)
     float top = -kInf;
@@ -331,6 +334,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
 #pragma unroll
         for (int i = 0; i < NM; ++i) out[q][i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
+    rows_are_here(own), rows_are_here(up);
     for (int at = first; at < last; at += T::kRows) {
         stage_k.store(tile_k);
         stage_v.store(tile_v);
@@ -411,6 +415,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     for (int q = 0; q < QB; ++q)
 #pragma unroll
         for (int i = 0; i < NM; ++i) dk[q][i] = dv[q][i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    rows_are_here(own_k), rows_are_here(own_v);
     for (int at = first; at < last; at += T::kRows) {
         stage_q.store(tile_q);
         stage_o.store(tile_o);
@@ -675,7 +680,8 @@ int dst_attend_forward(const DstAttendParams *p, void *stream) {
         if (a.cut.splits > 1) {
             const int64_t rows = a.cut.parted() * a.own;
             const int part = a.cut.per_split * Shape<TY, NK>::kRows;
-            if (a.cut.splits >= 16) k_attend_join_row<E><<<dim3((uint32_t)rows), kThreads, 0, s>>>(a, part);
+            const int some = a.own < a.rows ? a.own : a.rows;   // rows of a tile that are there
+            if (a.cut.splits >= 16) k_attend_join_row<E><<<dim3((uint32_t)(a.cut.parted() * some)), kThreads, 0, s>>>(a, part, some);
             else k_attend_join<E><<<dim3((uint32_t)div_up(rows * ((a.dv + 3) / 4), kThreads)), kThreads, 0, s>>>(a, part);
             DST_OP_LAUNCH("attention, joining");
         }

@@ -149,7 +149,7 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
     int label[QB];
 #pragma unroll
     for (int q = 0; q < QB; ++q) run[q] = Running{-kInf, 0.0f}, best[q] = second[q] = -kInf, label[q] = 0x7fffffff;
-
+    rows_are_here(own);
     for (int at = first; at < last; at += T::kRows) {
         stage.store(tile);
         if ((int)threadIdx.x < T::kRows) tile_bias[threadIdx.x] = stage_bias;
@@ -161,6 +161,8 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
         for (int q = 0; q < QB; ++q) before[q] = best[q], place[q] = 0;
 #pragma unroll
         for (int pair = 0; pair < T::kBlocks; pair += 2) {
+            if constexpr (TY::kRounds)
+                if (pair == 0) loads_between_products();
             if (NK <= 2 && at + pair * 16 >= last) break;   // (short rows: the work on a logit is most of all work)
             f4 s[2][QB];
 #pragma unroll
@@ -425,6 +427,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
 #pragma unroll
         for (int m = 0; m < NM; ++m) out[q][m] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
+    rows_are_here(own);
     for (int at = first; at < last; at += T::kRows) {
         stage.store(tile);
         if ((int)threadIdx.x < T::kRows) tile_bias[threadIdx.x] = stage_bias;
@@ -493,21 +496,24 @@ template <class TY, int NK, int QB, bool ONE> __global__ __launch_bounds__(kThre
     // Of every ray: lse (+inf where it is ignored or behind the end, which makes its weights 0), upstream gradient, label. They are a tile
     // ahead of the channels, which are read only of rays that are not ignored: those of the others may hold anything.
     float stage_lse2 = kInf, stage_up = 0.0f;
-    int stage_label = -1;
-    auto fetch_stats = [&](int64_t at) {
-        if ((int)threadIdx.x < T::kRows) {
-            const int64_t row = at + threadIdx.x, t = row < last ? a.target[row] : a.ignore;
-            stage_lse2 = row < last ? a.lse2[row] : kInf;
-            if (!ONE) stage_up = row < last ? upstream_of(a, row, t) : 0.0f;
-            else if (t != a.ignore && (t < 0 || t >= a.labels)) stage_lse2 = __builtin_nanf("");
-            stage_label = t >= 0 && t < a.labels && t != a.ignore ? (int)t : -1;
+    int64_t stage_target = a.ignore;
+    auto fetch_stats = [&](int64_t at) {   // (as they lie: what is made of them waits for them)
+        const int64_t row = at + threadIdx.x;
+        stage_target = a.ignore, stage_lse2 = kInf;
+        if ((int)threadIdx.x < T::kRows && row < last) {
+            stage_target = a.target[row], stage_lse2 = a.lse2[row];
+            if (!ONE) stage_up = a.upstream[row];
         }
     };
     auto store_stats = [&](int at) {
-        if ((int)threadIdx.x < T::kRows) tile_lse2[at][threadIdx.x] = stage_lse2, tile_up[at][threadIdx.x] = stage_up, tile_label[at][threadIdx.x] = stage_label;
+        if ((int)threadIdx.x >= T::kRows) return;
+        const bool ignored = stage_target == a.ignore, none = !ignored && (stage_target < 0 || stage_target >= a.labels);
+        tile_lse2[at][threadIdx.x] = none ? __builtin_nanf("") : stage_lse2;
+        tile_label[at][threadIdx.x] = ignored || none ? -1 : (int)stage_target;
+        if (!ONE) tile_up[at][threadIdx.x] = ignored ? 0.0f : stage_up;
     };
     auto fetch = [&](int64_t at, int half) {
-        stage.load((int)min(last - at, (int64_t)T::kRows), [&](int r) { return tile_lse2[half][r & (T::kRows - 1)] != kInf; });
+        stage.template load<true>((int)min(last - at, (int64_t)T::kRows), tile_lse2[half]);
     };
     fetch_stats(first);
     Own<TY, NK, QB> own;
@@ -527,6 +533,7 @@ template <class TY, int NK, int QB, bool ONE> __global__ __launch_bounds__(kThre
         for (int m = 0; m < NM; ++m) out[q][m] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     int half = 0;
+    rows_are_here(own);
     for (int64_t at = first; at < last; at += T::kRows, half ^= 1) {
         stage.store(tile);
         store_stats(half ^ 1);
@@ -544,7 +551,8 @@ template <class TY, int NK, int QB, bool ONE> __global__ __launch_bounds__(kThre
                 for (int q = 0; q < QB; ++q) p[j][q] = f4{bias[q], bias[q], bias[q], bias[q]};
                 product<TY, NK, QB>(tile, pair + j, own, p[j]);
                 const int at4 = (pair + j) * 16 + 4 * g;
-                const f4 lse2 = *reinterpret_cast<const f4 *>(tile_lse2[half] + at4), up = *reinterpret_cast<const f4 *>(tile_up[half] + at4);
+                const f4 lse2 = *reinterpret_cast<const f4 *>(tile_lse2[half] + at4);
+                const f4 up = ONE ? f4{} : *reinterpret_cast<const f4 *>(tile_up[half] + at4);
                 const int4 label = *reinterpret_cast<const int4 *>(tile_label[half] + at4);
                 const int labels[4] = {label.x, label.y, label.z, label.w};
 #pragma unroll
