@@ -6,7 +6,9 @@ example/render.py:48-155) on top of the MI355X tracer.
     python render.py --scene room --surfels 200000 --frames 8 --result_dir out          # a synthetic scene, orbit path
 
 For every camera it traces rgb / depth / normal and writes RENDER/, DEPTH/ and NORMAL/ images with the reference's
-post-processing (`normalize_depth`, `visualize_normal`: reference example/utils/data_utils.py:52-70).  What it
+post-processing (`normalize_depth`, `visualize_normal`: reference example/utils/data_utils.py:52-70).  A model with auxiliary channels (`aux_0` .. `aux_7` in the .ply,
+or a synthetic scene's) can be given what reads them: `--labels head.npz` writes the label of every pixel to LABEL/, and
+`--memory bank.npz` the features that every pixel gets out of a memory bank to FEATURE/.  What it
 does not need: plyfile (the .ply reader below parses the binary little-endian layout 3DGS / 2DGS trainers write),
 cv2 (PNG through zlib) and ffmpeg (no video; the frames are numbered for it).
 """
@@ -90,8 +92,63 @@ def load_surfel_model(path, max_sh_degree=3):
     rot = rot / rot.norm(dim=-1, keepdim=True)
     model = {"means3D": xyz.contiguous(), "shs": shs, "opacities": torch.sigmoid(f32("opacity"))[:, None].contiguous(),
              "scales": scales, "rotations": rot.contiguous()}
+    aux = numbered("aux_")
+    if aux:
+        model["others_precomp"] = torch.stack([f32(n) for n in aux], 1).contiguous()
     model["vertices"], model["faces"] = S.get_triangles(model["means3D"], model["scales"], model["rotations"])
     return model
+
+
+def _arrays(path, wanted, optional=()):
+    """float32 tensors of an .npz: {name: tensor}; `wanted`: {name: dimensions}."""
+    with np.load(path) as z:   # (no pickles: numpy's default)
+        missing = [n for n in wanted if n not in z.files and n not in optional]
+        if missing:
+            raise ValueError("%s lacks %s" % (path, ", ".join(missing)))
+        out = {n: torch.from_numpy(np.ascontiguousarray(z[n], dtype=np.float32)) for n in wanted if n in z.files}
+    for n, t in out.items():
+        if t.dim() != wanted[n]:
+            raise ValueError("%s in %s must have %d dimensions (got %s)" % (n, path, wanted[n], tuple(t.shape)))
+    return out
+
+
+def load_label_head(path):
+    """What labels are read off a pixel's channels with: weight (labels, channels), bias (labels) or none."""
+    head = _arrays(path, {"weight": 2, "bias": 1}, optional=("bias",))
+    if "bias" in head and head["bias"].shape[0] != head["weight"].shape[0]:
+        raise ValueError("bias in %s must have a value for every label" % path)
+    return head
+
+
+def load_memory_bank(path):
+    """What features are read out of a memory with: query (channels, heads, width) makes a pixel's queries of its channels,
+    keys (memory, kv_heads, width) and values (memory, kv_heads, features) are the memory."""
+    bank = _arrays(path, {"query": 3, "keys": 3, "values": 3})
+    q, k, v = bank["query"], bank["keys"], bank["values"]
+    if k.shape[:2] != v.shape[:2] or k.shape[2] != q.shape[2] or k.shape[1] < 1 or q.shape[1] % k.shape[1] != 0:
+        raise ValueError("query, keys and values in %s do not fit each other" % path)
+    return bank
+
+
+def pixel_labels(aux, head):
+    """(H,W) labels and log probabilities of a traced image's channels (H,W,C)."""
+    import diff_surfel_tracing as dst
+    return dst.label_rays(aux, head["weight"], head.get("bias"))
+
+
+def pixel_features(aux, bank):
+    """(H,W,heads*features) out of the memory for a traced image's channels (H,W,C)."""
+    import diff_surfel_tracing as dst
+    H, W, C = aux.shape
+    q = bank["query"]
+    queries = (aux.reshape(-1, C) @ q.reshape(C, -1)).reshape(1, H * W, q.shape[1], q.shape[2])
+    return dst.attend_memory(queries, bank["keys"][None], bank["values"][None]).reshape(H, W, -1)
+
+
+def label_colors(labels):
+    """A color for every label, the same in every image: (H,W) -> (H,W,3) in [0,1]."""
+    mixed = (labels.to(torch.int64)[..., None] + 1) * torch.tensor([2654435761, 2246822519, 3266489917], device=labels.device)
+    return ((mixed >> 13) & 255).float() / 255.0
 
 
 def load_nerf_camera(cam):
@@ -164,12 +221,19 @@ def save_png(path, img):
 
 
 def render_path(tracer, model, cameras, result_dir=None, white_bg=True, sh_degree=3, max_trace_depth=0,
-                specular_threshold=0.0, scale_modifier=1.0, dev="cuda"):
+                specular_threshold=0.0, scale_modifier=1.0, dev="cuda", label_head=None, memory_bank=None):
     """Trace every camera of the path; returns the list of (rgb, dpt, acc, norm) tensors and writes the three image
-    folders when `result_dir` is given.  Follows reference example/render.py:60-145 call for call."""
+    folders when `result_dir` is given.  With a `label_head` (load_label_head) the tuples go on with the pixels' labels, with a
+    `memory_bank` (load_memory_bank) with their features, and LABEL/ and FEATURE/ are written too.  Follows reference example/render.py:60-145 call for call."""
     import diff_surfel_tracing as dst
     g = {k: v.to(dev).contiguous() for k, v in model.items()}
     tracer.build_acceleration_structure(g["vertices"].detach().clone(), g["faces"].detach().clone(), rebuild=True)
+    channels = g["others_precomp"].shape[1] if "others_precomp" in g else 0
+    for what, name in ((label_head, "weight"), (memory_bank, "query")):
+        if what is not None and what[name].shape[1 if name == "weight" else 0] != channels:
+            raise ValueError("the model has %d auxiliary channels, %s is for %d"
+                             % (channels, name, what[name].shape[1 if name == "weight" else 0]))
+    label_head, memory_bank = ({k: v.to(dev) for k, v in d.items()} if d else None for d in (label_head, memory_bank))
     bg = torch.tensor([1.0, 1.0, 1.0] if white_bg else [0.0, 0.0, 0.0], dtype=torch.float32, device=dev)
     grads3D = torch.zeros_like(g["means3D"])
     eye = torch.eye(4, device=dev)
@@ -188,11 +252,19 @@ def render_path(tracer, model, cameras, result_dir=None, white_bg=True, sh_degre
                 colors_precomp=g.get("colors_precomp"), others_precomp=g.get("others_precomp"),
                 opacities=g["opacities"], scales=g["scales"], rotations=g["rotations"], cov3D_precomp=None,
                 tracer_settings=settings, start_from_first=True)
-        outs.append((rgb, dpt, acc, norm))
+            labels = pixel_labels(aux, label_head)[0] if label_head else None
+            features = pixel_features(aux, memory_bank) if memory_bank else None
+        outs.append((rgb, dpt, acc, norm) + tuple(t for t in (labels, features) if t is not None))
         if result_dir:
             save_png(os.path.join(result_dir, "RENDER", "%04d.png" % i), rgb)
             save_png(os.path.join(result_dir, "DEPTH", "%04d.png" % i), normalize_depth(dpt))
             save_png(os.path.join(result_dir, "NORMAL", "%04d.png" % i), visualize_normal(norm, R.to(dev)))
+            if labels is not None:
+                save_png(os.path.join(result_dir, "LABEL", "%04d.png" % i), label_colors(labels))
+                np.save(os.path.join(result_dir, "LABEL", "%04d.npy" % i), labels.cpu().numpy().astype(np.int32))
+            if features is not None:
+                os.makedirs(os.path.join(result_dir, "FEATURE"), exist_ok=True)
+                np.save(os.path.join(result_dir, "FEATURE", "%04d.npy" % i), features.cpu().numpy())
     return outs
 
 
@@ -211,12 +283,17 @@ def main():
     ap.add_argument("--frames", type=int, default=8)
     ap.add_argument("--height", type=int, default=540)
     ap.add_argument("--width", type=int, default=960)
+    ap.add_argument("--labels", type=str, default=None, help="label head (.npz: weight, bias): writes LABEL/")
+    ap.add_argument("--memory", type=str, default=None, help="memory bank (.npz: query, keys, values): writes FEATURE/")
     a = ap.parse_args()
+    head, bank = a.labels and load_label_head(a.labels), a.memory and load_memory_bank(a.memory)
     import diff_surfel_tracing as dst
     if a.model_path:
         model = load_surfel_model(a.model_path, a.max_sh_degree)
     else:
-        model = {"cube": S.scene_cube, "sphere": S.scene_sphere, "room": S.scene_room}[a.scene](a.surfels)
+        channels = head["weight"].shape[1] if head else bank["query"].shape[0] if bank else 0
+        more = {"aux": channels} if channels and a.scene != "sphere" else {}   # (the sphere has none to give)
+        model = {"cube": S.scene_cube, "sphere": S.scene_sphere, "room": S.scene_room}[a.scene](a.surfels, **more)
     print("[INFO] Loaded number of Gaussians: %d." % model["means3D"].shape[0])
     if a.camera_dir:
         cameras = [load_nerf_camera(c) for c in json.load(open(a.camera_dir))["frames"]]
@@ -225,7 +302,7 @@ def main():
         cameras = orbit_cameras(a.frames, a.height, a.width, 60.0, radius, 0.6)
     tracer = dst.SurfelTracer()
     render_path(tracer, model, cameras, a.result_dir, a.white_bg, a.max_sh_degree, a.max_trace_depth,
-                a.specular_threshold, a.scale_modifier)
+                a.specular_threshold, a.scale_modifier, label_head=head, memory_bank=bank)
     print("[INFO] Rendering finished: %d frames in %s." % (len(cameras), a.result_dir))
 
 
