@@ -545,9 +545,7 @@ template <class TY, int NK> Sets row_sets(const DstAttendParams *p, AttendArgs &
     a.q = s.q.rows, a.k = s.k.rows, a.v = s.v.rows, a.o = s.o.rows, a.up = s.up.rows;
     return s;
 }
-void prepare(const Sets &s, hipStream_t stream) {
-    for (const RowSet *r : {&s.q, &s.k, &s.v, &s.o, &s.up}) prepare(*r, stream);
-}
+void prepare(const Sets &s, hipStream_t stream) { prepare({&s.q, &s.k, &s.v, &s.o, &s.up}, stream); }
 
 // Cuts a pass's own tiles; whether its rows are few. `kernel(few)`: the pass's kernel; `own_bytes`: of a part's row.
 template <class TY, int NK, class K>

@@ -772,7 +772,7 @@ int dst_label_loss_forward(const DstLabelParams *p, void *stream) {
         if (p->reduction == DST_REDUCE_NONE) a.rows = p->loss;
         const hipStream_t s = (hipStream_t)stream;
         if (a.cut.tiles > 0) {
-            prepare(f.sets.x, s), prepare(f.sets.w, s);
+            prepare({&f.sets.x, &f.sets.w}, s);
             const dim3 grid((uint32_t)a.cut.blocks());
             if (f.few) k_label_forward<TY, NK, 1, false><<<grid, kThreads, 0, s>>>(a);
             else k_label_forward<TY, NK, forward_blocks<TY, NK>(), false><<<grid, kThreads, 0, s>>>(a);
@@ -814,7 +814,7 @@ int dst_label_loss_backward(const DstLabelParams *p, void *stream) {
             a.inverse = a.upstream_rows ? nullptr : p->inverse;
             a.out = dx ? p->grad_features : p->grad_weight, a.bias_out = p->grad_bias;
             const dim3 grid((uint32_t)a.cut.blocks());
-            if (!copied) prepare(b.sets.x, s), prepare(b.sets.w, s);   // (both passes have the copies in the same place)
+            if (!copied) prepare({&b.sets.x, &b.sets.w}, s);   // (both passes have the copies in the same place)
             copied = true;
             if (dx && b.few) k_label_dx<TY, NK, 1><<<grid, kThreads, 0, s>>>(a);
             else if (dx) k_label_dx<TY, NK, QB><<<grid, kThreads, 0, s>>>(a);
@@ -844,7 +844,7 @@ int dst_label_best(const DstLabelParams *p, void *stream) {
         if (int rc = check_workspace(p, f.bytes)) return rc;
         a.label = p->best, a.log_prob = p->log_prob;
         const hipStream_t s = (hipStream_t)stream;
-        prepare(f.sets.x, s), prepare(f.sets.w, s);
+        prepare({&f.sets.x, &f.sets.w}, s);
         k_label_bounds<TY><<<kBoundBlocks, kThreads, 0, s>>>(a, const_cast<float *>(a.bounds));
         const dim3 grid((uint32_t)a.cut.blocks());
         if (f.few) k_label_forward<TY, NK, 1, true><<<grid, kThreads, 0, s>>>(a);

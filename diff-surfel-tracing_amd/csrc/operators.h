@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <initializer_list>
 #include <type_traits>
 
 #include "dst_api.h"
@@ -189,8 +190,17 @@ struct RowCopy {
     int64_t rows, all_words;
     uint4 *to;
 };
-__global__ __launch_bounds__(256) void k_copy_rows(RowCopy c) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+constexpr int kMostSets = 5;
+struct CopyList {   // in one launch: set s has the blocks first[s] .. first[s + 1] - 1
+    RowCopy set[kMostSets];
+    uint32_t first[kMostSets + 1];
+};
+__global__ __launch_bounds__(256) void k_copy_rows(CopyList list) {
+    int s = 0;
+#pragma unroll
+    for (int k = 1; k < kMostSets; ++k) s = blockIdx.x >= list.first[k] ? k : s;
+    const RowCopy c = list.set[s];
+    const int64_t i = (int64_t)(blockIdx.x - list.first[s]) * 256 + threadIdx.x;
     if (i >= c.all_words) return;
     const int64_t at = i / c.words, r = at % c.rows, head = at / c.rows % c.heads, batch = at / c.rows / c.heads;
     const int w = (int)(i - at * c.words);
@@ -244,8 +254,18 @@ RowSet row_set(const void *p, int64_t batch, int64_t row, int64_t head, int64_t 
     }
     return s;
 }
-inline void prepare(const RowSet &s, hipStream_t stream) {
-    if (s.copied && s.copy.all_words > 0) k_copy_rows<<<dim3((uint32_t)div_up(s.copy.all_words, 256)), 256, 0, stream>>>(s.copy);
+// Makes the copies of the sets that have any.
+inline void prepare(std::initializer_list<const RowSet *> sets, hipStream_t stream) {
+    CopyList list = {};
+    int n = 0;
+    uint32_t blocks = 0;
+    for (const RowSet *s : sets)
+        if (s->copied && s->copy.all_words > 0) {
+            list.set[n] = s->copy, list.first[n++] = blocks;
+            blocks += (uint32_t)div_up(s->copy.all_words, 256);
+        }
+    for (int k = n; k <= kMostSets; ++k) list.first[k] = blocks;
+    if (blocks > 0) k_copy_rows<<<dim3(blocks), 256, 0, stream>>>(list);
 }
 
 }  // namespace
