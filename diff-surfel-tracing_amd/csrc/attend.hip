@@ -516,7 +516,7 @@ AttendArgs arguments(const DstAttendParams *p) {
 // f(type, integral constant of the fragments) for the call's type and channels
 template <class F> int with_type(const DstAttendParams *p, F f) {
     const int nk = fragments_of(longest(p), p->dtype);
-    if (p->dtype == DST_DTYPE_F32) return with_floats(longest(p), f);
+    if (p->dtype == DST_DTYPE_F32) return with_floats<false>(longest(p), f);
     return p->dtype == DST_DTYPE_BF16 ? with_fragments<BF16>(nk, f) : with_fragments<F16>(nk, f);
 }
 
@@ -729,7 +729,7 @@ int dst_attend_backward(const DstAttendParams *p, void *stream) {
         }
         return (int)DST_OK;
     };
-    return p->dtype == DST_DTYPE_F32 ? with_floats(longest(p), launch) : with_fragments<BF16>(fragments_of(longest(p), p->dtype), launch);
+    return p->dtype == DST_DTYPE_F32 ? with_floats<false>(longest(p), launch) : with_fragments<BF16>(fragments_of(longest(p), p->dtype), launch);
 }
 
 }  // extern "C"

@@ -44,9 +44,16 @@ template <class TY, class F> int with_fragments(int nk, F f) {
         }
     }
 }
-template <class F> int with_floats(int channels, F f) {
+// (SHORT: for products with a table, whose rows of up to eight values have a type of their own)
+template <bool SHORT, class F> int with_floats(int channels, F f) {
     const int nk = fragments_of(channels, DST_DTYPE_F32);
-    return channels <= kLongest32 ? with_fragments<F32>(nk, f) : with_fragments<Split32>(nk, f);
+    if constexpr (SHORT) {
+        if (channels <= 8) return f(Short32{}, std::integral_constant<int, 0>{});
+        if (channels <= kLongest32) return f(F32{}, std::integral_constant<int, 1>{});
+    } else {
+        if (channels <= kLongest32) return with_fragments<F32>(nk, f);
+    }
+    return with_fragments<Split32>(nk, f);
 }
 inline int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline uint64_t align_up(uint64_t bytes) { return (bytes + 255u) & ~(uint64_t)255u; }
