@@ -15,7 +15,7 @@
 namespace {
 
 struct AttendArgs {
-    Rows q, k, v, o, up;           // o: out as the backward pass reads it; up: its gradient
+    Rows q, k, v, o, low, up;      // o, low: out as the backward pass reads it, and what its rounding left; up: its gradient
     const int32_t *lengths;
     int32_t queries, memory, heads, kv_heads, group, rows;   // rows = queries * group
     int32_t d, dv;
@@ -24,7 +24,8 @@ struct AttendArgs {
     float scale, c;                // c: what brings a product of rows to a score in units of log 2, but for what own rows carry
     float own_scale;               // 32-bit rows
     int32_t flip;                  // 16-bit rows
-    void *out;
+    void *out, *out_low;           // out_low: of 16-bit rows, what out's rounding leaves, rounded to the same type; or nullptr
+    int32_t half;                  // gradients are written in binary16 though rows are in 32 bits
     float *lse2, *delta;
     void *dq, *dk, *dvalue;        // contiguous
     float2 *part;                  // of a part's rows: maximum and sum
@@ -58,8 +59,7 @@ __device__ inline int64_t out_row(const AttendArgs &a, const Place &p, int row) 
 // Row of lse, delta and the parts
 __device__ inline int64_t stat_row(const AttendArgs &a, const Place &p, int row) { return ((int64_t)p.batch * a.kv_heads + p.kv) * a.rows + row; }
 
-// What own rows carry of the scores' factor: rows in 32 bits all of it, rows of 16 bits or planes the sign. Either way a row with one
-// weight of 32 bits gets exactly 1: its score less the maximum, which is the score, is 0 (the product with c is rounded first).
+// What own rows carry of the scores' factor: rows in 32 bits all of it, rows of 16 bits or planes the sign.
 template <class TY, int NK, int QB> __device__ inline void carry_scale(Own<TY, NK, QB> &own, const AttendArgs &a) {
 #pragma unroll
     for (int q = 0; q < QB; ++q)
@@ -72,11 +72,25 @@ template <class TY, int NK, int QB> __device__ inline void carry_scale(Own<TY, N
                 else if (a.flip) w ^= u4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
             }
 }
-// The weight of a product of rows, `less` its row's maximum or lse.
-template <class TY> __device__ inline float weight_of(const AttendArgs &a, float s, float less) {
-    if constexpr (TY::kRounds) return exp2_of(__builtin_fmaf(s, a.c, -less));
-    else if constexpr (TY::kPlanes == 3) return exp2_of(s * a.c - less);
-    else return exp2_of(s - less);
+// The weight of a product of rows, `less` its row's maximum or lse. EXACT: the score is rounded before the difference is
+// formed, so a row with one weight gets exactly 1, its value and, in the backward pass, scores without a gradient. A forward pass that
+// a backward pass follows is exact; the others save the instruction (131,072 rows x 1024 in 4 heads of 64: 184 us, 176).
+template <class TY, bool EXACT> __device__ inline float weight_of(const AttendArgs &a, float s, float less) {
+    if constexpr (TY::kDepth == 16) return exp2_of(s - less);
+    else if constexpr (EXACT || TY::kPlanes == 3) return exp2_of(s * a.c - less);
+    else return exp2_of(__builtin_fmaf(s, a.c, -less));
+}
+
+// A row of out, and of what its rounding leaves: delta, a difference of what cancels, is formed of both.
+template <class E> __device__ inline void store_out(const AttendArgs &a, int64_t row, int at, f4 v, bool four) {
+    store_four(reinterpret_cast<E *>(a.out) + row * a.dv, at, a.dv, v, four);
+    if constexpr (sizeof(E) == 2)
+        if (a.out_low) {
+            f4 rest;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) rest[i] = v[i] - (float)(E)v[i];
+            store_four(reinterpret_cast<E *>(a.out_low) + row * a.dv, at, a.dv, rest, four);
+        }
 }
 
 // ---- forward --------------------------------------------------------------------------------------------------------
@@ -84,7 +98,7 @@ template <class TY> __device__ inline float weight_of(const AttendArgs &a, float
 // stay below 2^kSlack, which every type holds, and most tiles need no exchange between lanes.
 constexpr float kSlack = 8.0f;
 
-template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void k_attend_forward(AttendArgs a) {
+template <class TY, int NK, int QB, bool EXACT> __global__ __launch_bounds__(kThreads) void k_attend_forward(AttendArgs a) {
     typedef Shape<TY, NK> T;
     typedef typename TY::E E;
     constexpr int NM = depth_blocks<TY, NK>();
@@ -159,7 +173,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[j][q][r] = weight_of<TY>(a, s[j][q][r], use);
+                    for (int r = 0; r < 4; ++r) s[j][q][r] = weight_of<TY, EXACT>(a, s[j][q][r], use);
                 const f4 u = s[0][q], v = s[1][q];
                 l[q] += ((u[0] + u[1]) + (u[2] + u[3])) + ((v[0] + v[1]) + (v[2] + v[3]));
             }
@@ -184,9 +198,9 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
         }
         const float by = p.length > 0 ? 1.0f / sum : 0.0f;
         if (g == 0 && a.lse2) a.lse2[at] = p.length > 0 ? m[q] + log2_of(sum) : kInf;
-        E *o = reinterpret_cast<E *>(a.out) + out_row(a, p, row) * a.dv;
+        const int64_t to = out_row(a, p, row);
 #pragma unroll
-        for (int i = 0; i < NM; ++i) store_four(o, i * 16 + 4 * g, a.dv, out[q][i] * by, four);
+        for (int i = 0; i < NM; ++i) store_out<E>(a, to, i * 16 + 4 * g, out[q][i] * by, four);
     }
 }
 
@@ -244,7 +258,7 @@ template <class E> __global__ __launch_bounds__(kThreads) void k_attend_join_row
     }
     if (tid == 0 && a.lse2) a.lse2[at] = length > 0 ? m + log2_of(l) : kInf;
     if (lane == 0 && word < words)
-        store_four(reinterpret_cast<E *>(a.out) + out_row(a, p, row) * a.dv, 4 * word, a.dv, length > 0 ? sums[tid] * (1.0f / l) : sums[tid], four);
+        store_out<E>(a, out_row(a, p, row), 4 * word, length > 0 ? sums[tid] * (1.0f / l) : sums[tid], four);
 }
 
 // The same, a thread for four channels of a row.
@@ -278,19 +292,23 @@ template <class E> __global__ __launch_bounds__(kThreads) void k_attend_join(Att
         }
     }
     if (c == 0 && a.lse2) a.lse2[at] = length > 0 ? m + log2_of(l) : kInf;
-    store_four(reinterpret_cast<E *>(a.out) + out_row(a, p, row) * a.dv, c, a.dv, length > 0 ? o * (1.0f / l) : o, four);
+    store_out<E>(a, out_row(a, p, row), c, length > 0 ? o * (1.0f / l) : o, four);
 }
 
 // ---- backward -------------------------------------------------------------------------------------------------------
 // delta of the wave's rows, from fragments: by the matrix instruction that also forms do . v, so that where a row's weight is
 // on one value alone (o = v) the two are the same number and its ds is 0, not a rounding error.
-template <class TY, int NK, int QB> __device__ inline void deltas(const Own<TY, NK, QB> &o, const Own<TY, NK, QB> &up, float (&delta)[QB]) {
+template <class TY, int NK, int QB>
+__device__ inline void deltas(const Own<TY, NK, QB> &o, const Own<TY, NK, QB> &low, const Own<TY, NK, QB> &up, float (&delta)[QB]) {
     const int lane = threadIdx.x & 63, g = lane >> 4, l = lane & 15;
 #pragma unroll
     for (int q = 0; q < QB; ++q) {
         f4 s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int k = 0; k < fragments<NK>(); ++k) s = fragment_product<TY, NK>(o.f[q][k], up.f[q][k], s);
+        if constexpr (TY::kRounds)
+#pragma unroll
+            for (int k = 0; k < fragments<NK>(); ++k) s = fragment_product<TY, NK>(low.f[q][k], up.f[q][k], s);
         const float mine = (l & 2) ? ((l & 1) ? s[3] : s[2]) : ((l & 1) ? s[1] : s[0]);
         delta[q] = sum_group(g == (l >> 2) ? mine : 0.0f);   // (the diagonal's one value)
     }
@@ -322,7 +340,11 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     float delta[QB], lse2[QB];
     up.load(a.up, tile_base<true>(a.up, row0, p.batch, p.kv), a.rows - row0);
     own.load(a.o, tile_base<true>(a.o, row0, p.batch, p.kv), a.rows - row0);
-    deltas<TY, NK, QB>(own, up, delta);
+    {
+        Own<TY, NK, QB> low;
+        if constexpr (TY::kRounds) low.load(a.low, tile_base<true>(a.low, row0, p.batch, p.kv), a.rows - row0);
+        deltas<TY, NK, QB>(own, low, up, delta);
+    }
     own.load(a.q, tile_base<true>(a.q, row0, p.batch, p.kv), a.rows - row0);
     carry_scale(own, a);
     f4 out[QB][NM];
@@ -356,7 +378,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
                 for (int q = 0; q < QB; ++q)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        s[j][q][r] = weight_of<TY>(a, s[j][q][r], lse2[q]) * (dp[q][r] - delta[q]);
+                        s[j][q][r] = weight_of<TY, false>(a, s[j][q][r], lse2[q]) * (dp[q][r] - delta[q]);
             }
             accumulate<TY, NK, QB, NM>(tile_k, pair, s[0], s[1], out);
         }
@@ -373,7 +395,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
         for (int i = 0; i < NM; ++i) {
             const f4 v = out[q][i] * a.scale;
             if (turn.part) store_four(a.out_part + part_row(a.cut, turn, kWaves * 16 * QB, wave * 16 * QB + q * 16 + (lane & 15)) * a.d, i * 16 + 4 * g, a.d, v, four);
-            else store_four(reinterpret_cast<E *>(a.dq) + to * a.d, i * 16 + 4 * g, a.d, v, four);
+            else store_sums<E>(a.dq, to, i * 16 + 4 * g, a.d, v, four, a.half);
         }
     }
 }
@@ -437,7 +459,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
                 for (int q = 0; q < QB; ++q)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float e = weight_of<TY>(a, s[j][q][r], lse2[r]);
+                        const float e = weight_of<TY, false>(a, s[j][q][r], lse2[r]);
                         s[j][q][r] = e;
                         dp[j][q][r] = e * (dp[j][q][r] - delta[r]);
                     }
@@ -463,8 +485,8 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
                 store_four(a.out_part + part * a.d, i * 16 + 4 * g, a.d, k, four_k);
                 store_four(a.out_part2 + part * a.dv, i * 16 + 4 * g, a.dv, v, four_v);
             } else {
-                if (a.dk) store_four(reinterpret_cast<E *>(a.dk) + to * a.d, i * 16 + 4 * g, a.d, k, four_k);
-                if (a.dvalue) store_four(reinterpret_cast<E *>(a.dvalue) + to * a.dv, i * 16 + 4 * g, a.dv, v, four_v);
+                if (a.dk) store_sums<E>(a.dk, to, i * 16 + 4 * g, a.d, k, four_k, a.half);
+                if (a.dvalue) store_sums<E>(a.dvalue, to, i * 16 + 4 * g, a.dv, v, four_v, a.half);
             }
         }
     }
@@ -496,7 +518,7 @@ int check(const DstAttendParams *p) {
 
 int longest(const DstAttendParams *p) { return p->channels > p->value_channels ? p->channels : p->value_channels; }
 
-AttendArgs arguments(const DstAttendParams *p) {
+template <class TY> AttendArgs arguments(const DstAttendParams *p) {
     AttendArgs a = {};
     a.lengths = p->lengths;
     a.queries = p->queries, a.memory = p->memory, a.heads = p->heads, a.kv_heads = p->kv_heads;
@@ -507,8 +529,9 @@ AttendArgs arguments(const DstAttendParams *p) {
     // -inf what it is)
     a.c = __builtin_fabsf(p->scale) * kLog2E;
     if (a.c < 1.1754944e-38f) a.c = 1.1754944e-38f;
-    if (p->dtype == DST_DTYPE_F32 && longest(p) <= kLongest32) a.own_scale = a.flip ? -a.c : a.c, a.c = 1.0f;
-    a.out = p->out, a.lse2 = p->lse;
+    if (std::is_same_v<TY, F32>) a.own_scale = a.flip ? -a.c : a.c, a.c = 1.0f;
+    a.out = p->out, a.out_low = p->out_low, a.lse2 = p->lse;
+    a.half = p->dtype == DST_DTYPE_F16 && sizeof(typename TY::E) == 4;
     a.all_rows = (int64_t)p->batch * p->kv_heads * a.rows;
     return a;
 }
@@ -519,19 +542,23 @@ template <class F> int with_type(const DstAttendParams *p, F f) {
     if (p->dtype == DST_DTYPE_F32) return with_floats<false>(longest(p), f);
     return p->dtype == DST_DTYPE_BF16 ? with_fragments<BF16>(nk, f) : with_fragments<F16>(nk, f);
 }
+// Gradients of binary16 rows are formed in 32 bits.
+template <class F> int with_gradients(const DstAttendParams *p, F f) {
+    return p->dtype == DST_DTYPE_BF16 ? with_fragments<BF16>(fragments_of(longest(p), p->dtype), f) : with_floats<false>(longest(p), f);
+}
 
 // The rows of all sets, copied into the workspace's front where the kernels cannot read them where they lie.
 struct Sets {
-    RowSet q, k, v, o, up;
+    RowSet q, k, v, o, low, up;
 };
 template <class TY, int NK> Sets row_sets(const DstAttendParams *p, AttendArgs &a, bool backward, Carve &c) {
     // (a group has to fit whole into the steps between a thread's words, and into the blocks of 16 own rows)
     const int stride = Shape<TY, NK>::kStride < 16 ? Shape<TY, NK>::kStride : 16, group = a.group;
     auto memory = [&](const void *t, const int64_t (&s)[3], int channels) {
-        return row_set<TY>(t, s[0], s[1], s[2], p->batch, p->kv_heads, 1, p->memory, channels, stride, c);
+        return row_set<TY>(t, p->dtype, s[0], s[1], s[2], p->batch, p->kv_heads, 1, p->memory, channels, stride, c);
     };
-    auto queries = [&](const void *t, int64_t batch, int64_t row, int64_t head, int channels) {
-        return row_set<TY>(t, batch, row, head, p->batch, p->kv_heads, group, a.rows, channels, stride, c);
+    auto queries = [&](const void *t, int64_t batch, int64_t row, int64_t head, int channels, const void *low = nullptr) {
+        return row_set<TY>(t, p->dtype, batch, row, head, p->batch, p->kv_heads, group, a.rows, channels, stride, c, low);
     };
     const int64_t row = (int64_t)p->heads * p->value_channels;
     Sets s = {};
@@ -539,13 +566,14 @@ template <class TY, int NK> Sets row_sets(const DstAttendParams *p, AttendArgs &
     s.k = memory(p->k, p->k_strides, p->channels);
     s.v = memory(p->v, p->v_strides, p->value_channels);
     if (backward) {
-        s.o = queries(p->out, p->queries * row, row, p->value_channels, p->value_channels);
+        s.o = queries(p->out, p->queries * row, row, p->value_channels, p->value_channels, p->out_low);
+        if (TY::kRounds) s.low = queries(p->out_low, p->queries * row, row, p->value_channels, p->value_channels);
         s.up = queries(p->upstream, p->queries * row, row, p->value_channels, p->value_channels);
     }
-    a.q = s.q.rows, a.k = s.k.rows, a.v = s.v.rows, a.o = s.o.rows, a.up = s.up.rows;
+    a.q = s.q.rows, a.k = s.k.rows, a.v = s.v.rows, a.o = s.o.rows, a.low = s.low.rows, a.up = s.up.rows;
     return s;
 }
-void prepare(const Sets &s, hipStream_t stream) { prepare({&s.q, &s.k, &s.v, &s.o, &s.up}, stream); }
+void prepare(const Sets &s, hipStream_t stream) { prepare({&s.q, &s.k, &s.v, &s.o, &s.low, &s.up}, stream); }
 
 // Cuts a pass's own tiles; whether its rows are few. `kernel(few)`: the pass's kernel; `own_bytes`: of a part's row.
 template <class TY, int NK, class K>
@@ -567,8 +595,9 @@ struct Plan {
 };
 template <class TY, int NK> Plan plan_forward(AttendArgs &a, int64_t heads, Carve c) {
     Plan p;
+    constexpr bool some = !TY::kRounds;   // (32-bit rows are always exact)
     p.few = plan_cut<TY, NK>(a, forward_blocks<TY, NK>(), a.rows, a.memory, heads, 2, a.dv * 4.0 + 8.0, [](bool few) {
-        return few ? (const void *)&k_attend_forward<TY, NK, 1> : (const void *)&k_attend_forward<TY, NK, forward_blocks<TY, NK>()>;
+        return few ? (const void *)&k_attend_forward<TY, NK, 1, some> : (const void *)&k_attend_forward<TY, NK, forward_blocks<TY, NK>(), some>;
     });
     if (const uint64_t rows = parted_rows(a)) {
         a.part = c.take<float2>(rows);
@@ -633,26 +662,34 @@ extern "C" {
 uint64_t dst_attend_workspace_bytes(const DstAttendParams *p, int pass) {
     if (check(p) != DST_OK) return 0;
     uint64_t bytes = 0;
-    with_type(p, [&](auto ty, auto nk) {
-        typedef decltype(ty) TY;
-        constexpr int NK = decltype(nk)::value;
-        AttendArgs a = arguments(p);
-        const int64_t heads = (int64_t)p->batch * p->kv_heads;
-        if (a.all_rows == 0 && pass == DST_PASS_FORWARD) return DST_OK;
-        Carve c = {nullptr, 0};
-        row_sets<TY, NK>(p, a, pass != DST_PASS_FORWARD, c);
-        if (pass == DST_PASS_FORWARD) {
+    const int64_t heads = (int64_t)p->batch * p->kv_heads;
+    if (pass == DST_PASS_FORWARD) {
+        with_type(p, [&](auto ty, auto nk) {
+            typedef decltype(ty) TY;
+            constexpr int NK = decltype(nk)::value;
+            AttendArgs a = arguments<TY>(p);
+            if (a.all_rows == 0) return DST_OK;
+            Carve c = {nullptr, 0};
+            row_sets<TY, NK>(p, a, false, c);
             bytes = plan_forward<TY, NK>(a, heads, c).bytes;
-        } else {
+            return DST_OK;
+        });
+    } else {
+        with_gradients(p, [&](auto ty, auto nk) {
+            typedef decltype(ty) TY;
+            constexpr int NK = decltype(nk)::value;
+            AttendArgs a = arguments<TY>(p);
+            Carve c = {nullptr, 0};
+            row_sets<TY, NK>(p, a, true, c);
             a.dq = p->grad_q;
             bytes = plan_dq<TY, NK>(a, heads, c).bytes;
             if (p->grad_k || p->grad_v) {
                 const uint64_t more = plan_dkv<TY, NK>(a, heads, c).bytes;
                 bytes = more > bytes ? more : bytes;
             }
-        }
-        return DST_OK;
-    });
+            return DST_OK;
+        });
+    }
     return bytes;
 }
 
@@ -662,7 +699,7 @@ int dst_attend_forward(const DstAttendParams *p, void *stream) {
         typedef decltype(ty) TY;
         typedef typename TY::E E;
         constexpr int NK = decltype(nk)::value, QB = forward_blocks<TY, NK>();
-        AttendArgs a = arguments(p);
+        AttendArgs a = arguments<TY>(p);
         if (a.all_rows == 0) return (int)DST_OK;
         const int64_t heads = (int64_t)p->batch * p->kv_heads;
         Carve c = {(char *)p->workspace, 0};
@@ -672,8 +709,13 @@ int dst_attend_forward(const DstAttendParams *p, void *stream) {
         const hipStream_t s = (hipStream_t)stream;
         prepare(sets, s);
         const dim3 grid((uint32_t)a.cut.blocks());
-        if (plan.few) k_attend_forward<TY, NK, 1><<<grid, kThreads, 0, s>>>(a);
-        else k_attend_forward<TY, NK, QB><<<grid, kThreads, 0, s>>>(a);
+        if (TY::kRounds && !a.out_low) {
+            if (plan.few) k_attend_forward<TY, NK, 1, !TY::kRounds><<<grid, kThreads, 0, s>>>(a);
+            else k_attend_forward<TY, NK, QB, !TY::kRounds><<<grid, kThreads, 0, s>>>(a);
+        } else {
+            if (plan.few) k_attend_forward<TY, NK, 1, true><<<grid, kThreads, 0, s>>>(a);
+            else k_attend_forward<TY, NK, QB, true><<<grid, kThreads, 0, s>>>(a);
+        }
         DST_OP_LAUNCH("attention");
         if (a.cut.splits > 1) {
             const int64_t rows = a.cut.parted() * a.own;
@@ -689,18 +731,19 @@ int dst_attend_forward(const DstAttendParams *p, void *stream) {
 
 int dst_attend_backward(const DstAttendParams *p, void *stream) {
     if (int rc = check(p)) return rc;
-    if (p->dtype == DST_DTYPE_F16) return dst_op_fail(DST_E_UNSUPPORTED, "gradients are of float32 and bfloat16 rows");
     if (!p->grad_q && !p->grad_k && !p->grad_v) return DST_OK;
     if (p->batch > 0 && p->queries > 0 && (!p->lse || !p->upstream)) return dst_op_fail(DST_E_INVALID, "lse and upstream are required");
+    if (p->batch > 0 && p->queries > 0 && p->dtype != DST_DTYPE_F32 && !p->out_low)
+        return dst_op_fail(DST_E_INVALID, "out_low is required of 16-bit rows");
     if ((reinterpret_cast<uintptr_t>(p->grad_q) | reinterpret_cast<uintptr_t>(p->grad_k) | reinterpret_cast<uintptr_t>(p->grad_v)) & 15u)
         return dst_op_fail(DST_E_INVALID, "gradients must be aligned to 16 bytes");
-    auto launch = [&](auto ty, auto nk) {
+    return with_gradients(p, [&](auto ty, auto nk) {
         typedef decltype(ty) TY;
         typedef typename TY::E E;
         constexpr int NK = decltype(nk)::value;
         const hipStream_t s = (hipStream_t)stream;
         const int64_t heads = (int64_t)p->batch * p->kv_heads;
-        AttendArgs a = arguments(p);
+        AttendArgs a = arguments<TY>(p);
         Carve c = {(char *)p->workspace, 0};
         const Sets sets = row_sets<TY, NK>(p, a, true, c);
         a.dq = p->grad_q, a.dk = p->grad_k, a.dvalue = p->grad_v;
@@ -713,7 +756,10 @@ int dst_attend_backward(const DstAttendParams *p, void *stream) {
             else k_attend_dq<TY, NK, dq_blocks<TY, NK>()><<<grid, kThreads, 0, s>>>(a);
             DST_OP_LAUNCH("attention gradient, queries");
             const QueryRow to = {a.cut.whole, a.tiles, a.own, a.rows, a.kv_heads, a.group, a.queries};
-            sum_parts(Parts<E>{a.out_part, (E *)a.dq, a.d}, Parts<E>{nullptr, nullptr, 1}, a.cut, a.own, to, s);
+            with_output<E>(a.half, [&](auto one) {
+                typedef decltype(one) To;
+                sum_parts(Parts<To>{a.out_part, (To *)a.dq, a.d}, Parts<To>{nullptr, nullptr, 1}, a.cut, a.own, to, s);
+            });
             DST_OP_LAUNCH("attention gradient, summing");
         }
         if ((a.dk || a.dvalue) && heads * a.memory > 0) {
@@ -724,12 +770,14 @@ int dst_attend_backward(const DstAttendParams *p, void *stream) {
             else k_attend_dkv<TY, NK, dkv_blocks<TY, NK>()><<<grid, kThreads, 0, s>>>(a);
             DST_OP_LAUNCH("attention gradient, memory");
             const MemoryRow to = {a.cut.whole, a.tiles, a.own, a.memory, a.kv_heads};
-            sum_parts(Parts<E>{a.out_part, (E *)a.dk, a.d}, Parts<E>{a.out_part2, (E *)a.dvalue, a.dv}, a.cut, a.own, to, s);
+            with_output<E>(a.half, [&](auto one) {
+                typedef decltype(one) To;
+                sum_parts(Parts<To>{a.out_part, (To *)a.dk, a.d}, Parts<To>{a.out_part2, (To *)a.dvalue, a.dv}, a.cut, a.own, to, s);
+            });
             DST_OP_LAUNCH("attention gradient, summing");
         }
         return (int)DST_OK;
-    };
-    return p->dtype == DST_DTYPE_F32 ? with_floats<false>(longest(p), launch) : with_fragments<BF16>(fragments_of(longest(p), p->dtype), launch);
+    });
 }
 
 }  // extern "C"

@@ -42,6 +42,7 @@ struct LabelArgs {
     const float *upstream;          // (rays) or one value
     const float *inverse;           // one value that multiplies a single upstream value, or nullptr
     int32_t upstream_rows;
+    int32_t half;                   // gradients are written in binary16 though rows are in 32 bits
     void *out;                      // (rays, d) or (labels, d), of the inputs' type
     float *out_part;                // of a part's rows: d values
     float *bias_out, *bias_part;    // (labels); of a part's rows
@@ -473,7 +474,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
             f4 v = out[q][m] * up[q];
             if (up[q] == 0.0f) v = f4{0.0f, 0.0f, 0.0f, 0.0f};   // (an ignored ray's channels may hold anything)
             if (turn.part) store_four(a.out_part + part_row(a.cut, turn, kWaves * 16 * QB, wave * 16 * QB + q * 16 + (lane & 15)) * a.d, m * 16 + 4 * g, a.d, v, four);
-            else store_four(reinterpret_cast<E *>(a.out) + row * a.d, m * 16 + 4 * g, a.d, v, four);
+            else store_sums<E>(a.out, row, m * 16 + 4 * g, a.d, v, four, a.half);
         }
     }
 }
@@ -593,7 +594,7 @@ template <class TY, int NK, int QB, bool ONE> __global__ __launch_bounds__(kThre
 #pragma unroll
         for (int m = 0; m < NM; ++m) {
             if (turn.part) store_four(a.out_part + part * a.d, m * 16 + 4 * g, a.d, out[q][m] * by, four);
-            else if (a.out) store_four(reinterpret_cast<E *>(a.out) + (int64_t)v * a.d, m * 16 + 4 * g, a.d, out[q][m] * by, four);
+            else if (a.out) store_sums<E>(a.out, v, m * 16 + 4 * g, a.d, out[q][m] * by, four, a.half);
         }
     }
 }
@@ -631,8 +632,8 @@ struct Sets {
 };
 template <class TY> Sets row_sets(const DstLabelParams *p, Carve &c) {
     Sets s;
-    s.x = row_set<TY>(p->features, 0, p->features_stride, 0, 1, 1, 1, p->rays, p->channels, 1, c);
-    s.w = row_set<TY>(p->weight, 0, p->weight_stride, 0, 1, 1, 1, p->labels, p->channels, 1, c);
+    s.x = row_set<TY>(p->features, p->dtype, 0, p->features_stride, 0, 1, 1, 1, p->rays, p->channels, 1, c);
+    s.w = row_set<TY>(p->weight, p->dtype, 0, p->weight_stride, 0, 1, 1, 1, p->labels, p->channels, 1, c);
     return s;
 }
 
@@ -643,11 +644,14 @@ template <class TY, int NK> struct Shapes {   // own rows of a workgroup, rows o
 
 // f(type, integral constant of the fragments) for the call's type and channels. The backward kernels take 32-bit rows of up to eight values
 // in planes (Short32), the forward ones, which have half the products, in 32 bits (921,600 rays x 256 labels: dx 111 us for 131,
-// dw 128 for 155, forward 96 for 89).
-template <bool BACKWARD, class F> int with_type(const DstLabelParams *p, F f) {
+// dw 128 for 155, forward 96 for 89). Gradients of binary16 rows are formed in 32 bits.
+template <class F> int with_type(const DstLabelParams *p, F f) {
     const int nk = fragments_of(p->channels, p->dtype);
-    if (p->dtype == DST_DTYPE_F32) return with_floats<BACKWARD>(p->channels, f);
+    if (p->dtype == DST_DTYPE_F32) return with_floats<false>(p->channels, f);
     return p->dtype == DST_DTYPE_BF16 ? with_fragments<BF16>(nk, f) : with_fragments<F16>(nk, f);
+}
+template <class F> int with_gradients(const DstLabelParams *p, F f) {
+    return p->dtype == DST_DTYPE_BF16 ? with_fragments<BF16>(fragments_of(p->channels, p->dtype), f) : with_floats<true>(p->channels, f);
 }
 
 struct ForwardPlan {
@@ -748,19 +752,16 @@ uint64_t dst_label_workspace_bytes(const DstLabelParams *p, int pass) {
     uint64_t bytes = 0;
     LabelArgs a = {};
     if (pass == DST_PASS_BACKWARD) {
-        if (p->dtype == DST_DTYPE_F16) return 0;
-        with_type<true>(p, [&](auto ty, auto nk) {
+        with_gradients(p, [&](auto ty, auto nk) {
             typedef decltype(ty) TY;
             constexpr int NK = decltype(nk)::value;
-            if constexpr (!std::is_same_v<TY, F16>) {
-                const uint64_t x = p->grad_features ? backward_plan<TY, NK, true>(p, a, nullptr).bytes : 0;
-                const uint64_t w = p->grad_weight || p->grad_bias ? backward_plan<TY, NK, false>(p, a, nullptr).bytes : 0;
-                bytes = x > w ? x : w;
-            }
+            const uint64_t x = p->grad_features ? backward_plan<TY, NK, true>(p, a, nullptr).bytes : 0;
+            const uint64_t w = p->grad_weight || p->grad_bias ? backward_plan<TY, NK, false>(p, a, nullptr).bytes : 0;
+            bytes = x > w ? x : w;
             return DST_OK;
         });
     } else {
-        with_type<false>(p, [&](auto ty, auto nk) {
+        with_type(p, [&](auto ty, auto nk) {
             typedef decltype(ty) TY;
             constexpr int NK = decltype(nk)::value;
             bytes = pass == DST_PASS_BEST ? forward_plan<TY, NK, true>(p, a, nullptr).bytes : forward_plan<TY, NK, false>(p, a, nullptr).bytes;
@@ -775,7 +776,7 @@ int dst_label_loss_forward(const DstLabelParams *p, void *stream) {
     if (p->rays > 0 && (!p->targets || !p->lse)) return dst_op_fail(DST_E_INVALID, "targets and lse are required");
     if (!p->loss && (p->rays > 0 || p->reduction != DST_REDUCE_NONE)) return dst_op_fail(DST_E_INVALID, "loss is required");
     if (p->reduction != DST_REDUCE_NONE && !p->inverse) return dst_op_fail(DST_E_INVALID, "a reduced loss needs inverse");
-    return with_type<false>(p, [&](auto ty, auto nk) {
+    return with_type(p, [&](auto ty, auto nk) {
         typedef decltype(ty) TY;
         constexpr int NK = decltype(nk)::value;
         LabelArgs a = arguments(p);
@@ -807,10 +808,9 @@ int dst_label_loss_backward(const DstLabelParams *p, void *stream) {
     if (int rc = check(p)) return rc;
     if (p->rays > 0 && (!p->targets || !p->lse || !p->upstream)) return dst_op_fail(DST_E_INVALID, "targets, lse and upstream are required");
     if (p->reduction != DST_REDUCE_NONE && !p->inverse) return dst_op_fail(DST_E_INVALID, "a reduced loss needs inverse");
-    if (p->dtype == DST_DTYPE_F16) return dst_op_fail(DST_E_UNSUPPORTED, "gradients are of float32 and bfloat16 features");
     if ((reinterpret_cast<uintptr_t>(p->grad_features) | reinterpret_cast<uintptr_t>(p->grad_weight)) & 15u)
         return dst_op_fail(DST_E_INVALID, "gradients must be aligned to 16 bytes");
-    auto launch = [&](auto ty, auto nk) {
+    return with_gradients(p, [&](auto ty, auto nk) {
         typedef decltype(ty) TY;
         typedef typename TY::E E;
         constexpr int NK = decltype(nk)::value, QB = backward_blocks<TY, NK>();
@@ -822,6 +822,7 @@ int dst_label_loss_backward(const DstLabelParams *p, void *stream) {
             LabelArgs a = arguments(p);
             const BackwardPlan b = dx ? backward_plan<TY, NK, true>(p, a, (char *)p->workspace) : backward_plan<TY, NK, false>(p, a, (char *)p->workspace);
             if (int rc = check_workspace(p, b.bytes)) return rc;
+            a.half = p->dtype == DST_DTYPE_F16;
             a.upstream = p->upstream, a.upstream_rows = p->reduction == DST_REDUCE_NONE;
             a.inverse = a.upstream_rows ? nullptr : p->inverse;
             a.out = dx ? p->grad_features : p->grad_weight, a.bias_out = p->grad_bias;
@@ -836,19 +837,21 @@ int dst_label_loss_backward(const DstLabelParams *p, void *stream) {
             else k_label_dw<TY, NK, QB, true><<<grid, kThreads, 0, s>>>(a);
             DST_OP_LAUNCH("label gradient");
             const LabelRow to = {(int64_t)a.cut.whole * a.own, dx ? p->rays : (int64_t)p->labels, a.own};
-            sum_parts(Parts<E>{a.out_part, (E *)a.out, p->channels}, Parts<float>{a.bias_part, dx ? nullptr : p->grad_bias, 1}, a.cut, a.own, to, s);
+            with_output<E>(a.half, [&](auto one) {
+                typedef decltype(one) To;
+                sum_parts(Parts<To>{a.out_part, (To *)a.out, p->channels}, Parts<float>{a.bias_part, dx ? nullptr : p->grad_bias, 1}, a.cut, a.own, to, s);
+            });
             DST_OP_LAUNCH("label gradient, summing");
         }
         return (int)DST_OK;
-    };
-    return p->dtype == DST_DTYPE_F32 ? with_floats<true>(p->channels, launch) : with_fragments<BF16>(fragments_of(p->channels, p->dtype), launch);
+    });
 }
 
 int dst_label_best(const DstLabelParams *p, void *stream) {
     if (int rc = check(p)) return rc;
     if (p->rays == 0) return DST_OK;
     if (!p->best || !p->log_prob) return dst_op_fail(DST_E_INVALID, "best and log_prob are required");
-    return with_type<false>(p, [&](auto ty, auto nk) {
+    return with_type(p, [&](auto ty, auto nk) {
         typedef decltype(ty) TY;
         constexpr int NK = decltype(nk)::value;
         LabelArgs a = arguments(p);

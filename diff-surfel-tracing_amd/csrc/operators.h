@@ -179,6 +179,12 @@ __global__ __launch_bounds__(256) void k_sum_parts(Parts<E> a, Parts<E2> b, Cut 
         else a.out[where * width + (i - row * width)] = (E)s;
     }
 }
+// f(a value of the type that gradients of E rows are written in)
+template <class E, class F> inline void with_output(bool half, F f) {
+    if constexpr (sizeof(E) == 4)
+        if (half) return f((_Float16)0.0f);
+    f(E{});
+}
 template <class E, class E2, class To> inline void sum_parts(Parts<E> a, Parts<E2> b, const Cut &cut, int own, To to, hipStream_t s) {
     if (cut.splits < 2 || (!a.out && !b.out)) return;
     const int columns = cut.splits >= 16 ? 32 : 256;
@@ -189,15 +195,15 @@ template <class E, class E2, class To> inline void sum_parts(Parts<E> a, Parts<E
 }
 
 // Rows that the kernels cannot read where they lie, copied: (batches, heads, rows) of whole words, zeros behind the channels; 32-bit
-// values split into planes where `split`.
+// values split into planes where `split`, binary16 values widened to 32 bits where `half`; `low`: 0, or rows like `from` that are added.
 struct RowCopy {
-    const char *from;
+    const char *from, *low;
     int64_t batch, row, in_group;   // bytes; a head is `group` steps of in_group
-    int32_t heads, group, size, channels, words, split;
+    int32_t heads, group, size, channels, words, split, half;
     int64_t rows, all_words;
     uint4 *to;
 };
-constexpr int kMostSets = 5;
+constexpr int kMostSets = 6;
 struct CopyList {   // in one launch: set s has the blocks first[s] .. first[s + 1] - 1
     RowCopy set[kMostSets];
     uint32_t first[kMostSets + 1];
@@ -211,25 +217,27 @@ __global__ __launch_bounds__(256) void k_copy_rows(CopyList list) {
     if (i >= c.all_words) return;
     const int64_t at = i / c.words, r = at % c.rows, head = at / c.rows % c.heads, batch = at / c.rows / c.heads;
     const int w = (int)(i - at * c.words);
-    const char *from = c.from + batch * c.batch + r / c.group * c.row + (head * c.group + r % c.group) * c.in_group;
+    const int64_t offset = batch * c.batch + r / c.group * c.row + (head * c.group + r % c.group) * c.in_group;
+    const char *from = c.from + offset;
+    auto value = [&](int k) {   // in 32 bits
+        if (k >= c.channels) return 0.0f;
+        if (!c.half) return reinterpret_cast<const float *>(from)[k];
+        const float v = (float)reinterpret_cast<const _Float16 *>(from)[k];
+        return c.low ? v + (float)reinterpret_cast<const _Float16 *>(c.low + offset)[k] : v;
+    };
     if (c.split) {
-        f4 v[2] = {};
-        for (int h = 0; h < 2; ++h) {
-            const float *p = reinterpret_cast<const float *>(from) + 8 * w + 4 * h;
-            if (8 * w + 4 * h + 4 <= c.channels) __builtin_memcpy(&v[h], p, 16);
-            else
-                for (int k = 0; k < 4; ++k)
-                    if (8 * w + 4 * h + k < c.channels) v[h][k] = p[k];
-        }
+        f4 v[2];
+        for (int h = 0; h < 2; ++h)
+            if (!c.half && 8 * w + 4 * h + 4 <= c.channels) __builtin_memcpy(&v[h], from + 32 * w + 16 * h, 16);
+            else v[h] = f4{value(8 * w + 4 * h), value(8 * w + 4 * h + 1), value(8 * w + 4 * h + 2), value(8 * w + 4 * h + 3)};
         u4 planes[3];
         Split32::pack(v[0], v[1], planes);
         for (int p = 0; p < 3; ++p) reinterpret_cast<u4 *>(c.to)[(at * 3 + p) * c.words + w] = planes[p];
         return;
     }
     uint32_t word[4] = {0u, 0u, 0u, 0u};
-    if (c.size == 4) {
-        for (int k = 0; k < 4; ++k)
-            if (4 * w + k < c.channels) word[k] = reinterpret_cast<const uint32_t *>(from)[4 * w + k];
+    if (c.size == 4 || c.half) {
+        for (int k = 0; k < 4; ++k) word[k] = __builtin_bit_cast(uint32_t, value(4 * w + k));
     } else {
         for (int k = 0; k < 8; ++k)
             if (8 * w + k < c.channels) word[k / 2] |= (uint32_t) reinterpret_cast<const uint16_t *>(from)[8 * w + k] << (16 * (k & 1));
@@ -245,18 +253,20 @@ struct RowSet {
     bool copied;
 };
 template <class TY>
-RowSet row_set(const void *p, int64_t batch, int64_t row, int64_t head, int64_t batches, int heads, int group, int64_t n, int channels, int stride, Carve &c) {
+RowSet row_set(const void *p, int dtype, int64_t batch, int64_t row, int64_t head, int64_t batches, int heads, int group, int64_t n, int channels, int stride,
+               Carve &c, const void *low = nullptr) {
     constexpr bool split = TY::kPlanes == 3;
-    const int size = sizeof(typename TY::E), words = split ? (channels + 7) / 8 : (channels * size + 15) / 16;
+    const bool half = dtype == DST_DTYPE_F16 && sizeof(typename TY::E) == 4;   // gradients of binary16 rows are formed in 32 bits
+    const int size = value_size(dtype), words = split ? (channels + 7) / 8 : (channels * (int)sizeof(typename TY::E) + 15) / 16;
     RowSet s = {};
     s.rows = Rows{(const char *)p, batch * size, head * size * group, row * size, head * size > 0x7fffffff ? 0 : (int32_t)(head * size), group, words};
     const int64_t widest = (256 / group + 1) * s.rows.row + (int64_t)group * head * size + 4096;   // within 256 rows
-    s.copied = split || (channels * size) % 16 != 0 || (reinterpret_cast<uintptr_t>(p) & 3u) != 0 || (batch * size) % 4 != 0 ||
+    s.copied = split || half || (channels * size) % 16 != 0 || (reinterpret_cast<uintptr_t>(p) & 3u) != 0 || (batch * size) % 4 != 0 ||
                (row * size) % 4 != 0 || (head * size) % 4 != 0 || stride % group != 0 || widest > 0x7fffffff || head * size > 0x7fffffff;
     if (s.copied) {
         const int64_t all = batches * heads * n * words, line = words * TY::kPlanes * 16;
-        s.copy = RowCopy{(const char *)p, batch * size, row * size, head * size, heads, group, size, channels, words, split, n, all,
-                         c.take<uint4>(all * TY::kPlanes)};
+        s.copy = RowCopy{(const char *)p, half ? (const char *)low : nullptr, batch * size, row * size, head * size, heads, group, size, channels, words,
+                         split, half, n, all, c.take<uint4>(all * TY::kPlanes)};
         s.rows = Rows{(const char *)s.copy.to, (int64_t)heads * n * line, n * line, line, 0, 1, words};
     }
     return s;

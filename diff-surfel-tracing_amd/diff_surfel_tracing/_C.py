@@ -72,7 +72,7 @@ class DstAttendParams(C.Structure):
                                           "dtype")]
                 + [("scale", C.c_float), ("reserved", C.c_int32), ("q", _FP), ("k", _FP), ("v", _FP)]
                 + [(n, C.c_int64 * 3) for n in ("q_strides", "k_strides", "v_strides")]
-                + [(n, _FP) for n in ("lengths", "out", "lse", "upstream", "grad_q", "grad_k", "grad_v", "workspace")]
+                + [(n, _FP) for n in ("lengths", "out", "lse", "out_low", "upstream", "grad_q", "grad_k", "grad_v", "workspace")]
                 + [("workspace_bytes", C.c_uint64)])
 
 

@@ -152,7 +152,7 @@ def label_loss(features, weight, targets, bias=None, *, ignore_index=-100, reduc
     `s = features @ weight.T + bias`, without the logits ever in memory, forward or backward.
 
     features: (..., channels), 1 to 256 channels, for instance a trace's `aux` (H, W, channels); weight: (labels, channels);
-    both float32, bfloat16 or float16 (training in float16 goes through float32 copies); bias: (labels,), -inf switches a
+    both float32, bfloat16 or float16 (gradients in float16 are formed in 32 bits and rounded once); bias: (labels,), -inf switches a
     label off; targets: whole numbers of the leading dimensions of features.  `ignore_index` takes a ray out: no loss, no
     gradient, whatever its channels hold.  Any other target outside 0..labels-1 makes the loss and the gradients it
     reaches NaN.  Returns float32: the mean over the rays not ignored (NaN if there are none), the sum, or with "none" a loss
@@ -167,8 +167,6 @@ def label_loss(features, weight, targets, bias=None, *, ignore_index=-100, reduc
     ignore_index = int(ignore_index)
     shape, d = features.shape[:-1], features.size(-1)
     wants = _wants_grad(features, weight, bias)
-    if wants and features.dtype == torch.float16:   # (gradients of binary16 rows would need a scale of their own)
-        features, weight = features.float(), weight.float()
     x, w, t = _matrix(features, d), _matrix(weight, d), targets.reshape(-1).to(torch.int64).contiguous()
     b = None if bias is None else bias.to(torch.float32).contiguous()
     args = (x, w, t, b, ignore_index, _REDUCTIONS[reduction])
@@ -228,35 +226,39 @@ def _run_attend(p, what, launch, like):
         _fail(rc)
 
 
-def _attend_forward(q, k, v, lengths, scale, wants_lse):
+def _attend_forward(q, k, v, lengths, scale, for_backward):
     with _on(q):
         p = _attend_params(q, k, v, lengths, scale)
         out = torch.empty(q.shape[:3] + v.shape[3:], dtype=q.dtype, device=q.device)
-        lse = None
-        if wants_lse:
+        lse = low = None
+        if for_backward:
             lse = torch.empty(q.size(0) * q.size(1) * q.size(2), dtype=torch.float32, device=q.device)
             p.lse = lse.data_ptr()
+            if q.dtype != torch.float32:
+                low = torch.empty(out.shape, dtype=out.dtype, device=q.device)
+                p.out_low = low.data_ptr()
         p.out = out.data_ptr()
         _run_attend(p, _FORWARD, _C.load_library().dst_attend_forward, q)
-    return out, lse
+    return out, lse, low
 
 
 class _Attend(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lengths, scale):
-        out, lse = _attend_forward(q, k, v, lengths, scale, True)
-        ctx.save_for_backward(q, k, v, lengths, out, lse)
+        out, lse, low = _attend_forward(q, k, v, lengths, scale, True)
+        ctx.save_for_backward(q, k, v, lengths, out, lse, low)
         ctx.scale = scale
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, upstream):
-        q, k, v, lengths, out, lse = ctx.saved_tensors
+        q, k, v, lengths, out, lse, low = ctx.saved_tensors
         with _on(q):
             p = _attend_params(q, k, v, lengths, ctx.scale)
             upstream = upstream.contiguous()
             p.out, p.lse, p.upstream = out.data_ptr(), lse.data_ptr(), upstream.data_ptr()
+            p.out_low = None if low is None else low.data_ptr()
             dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if want else None
                           for t, want in zip((q, k, v), ctx.needs_input_grad))
             p.grad_q, p.grad_k, p.grad_v = (None if t is None else t.data_ptr() for t in (dq, dk, dv))
@@ -269,8 +271,8 @@ def attend_memory(queries, keys, values, lengths=None, *, scale=None):
     `softmax(scale * queries . keys) @ values`, without the weights ever in memory, forward or backward.
 
     queries: (batch, queries, heads, channels); keys: (batch, memory, kv_heads, channels); values: (batch, memory, kv_heads,
-    value_channels); 1 to 256 channels; float32, bfloat16 or float16, one dtype for all (training in float16 goes
-    through float32 copies); any strides.  heads is a multiple of kv_heads: query head h reads kv head h // (heads // kv_heads).
+    value_channels); 1 to 256 channels; float32, bfloat16 or float16, one dtype for all (gradients in float16 are
+    formed in 32 bits and rounded once); any strides.  heads is a multiple of kv_heads: query head h reads kv head h // (heads // kv_heads).
     lengths: (batch,) whole numbers on the same device, how much of its memory each batch has (clamped to 0..memory; None: all).  What lies behind
     it is not used and gets a gradient of zero; a batch without memory gets zeros.  scale: 1 / sqrt(channels) by default.
     Returns (batch, queries, heads, value_channels).  Differentiable (once) in queries, keys and values; the same bits
@@ -294,9 +296,5 @@ def attend_memory(queries, keys, values, lengths=None, *, scale=None):
         lengths = lengths.contiguous()
     scale = queries.size(3) ** -0.5 if scale is None else float(scale)
     wants = _wants_grad(queries, keys, values)
-    dtype = queries.dtype
-    if wants and dtype == torch.float16:   # (gradients of binary16 rows would need a scale of their own)
-        queries, keys, values = queries.float(), keys.float(), values.float()
     q, k, v = _consecutive(queries), _consecutive(keys), _consecutive(values)
-    out = _Attend.apply(q, k, v, lengths, scale) if wants else _attend_forward(q, k, v, lengths, scale, False)[0]
-    return out.to(dtype)
+    return _Attend.apply(q, k, v, lengths, scale) if wants else _attend_forward(q, k, v, lengths, scale, False)[0]

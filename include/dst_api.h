@@ -304,7 +304,7 @@ int dst_pack_sh_half(const float *shs, uint16_t *out, uint64_t n_values, void *s
  * thread's last failure.  All sums are in fp32 or wider and have one order: the same inputs give the same bits. */
 #define DST_DTYPE_F32 0
 #define DST_DTYPE_BF16 1
-#define DST_DTYPE_F16 2             /* forward passes only: gradients of binary16 rows would need a scale of their own */
+#define DST_DTYPE_F16 2             /* gradients of binary16 rows are formed in 32 bits and rounded once */
 #define DST_MAX_CHANNELS 256
 #define DST_MAX_LABELS 0x3fffffff
 #define DST_REDUCE_NONE 0
@@ -365,6 +365,8 @@ typedef struct DstAttendParams {
     void *out;                        /* (batch, queries, heads, value_channels), contiguous, as all that follow */
     float *lse;                       /* (batch, kv_heads, queries * heads / kv_heads): forward writes (NULL: not wanted),
                                        * backward reads (log2 of the sum of exponentials; +inf where there is no memory) */
+    void *out_low;                    /* 16-bit rows: what the rounding of out leaves, of its shape and type: forward writes (NULL: not
+                                       * wanted), backward reads; 32-bit rows: not used */
     const void *upstream;             /* backward: gradient of out, of its shape */
     void *grad_q;                     /* (batch, queries, heads, channels) */
     void *grad_k, *grad_v;            /* (batch, memory, kv_heads, ...): zeros behind the lengths; NULL (either, or grad_q): not wanted */

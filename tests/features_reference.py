@@ -83,14 +83,14 @@ def attend(q, k, v, lengths=None, scale=None, up=None):
             eds = abs(scale) * p * (rel * (dp - delta).abs() + edp) + (half + 4 * U) * ds.abs()
             dq, dk, dv = ds @ K, ds.T @ Q, p.T @ dO
             res["dq"][0][i, :, h] = dq
-            res["dq"][1][i, :, h] = eds @ K.abs() + (n / 16 + 8) * U * (ds.abs() @ K.abs()) + (half + 2 * U) * dq.abs()
+            res["dq"][1][i, :, h] = eds @ K.abs() + (n / 16 + 8) * U * (ds.abs() @ K.abs()) + (half + 2 * U) * dq.abs() + tiny
             rows = Lq * (H // Hkv) / 16 + 8
             res["dk"][0][i, :n, kv] += dk
             res["dk"][1][i, :n, kv] += eds.T @ Q.abs() + rows * U * (ds.abs().T @ Q.abs())
             res["dv"][0][i, :n, kv] += dv
             res["dv"][1][i, :n, kv] += ep.T @ dO.abs() + rows * U * (p.T @ dO.abs())
     for name in ("dk", "dv"):   # (what is written is the sum over the heads)
-        res[name][1].add_((half + 2 * U) * res[name][0].abs())
+        res[name][1].add_((half + 2 * U) * res[name][0].abs() + tiny)
     return res
 
 

@@ -68,8 +68,6 @@ def test_label_calls_without_their_buffers(binding):
     for at, size in ((None, need), (4096, need - 1), (4097, need)):
         p.workspace, p.workspace_bytes = at, size
         assert lib.dst_label_loss_forward(C.byref(p), None) == 1 and b"workspace" in lib.dst_op_error()
-    p = _label(binding, dtype=2, grad_features=4096)
-    assert lib.dst_label_loss_backward(C.byref(p), None) == 5 and b"gradients" in lib.dst_op_error()
     p = _label(binding, grad_features=4100)
     assert lib.dst_label_loss_backward(C.byref(p), None) == 1 and b"aligned" in lib.dst_op_error()
 
@@ -105,7 +103,9 @@ def test_attention_calls_without_their_buffers(binding):
     for name in ("lse", "upstream"):
         assert lib.dst_attend_backward(C.byref(_attend(binding, **{name: None})), None) == 1
         assert name.encode() in lib.dst_op_error()
-    assert lib.dst_attend_backward(C.byref(_attend(binding, dtype=2)), None) == 5
+    for dtype in (1, 2):   # (16-bit rows: what the rounding of out left)
+        assert lib.dst_attend_backward(C.byref(_attend(binding, dtype=dtype)), None) == 1
+        assert b"out_low" in lib.dst_op_error()
     assert lib.dst_attend_backward(C.byref(_attend(binding, grad_q=4104)), None) == 1
     for queries, memory in ((1, 65536), (100, 100)):
         p = _attend(binding, queries=queries, memory=memory)
