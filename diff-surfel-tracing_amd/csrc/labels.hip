@@ -51,9 +51,11 @@ struct LabelArgs {
 constexpr int kBoundBlocks = 64;
 
 // Own blocks of 16 rows of a wave. More of them read a streamed tile fewer times from LDS, fewer leave registers for a second wave
-// on a SIMD, which counts for more (32768 rays x 32771 labels, 256 channels, bf16: dx 1661 us with 2 blocks, 1268 with 1).
+// on a SIMD, which counts for more (32768 rays x 32771 labels, 256 channels, bf16: dx with 2 blocks and one wave 1661 us, with
+// 1 and two 1237, with 2 and two, which its registers just hold, 1042).
 template <class TY, int NK> constexpr int forward_blocks() { return NK <= 1 ? 4 : NK * TY::kPlanes <= 12 ? 2 : 1; }
-template <class TY, int NK> constexpr int backward_blocks() { return NK <= 1 ? (TY::kDepth == 32 ? 2 : 4) : NK * TY::kPlanes <= 6 ? 2 : 1; }
+template <class TY, int NK> constexpr int dx_blocks() { return NK <= 1 ? (TY::kDepth == 32 ? 2 : 4) : NK * TY::kPlanes <= 8 ? 2 : 1; }
+template <class TY, int NK> constexpr int dw_blocks() { return NK <= 1 ? (TY::kDepth == 32 ? 2 : 4) : NK * TY::kPlanes <= 6 ? 2 : 1; }
 
 // The one value that the rays share
 __device__ inline float upstream_value(const LabelArgs &a) { return a.upstream[0] * a.inverse[0]; }
@@ -394,7 +396,7 @@ template <class TY> __global__ __launch_bounds__(kThreads) void k_label_near(Lab
 }
 // ---- backward -------------------------------------------------------------------------------------------------------
 // dx: rays as own rows, the table streamed.
-template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void k_label_dx(LabelArgs a) {
+template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads, TY::kPlanes == 1 ? 2 : 1) void k_label_dx(LabelArgs a) {
     typedef Shape<TY, NK> T;
     constexpr int NM = depth_blocks<TY, NK>();
     __shared__ alignas(16) char tile[T::kTile];
@@ -638,7 +640,8 @@ template <class TY> Sets row_sets(const DstLabelParams *p, Carve &c) {
 }
 
 template <class TY, int NK> struct Shapes {   // own rows of a workgroup, rows of a tile
-    static constexpr int kForward = kWaves * 16 * forward_blocks<TY, NK>(), kBackward = kWaves * 16 * backward_blocks<TY, NK>();
+    static constexpr int kForward = kWaves * 16 * forward_blocks<TY, NK>(), kDx = kWaves * 16 * dx_blocks<TY, NK>(),
+                         kDw = kWaves * 16 * dw_blocks<TY, NK>();
     static constexpr int kTile = Shape<TY, NK>::kRows;
 };
 
@@ -702,11 +705,12 @@ struct BackwardPlan {
 // DX: the rays are the own rows; else the labels
 template <class TY, int NK, bool DX> BackwardPlan backward_plan(const DstLabelParams *p, LabelArgs &a, char *base) {
     typedef Shapes<TY, NK> S;
-    constexpr int QB = backward_blocks<TY, NK>();
+    constexpr int QB = DX ? dx_blocks<TY, NK>() : dw_blocks<TY, NK>();
     const int64_t own = DX ? p->rays : p->labels, streamed = div_up(DX ? p->labels : p->rays, S::kTile);
     BackwardPlan b;
-    b.few = few_rows(div_up(own, S::kBackward), streamed);
-    a.own = b.few ? kWaves * 16 : S::kBackward;
+    constexpr int whole = DX ? S::kDx : S::kDw;
+    b.few = few_rows(div_up(own, whole), streamed);
+    a.own = b.few ? kWaves * 16 : whole;
     const void *kernel;
     if constexpr (DX) kernel = b.few ? (const void *)&k_label_dx<TY, NK, 1> : (const void *)&k_label_dx<TY, NK, QB>;
     else if (p->reduction == DST_REDUCE_NONE) kernel = b.few ? (const void *)&k_label_dw<TY, NK, 1, false> : (const void *)&k_label_dw<TY, NK, QB, false>;
@@ -813,7 +817,7 @@ int dst_label_loss_backward(const DstLabelParams *p, void *stream) {
     return with_gradients(p, [&](auto ty, auto nk) {
         typedef decltype(ty) TY;
         typedef typename TY::E E;
-        constexpr int NK = decltype(nk)::value, QB = backward_blocks<TY, NK>();
+        constexpr int NK = decltype(nk)::value, QB = dw_blocks<TY, NK>();
         const hipStream_t s = (hipStream_t)stream;
         bool copied = false;
         for (int pass = 0; pass < 2; ++pass) {
@@ -830,7 +834,7 @@ int dst_label_loss_backward(const DstLabelParams *p, void *stream) {
             if (!copied) prepare({&b.sets.x, &b.sets.w}, s);   // (both passes have the copies in the same place)
             copied = true;
             if (dx && b.few) k_label_dx<TY, NK, 1><<<grid, kThreads, 0, s>>>(a);
-            else if (dx) k_label_dx<TY, NK, QB><<<grid, kThreads, 0, s>>>(a);
+            else if (dx) k_label_dx<TY, NK, dx_blocks<TY, NK>()><<<grid, kThreads, 0, s>>>(a);
             else if (b.few && a.upstream_rows) k_label_dw<TY, NK, 1, false><<<grid, kThreads, 0, s>>>(a);
             else if (b.few) k_label_dw<TY, NK, 1, true><<<grid, kThreads, 0, s>>>(a);
             else if (a.upstream_rows) k_label_dw<TY, NK, QB, false><<<grid, kThreads, 0, s>>>(a);
