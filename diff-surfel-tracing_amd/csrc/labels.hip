@@ -57,6 +57,11 @@ template <class TY, int NK> constexpr int forward_blocks() { return NK <= 1 ? 4 
 template <class TY, int NK> constexpr int dx_blocks() { return NK <= 1 ? (TY::kDepth == 32 ? 2 : 4) : NK * TY::kPlanes <= 8 ? 2 : 1; }
 template <class TY, int NK> constexpr int dw_blocks() { return NK <= 1 ? (TY::kDepth == 32 ? 2 : 4) : NK * TY::kPlanes <= 6 ? 2 : 1; }
 
+// Whether a block's products go before the other waves' instructions, in the forward kernels and in that of dx (32768 rays x 32771 labels of 256
+// channels in 16 bits: forward 692 us, 573 with it, dx 1094 and 1057; best label of 65,536 rays among 4096, eight channels in 32 bits:
+// 137 us and 128). Short rows of 16 bits, planes, dw and the attention gain nothing by it, or lose.
+template <class TY, int NK> constexpr bool goes_first() { return TY::kPlanes == 1 && (!TY::kRounds || NK >= 4); }
+
 // The one value that the rays share
 __device__ inline float upstream_value(const LabelArgs &a) { return a.upstream[0] * a.inverse[0]; }
 // The upstream gradient of a ray's loss: 0 where it is ignored, NaN where its label is none.
@@ -173,7 +178,7 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
                 const f4 b = *reinterpret_cast<const f4 *>(tile_bias + (pair + j) * 16 + 4 * g);
 #pragma unroll
                 for (int q = 0; q < QB; ++q) s[j][q] = b;
-                product<TY, NK, QB>(tile, pair + j, own, s[j]);
+                product<TY, NK, QB, false, goes_first<TY, NK>()>(tile, pair + j, own, s[j]);
             }
 #pragma unroll
             for (int q = 0; q < QB; ++q) {
@@ -444,7 +449,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads, TY::k
                 const f4 b = *reinterpret_cast<const f4 *>(tile_bias + (pair + j) * 16 + 4 * g);
 #pragma unroll
                 for (int q = 0; q < QB; ++q) p[j][q] = b;
-                product<TY, NK, QB>(tile, pair + j, own, p[j]);
+                product<TY, NK, QB, false, goes_first<TY, NK>()>(tile, pair + j, own, p[j]);
 #pragma unroll
                 for (int q = 0; q < QB; ++q)
 #pragma unroll
