@@ -310,7 +310,7 @@ __global__ __launch_bounds__(kThreads) void k_label_mean(const double *sums, con
     }
     if (threadIdx.x == 0) {
         *loss = (float)(mean ? s[0] / (double)c[0] : s[0]);
-        *inverse = mean ? (float)(1.0 / (double)c[0]) : 1.0f;
+        *inverse = !mean ? 1.0f : c[0] != 0 ? (float)(1.0 / (double)c[0]) : 0.0f;   // (of nothing: a loss of NaN, and no gradient)
     }
 }
 

@@ -299,3 +299,10 @@ def test_second_derivatives_are_refused():
     g, = torch.autograd.grad(dst.label_loss(x, w, t, b, reduction="sum"), x, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("channels,dtype", [(8, torch.float32), (64, torch.float32), (64, torch.bfloat16), (64, torch.float16)])
+def test_the_mean_of_nothing_has_no_gradient(channels, dtype):
+    x, w, b, t, _ = _inputs(70, channels, 90, dtype)
+    out = _grads(x, w, torch.full_like(t, -100), b, torch.tensor(1.0, device="cuda"))
+    assert torch.isnan(out[0]) and all((o == 0).all() for o in out[1:])
