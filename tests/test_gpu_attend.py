@@ -9,7 +9,8 @@ pytestmark = pytest.mark.gpu
 #        B, Lq, Lk, H, Hkv, D, Dv
 SIZES = [(1, 1, 1, 1, 1, 8, 8), (1, 1, 5000, 8, 8, 128, 128), (2, 3, 700, 4, 2, 64, 64), (1, 65, 63, 1, 1, 16, 16),
          (3, 17, 130, 6, 2, 40, 24), (1, 300, 33, 2, 2, 32, 32), (1, 130, 257, 2, 1, 256, 256), (2, 70, 64, 1, 1, 100, 7),
-         (1, 2, 65, 3, 1, 1, 1), (1, 1000, 20, 1, 1, 3, 5), (1, 40, 2100, 2, 2, 96, 128)]
+         (1, 2, 65, 3, 1, 1, 1), (1, 9, 70, 16, 1, 32, 32), (1, 5, 40, 32, 1, 130, 64), (2, 21, 90, 8, 2, 8, 4), (1, 600, 600, 1, 1, 16, 8),
+        (1, 1000, 20, 1, 1, 3, 5), (1, 40, 2100, 2, 2, 96, 128)]
 
 
 def _inputs(B, Lq, Lk, H, Hkv, D, Dv, dtype, seed=0):
@@ -228,3 +229,32 @@ def test_a_row_far_into_a_large_memory():
     q, kk, vv, _ = _inputs(2, 9, 100, 1, 1, 64, 64, torch.bfloat16)
     k.copy_(kk), v.copy_(vv)
     R.check(dst.attend_memory(q, k, v), R.attend(q, kk, vv)["out"], "out")
+
+
+def test_rows_far_apart_in_memory():
+    import diff_surfel_tracing as dst
+    pitch = 2 ** 24
+    big = torch.empty(100 * pitch + 2 ** 20, dtype=torch.bfloat16, device="cuda")
+    q, kk, vv, up = _inputs(1, 9, 100, 2, 2, 64, 64, torch.bfloat16)
+    k = big.as_strided((1, 100, 2, 64), (0, pitch, 2 ** 12, 1))
+    v = big.as_strided((1, 100, 2, 64), (0, pitch, 2 ** 12, 1), 2 ** 10)
+    k.copy_(kk), v.copy_(vv)
+    for a, b in zip(_grads(q, k, v, up), _grads(q, kk, vv, up)):
+        assert torch.equal(a, b)
+
+
+def test_many_own_tiles_and_a_rest_that_is_cut():
+    """512 own tiles of 128 rows, two rounds or one of the device's places, and one more, against enough rows that cutting it pays: queries for
+    the forward kernel and that of dq, memory for that of dk and dv."""
+    for size in ((1, 128 * 513, 1500, 1, 1, 64, 64), (1, 1500, 128 * 513, 1, 1, 64, 64)):
+        q, k, v, up = _inputs(*size, torch.bfloat16)
+        _check(_grads(q, k, v, up), R.attend(q, k, v, up=up))
+
+
+def test_a_graph_walked_twice():
+    import diff_surfel_tracing as dst
+    q, k, v, up = (t.requires_grad_(True) for t in _inputs(1, 70, 90, 2, 1, 40, 40, torch.bfloat16))
+    out = dst.attend_memory(q, k, v)
+    first = torch.autograd.grad(out, [q, k, v], up.detach(), retain_graph=True)
+    second = torch.autograd.grad(out, [q, k, v], up.detach())
+    assert all(torch.equal(a, b) for a, b in zip(first, second))

@@ -306,3 +306,45 @@ def test_the_mean_of_nothing_has_no_gradient(channels, dtype):
     x, w, b, t, _ = _inputs(70, channels, 90, dtype)
     out = _grads(x, w, torch.full_like(t, -100), b, torch.tensor(1.0, device="cuda"))
     assert torch.isnan(out[0]) and all((o == 0).all() for o in out[1:])
+
+
+def test_a_graph_walked_twice():
+    import diff_surfel_tracing as dst
+    x, w, b, t, up = _inputs(300, 40, 70, torch.float32)
+    leaves = [v.requires_grad_(True) for v in (x, w, b)]
+    out = dst.label_loss(x, w, t, b, reduction="none")
+    first = torch.autograd.grad(out, leaves, up, retain_graph=True)
+    second = torch.autograd.grad(out, leaves, up)
+    assert all(torch.equal(a, c) for a, c in zip(first, second))
+    t[0] = 3   # what the backward pass would need is no longer what the forward pass saw
+    out = dst.label_loss(x, w, t, b, reduction="none")
+    t[1] = 4
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out, leaves, up)
+
+
+def test_many_own_tiles_and_a_rest_that_is_cut():
+    """512 own tiles, two rounds or one of the device's places, and two more: whole tiles and cut ones in one launch. Rays for the forward
+    kernel, the best label's and that of dx (128 rows a tile), labels for that of dw (64)."""
+    import diff_surfel_tracing as dst
+    for N, V in ((128 * 513 + 5, 700), (700, 64 * 513 + 3)):
+        x, w, b, t, up = _inputs(N, 129, V, torch.bfloat16)
+        got, ref = _grads(x, w, t, b, up, reduction="none"), R.labels(x, w, t, b, up)
+        for v, name in zip(got, ("loss", "dx", "dw", "db")):
+            R.check(v, ref[name], name)
+        label, _ = dst.label_rays(x, w, b)
+        s = x.double() @ w.double().T + b.double()
+        assert torch.equal(label, torch.where(s == s.amax(1, keepdim=True), torch.arange(V, device="cuda"), V).amin(1))
+
+
+def test_a_table_and_rays_far_apart_in_memory():
+    import diff_surfel_tracing as dst
+    x, w, b, t, up = _inputs(300, 24, 90, torch.float32)
+    want = _grads(x, w, t, b, up, reduction="none")
+    for pitch in (2 ** 23, 2 ** 23 + 1):    # 257 rows of them are more than 2^31 bytes: read from copies
+        big = torch.empty(300 * pitch, dtype=torch.float32, device="cuda")
+        far_x, far_w = big.as_strided((300, 24), (pitch, 1)), big.as_strided((90, 24), (pitch, 1), 1000)
+        far_x.copy_(x), far_w.copy_(w)
+        for p, q in zip(want, _grads(far_x, far_w, t, b, up, reduction="none")):
+            assert torch.equal(p, q)
+        del big, far_x, far_w
