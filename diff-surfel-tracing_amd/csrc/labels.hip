@@ -6,8 +6,8 @@
 // The (rays, labels) matrix is never stored: the forward kernel goes over the table in tiles and keeps a running maximum
 // and sum for every ray; each of the two backward kernels forms the tiles again from the saved lse, one with the rays
 // as own rows (dx), one with the labels (dw, db). Every sum has one owner and one order: no atomics, the same bits every
-// time. Where the own rows are too few to fill the device, the streamed rows are split over workgroups, and a closing kernel
-// adds the parts.
+// time. Own tiles that do not fill the device's last round, or are too few to fill it at all, are cut into parts of the streamed
+// rows, which a closing kernel adds.
 #include <type_traits>
 
 #include "operators.h"
@@ -131,6 +131,11 @@ __device__ inline void merge_best(float &best, int &label, float &second, float 
 }
 
 // Rays as own rows, the table streamed. BEST: the best label instead of the loss.
+// A lane keeps the maximum and sum of its own quarter of the table (its group's rows of every block), so nothing is exchanged until the
+// end. Short rows are bound by the vector unit, not by the products: fused multiply-add, exponential, half a maximum and an
+// addition for a logit, and four instructions more for the best label (full-HD, 8 channels, 151 labels: 150 us, vector
+// instructions 82 % of the cycles). Long ones by vector and matrix instructions, 50 % and 47 % of the cycles, which overlap in part (32768 rays x
+// 32771 labels of 256 channels, bf16: 560 us, 981 TFLOP/s, of the 1119 that a large library product reaches).
 template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThreads) void k_label_forward(LabelArgs a) {
     typedef Shape<TY, NK> T;
     __shared__ alignas(16) char tile[T::kTile > kThreads * 12 ? T::kTile : kThreads * 12];
@@ -400,7 +405,9 @@ template <class TY> __global__ __launch_bounds__(kThreads) void k_label_near(Lab
     }
 }
 // ---- backward -------------------------------------------------------------------------------------------------------
-// dx: rays as own rows, the table streamed.
+// dx: rays as own rows, the table streamed; the tile is read twice from LDS, by rows for the logits and turned for the sums.
+// 921,600 rays x 256 labels of 8 channels: 111 us, vector instructions 81 % of the cycles; 131,072 x 4096 of 64 channels
+// in planes: 602 us, matrix instructions 71 %; 32768 x 32771 of 256 channels, bf16: 1027 us, 1070 TFLOP/s, matrix instructions 49 %.
 template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads, TY::kPlanes == 1 ? 2 : 1) void k_label_dx(LabelArgs a) {
     typedef Shape<TY, NK> T;
     constexpr int NM = depth_blocks<TY, NK>();
@@ -486,7 +493,9 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads, TY::k
     }
 }
 
-// dw and db: labels as own rows, the rays streamed.
+// dw and db: labels as own rows, the rays streamed, with their lse, upstream gradient and label in LDS. Few labels are cut into as many
+// parts of the rays as fill the device. 921,600 rays x 256 labels of 8 channels: 126 us, vector instructions 80 % of the cycles; 131,072 x
+// 4096 of 64 channels in planes: 717 us, matrix instructions 58 %; 32768 x 32771 of 256 channels, bf16: 1408 us, 781 TFLOP/s, LDS reads 51 %.
 // ONE: the rays share one upstream gradient, which multiplies the sums at the end; else each ray's weights have its own.
 template <class TY, int NK, int QB, bool ONE> __global__ __launch_bounds__(kThreads) void k_label_dw(LabelArgs a) {
     typedef Shape<TY, NK> T;
