@@ -31,7 +31,8 @@ struct LabelArgs {
     double *sums;                   // (blocks): sums of losses ...
     uint32_t *counts;               // ... and rays counted in them
     // the best label
-    const float *bounds;            // (kBoundBlocks, 2): largest row norm of the table, largest |bias|
+    const float *bounds;            // (kBoundBlocks, 3): largest row norm of the table, |bias| and bias
+    float margin;                   // what a logit may be off by, of the norms and the |bias|
     int4 *best;                     // of a part's rays: bits of the best logit, its label, bits of the second best, -
     int64_t *label;                 // (rays)
     float *log_prob;                // (rays)
@@ -100,12 +101,19 @@ __device__ inline void block_sums(const LabelArgs &a, int at, double sum, uint32
     if (threadIdx.x == 0) a.sums[at] = s[0], a.counts[at] = c[0];
 }
 
-// The best label of a ray, or a place on the list of those that 32 bits cannot decide: a logit of d products is off by less
-// than (d + 16) 2^-22 times the norms (the tile product rounds at most once a product and once a block), twice that between
-// two; a ray without channels has none.
-__device__ inline void finish_best(const LabelArgs &a, int64_t row, Running r, float best, int label, float second, float norm, float2 bound) {
-    const float wide = bound.x, tall = bound.y;
-    const float off = norm > 0.0f ? 2.3841858e-7f * ((float)(a.d + 16) * norm * wide + 2.0f * tall) : 0.0f;
+// A norm is at least what its squares' sum says, and more by what squares below 2^-126 lost: sqrt(256) 2^-63 at most.
+constexpr float kNormLost = 2e-18f;
+
+// The best label of a ray, or a place on the list of those that 32 bits cannot decide. A logit starts as its label's bias and takes d
+// products (six a channel, in planes); the tile product rounds at most once a product and once a block, each time by at most 2^-23 of the
+// norms and the |bias|: it is off by less than (d + 16) 2^-22 of them, (3 d + 32) 2^-22 in planes (and by products too small for 32
+// bits), twice that between two. A ray without channels (norm 0)
+// has the biases themselves. Of the biases those count that can be the best label's: one more than 2 norms below the largest cannot, so a
+// label that is masked by the lowest value of its type does not bring every ray onto the list. (Full-HD rays, 8 channels, 151 labels, a third
+// of them so masked: 3767 us with all biases counted, 173 with these.)
+__device__ inline void finish_best(const LabelArgs &a, int64_t row, Running r, float best, int label, float second, float norm, float3 bound) {
+    const float reach = norm * bound.x, tall = fminf(bound.y, __builtin_fabsf(bound.z) + 2.1f * reach);
+    const float off = norm > 0.0f ? a.margin * (reach + tall) + 1e-35f : 0.0f;
     a.label[row] = label == 0x7fffffff ? 0 : label;
     a.log_prob[row] = -log2_of(r.l) * kLn2;
     if (best - second < 2.0f * off) {
@@ -114,10 +122,12 @@ __device__ inline void finish_best(const LabelArgs &a, int64_t row, Running r, f
         a.near_floor[i] = best - 3.0f * off;   // (the best label's logit is best - off at least, and another sum of it off by as much)
     }
 }
-// The largest norm and |bias| over the blocks that looked for them: every lane of a wave takes one.
-__device__ inline float2 table_bound(const LabelArgs &a) {
-    float2 b = reinterpret_cast<const float2 *>(a.bounds)[threadIdx.x & 63];
-    for (int step = 32; step > 0; step >>= 1) b.x = fmaxf(b.x, __shfl_xor(b.x, step)), b.y = fmaxf(b.y, __shfl_xor(b.y, step));
+// The largest norm, |bias| and bias over the blocks that looked for them: every lane of a wave takes one.
+__device__ inline float3 table_bound(const LabelArgs &a) {
+    const float *from = a.bounds + 3 * (threadIdx.x & 63);
+    float3 b = {from[0], from[1], from[2]};
+    for (int step = 32; step > 0; step >>= 1)
+        b.x = fmaxf(b.x, __shfl_xor(b.x, step)), b.y = fmaxf(b.y, __shfl_xor(b.y, step)), b.z = fmaxf(b.z, __shfl_xor(b.z, step));
     return b;
 }
 static_assert(kBoundBlocks == 64, "a lane each");
@@ -222,7 +232,7 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
 
     double sum = 0.0;
     uint32_t count = 0;
-    float2 bound = {0.0f, 0.0f};
+    float3 bound = {0.0f, 0.0f, 0.0f};
     if constexpr (BEST) bound = table_bound(a);
 #pragma unroll
     for (int q = 0; q < QB; ++q) {
@@ -230,9 +240,19 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
         const Running r = merge_group(run[q]);
         if constexpr (BEST) {
             float norm = 0.0f;
+            uint32_t any = 0u;   // of the bits but the signs
 #pragma unroll
-            for (int k = 0; k < fragments<NK>(); ++k) norm += fragment_dot<TY>(own.f[q][k], own.f[q][k]);
+            for (int k = 0; k < fragments<NK>(); ++k) {
+                norm += fragment_dot<TY>(own.f[q][k], own.f[q][k]);
+#pragma unroll
+                for (int p = 0; p < TY::kPlanes; ++p) {
+                    const u4 w = own.f[q][k].w[p] & (TY::kDepth == 16 ? 0x7fffffffu : 0x7fff7fffu);
+                    any |= (w[0] | w[1]) | (w[2] | w[3]);
+                }
+            }
+            any |= __shfl_xor(any, 16), any |= __shfl_xor(any, 32);
             norm = sqrtf(sum_group(norm));
+            norm = any ? norm + kNormLost : 0.0f;
 #pragma unroll
             for (int step = 16; step <= 32; step <<= 1)
                 merge_best(best[q], label[q], second[q], __shfl_xor(best[q], step), __shfl_xor(label[q], step), __shfl_xor(second[q], step));
@@ -278,7 +298,7 @@ template <bool BEST> __global__ __launch_bounds__(kThreads) void k_label_join(La
     const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x, row = (int64_t)a.cut.whole * a.own + i;
     double sum = 0.0;
     uint32_t count = 0;
-    float2 bound = {0.0f, 0.0f};
+    float3 bound = {0.0f, 0.0f, 0.0f};
     if constexpr (BEST) bound = table_bound(a);
     if (row < a.rays) {
         Running r = {-kInf, 0.0f};
@@ -320,11 +340,11 @@ __global__ __launch_bounds__(kThreads) void k_label_mean(const double *sums, con
 }
 
 // ---- the best label where 32 bits do not decide ---------------------------------------------------------------------
-// Largest norm of a row of the table and largest |bias|, for every block; empties the list of near rays.
+// Largest norm of a row of the table, largest |bias| and bias, for every block; empties the list of near rays.
 template <class TY> __global__ __launch_bounds__(kThreads) void k_label_bounds(LabelArgs a, float *bounds) {
-    __shared__ float s[2 * kThreads];
+    __shared__ float s[3 * kThreads];
     const int lane = threadIdx.x & 63;
-    float wide = 0.0f, tall = 0.0f;
+    float wide = 0.0f, tall = 0.0f, most = a.bias ? -kInf : 0.0f;
     for (int64_t v = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6); v < a.labels; v += (int64_t)kBoundBlocks * kWaves) {
         float n = 0.0f;
         for (int k = lane; k < a.w.words; k += 64) {
@@ -337,18 +357,20 @@ template <class TY> __global__ __launch_bounds__(kThreads) void k_label_bounds(L
         if (a.bias) {   // (a label switched off by an infinite bias bounds nothing)
             const float b = __builtin_fabsf(a.bias[v]);
             tall = fmaxf(tall, b == kInf ? 0.0f : b);
+            most = fmaxf(most, b == kInf ? -kInf : a.bias[v]);
         }
     }
-    s[threadIdx.x] = wide, s[kThreads + threadIdx.x] = tall;
+    s[threadIdx.x] = wide, s[kThreads + threadIdx.x] = tall, s[2 * kThreads + threadIdx.x] = most;
     for (int step = kThreads / 2; step > 0; step >>= 1) {
         __syncthreads();
         if ((int)threadIdx.x < step) {
             s[threadIdx.x] = fmaxf(s[threadIdx.x], s[threadIdx.x + step]);
             s[kThreads + threadIdx.x] = fmaxf(s[kThreads + threadIdx.x], s[kThreads + threadIdx.x + step]);
+            s[2 * kThreads + threadIdx.x] = fmaxf(s[2 * kThreads + threadIdx.x], s[2 * kThreads + threadIdx.x + step]);
         }
     }
     if (threadIdx.x == 0) {
-        bounds[2 * blockIdx.x] = sqrtf(s[0]) * 1.0001f, bounds[2 * blockIdx.x + 1] = s[kThreads];
+        bounds[3 * blockIdx.x] = sqrtf(s[0]) * 1.0001f + kNormLost, bounds[3 * blockIdx.x + 1] = s[kThreads], bounds[3 * blockIdx.x + 2] = s[2 * kThreads];
         if (blockIdx.x == 0) *a.near_count = 0u;
     }
 }
@@ -699,7 +721,8 @@ template <class TY, int NK, bool BEST> ForwardPlan forward_plan(const DstLabelPa
         else a.target_logit = c.take<float>(rest);
     }
     if (BEST) {
-        a.bounds = c.take<float>(2 * kBoundBlocks);
+        a.margin = 2.3841858e-7f * (float)(TY::kPlanes == 3 ? 3 * p->channels + 32 : p->channels + 16);
+        a.bounds = c.take<float>(3 * kBoundBlocks);
         a.near_count = c.take<uint32_t>(1);
         a.near_list = c.take<uint32_t>(p->rays);
         a.near_floor = c.take<float>(p->rays);

@@ -348,3 +348,61 @@ def test_a_table_and_rays_far_apart_in_memory():
         for p, q in zip(want, _grads(far_x, far_w, t, b, up, reduction="none")):
             assert torch.equal(p, q)
         del big, far_x, far_w
+
+
+def _best(x, w, b):
+    s = x.double() @ w.double().T + (0.0 if b is None else b.double())
+    return torch.where(s == s.amax(1, keepdim=True), torch.arange(len(w), device="cuda"), len(w)).amin(1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("channels", [8, 16, 64, 256])
+def test_best_label_under_a_large_bias(channels, dtype):
+    """Products that a bias of 4096 (values apart by 2^-11) rounds away, or up to a whole step, at every addition."""
+    import diff_surfel_tracing as dst
+    step = 2.0 ** -11
+    w = torch.zeros(4, channels, device="cuda")
+    w[0], w[1, :-1] = 0.49 * step, 0.51 * step       # (as each product is added by itself)
+    w[2, ::4], w[3, :-4:4] = 0.49 * step, 0.51 * step   # (as four are)
+    w = w.to(dtype)
+    b = torch.full((4,), 4096.0, device="cuda")
+    x = torch.ones(70, channels, device="cuda").to(dtype)
+    for rows in ([0, 1], [1, 0], [2, 3], [3, 2], [0, 1, 2, 3]):
+        label, _ = dst.label_rays(x, w[rows], b[rows])
+        assert torch.equal(label, _best(x, w[rows], b[rows]))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("channels", [8, 40])
+def test_best_label_of_channels_whose_squares_vanish(channels, dtype):
+    """A ray of 1e-24, whose square is 0 in 32 bits, against rows apart by their last bit."""
+    import diff_surfel_tracing as dst
+    x = torch.full((70, channels), 1e-24, device="cuda").to(dtype)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    w = (torch.rand(1, channels, generator=g, device="cuda") + 1.0).to(dtype).repeat(9, 1)
+    w[6, 3] += torch.finfo(dtype).eps
+    label, _ = dst.label_rays(x, w)
+    assert torch.equal(label, _best(x, w, None))
+    label, _ = dst.label_rays(x * 0, w)
+    assert (label == 0).all()
+
+
+@pytest.mark.parametrize("low", [float("-inf"), torch.finfo(torch.float32).min, -1e30])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_labels_masked_by_a_low_bias(low, dtype):
+    x, w, b, t, up = _inputs(900, 40, 130, dtype)
+    b[::3] = low
+    t = torch.where(t % 3 == 0, t + 1, t)
+    t[t >= 130] = 1
+    import diff_surfel_tracing as dst
+    label, logp = dst.label_rays(x, w, b)
+    assert torch.equal(label, _best(x, w, b)) and (label % 3 != 0).all() and torch.isfinite(logp).all()
+    there = torch.arange(130, device="cuda") % 3 != 0
+    at = torch.cumsum(there, 0) - 1
+    got = _grads(x, w, t, b, up, reduction="none")
+    ref = R.labels(x, w[there], torch.where(t < 0, t, at[t.clamp(min=0)]), b[there], up)
+    R.check(got[0], ref["loss"], "loss")
+    R.check(got[1], ref["dx"], "dx")
+    R.check(got[2][there], ref["dw"], "dw")
+    R.check(got[3][there], ref["db"], "db")
+    assert (got[2][~there] == 0).all() and (got[3][~there] == 0).all()
