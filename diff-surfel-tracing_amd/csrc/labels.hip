@@ -143,8 +143,8 @@ __device__ inline void merge_best(float &best, int &label, float &second, float 
 // Rays as own rows, the table streamed. BEST: the best label instead of the loss.
 // A lane keeps the maximum and sum of its own quarter of the table (its group's rows of every block), so nothing is exchanged until the
 // end. Short rows are bound by the vector unit, not by the products: fused multiply-add, exponential, half a maximum and an
-// addition for a logit, and four instructions more for the best label (full-HD, 8 channels, 151 labels: 150 us, vector
-// instructions 82 % of the cycles). Long ones by vector and matrix instructions, 50 % and 47 % of the cycles, which overlap in part (32768 rays x
+// addition for a logit, and four instructions more for the best label (full-HD, 8 channels, 151 labels: 155 us, vector
+// instructions 83 % of the cycles). Long ones by vector and matrix instructions, 50 % and 47 % of the cycles, which overlap in part (32768 rays x
 // 32771 labels of 256 channels, bf16: 560 us, 981 TFLOP/s, of the 1119 that a large library product reaches).
 template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThreads) void k_label_forward(LabelArgs a) {
     typedef Shape<TY, NK> T;

@@ -155,8 +155,9 @@ def label_loss(features, weight, targets, bias=None, *, ignore_index=-100, reduc
     both float32, bfloat16 or float16 (gradients in float16 are formed in 32 bits and rounded once); bias: (labels,), -inf switches a
     label off; targets: whole numbers of the leading dimensions of features.  `ignore_index` takes a ray out: no loss, no
     gradient, whatever its channels hold.  Any other target outside 0..labels-1 makes the loss and the gradients it
-    reaches NaN.  Returns float32: the mean over the rays not ignored (NaN if there are none), the sum, or with "none" a loss
-    for every ray.  Differentiable (once) in features, weight and bias; sums in 32 bits or more in one order: the same bits every time."""
+    reaches NaN.  Returns float32: the mean over the rays not ignored (NaN, without gradients, if there are none), the sum, or with "none" a loss
+    for every ray.  Differentiable (once) in features, weight and bias; sums in 32 bits or more in one order: the same bits every time.
+    Logits beyond 2.3e38 count as infinite."""
     _check_labels(features, weight, bias)
     if reduction not in _REDUCTIONS:
         raise RuntimeError("reduction must be one of none, sum, mean (got %r)" % (reduction,))
