@@ -11,10 +11,9 @@ from typing import NamedTuple
 
 import torch
 import torch.nn as nn
-from torch.autograd import forward_ad
 
 from . import _C
-from .features import attend_memory, label_loss, label_rays
+from .features import _transforms_active, attend_memory, label_loss, label_rays
 
 __all__ = ["SurfelTracer", "SurfelTracingSettings", "trace_surfels", "label_loss", "label_rays", "attend_memory"]
 
@@ -151,14 +150,6 @@ class _TraceSurfels(torch.autograd.Function):
         return (None, None, None, g_ray_o, g_ray_d, None, g_means3D, g_grads3D, like(g_shs, shs),
                 like(g_colors, colors_precomp), like(g_others, others_precomp), g_opacities, g_scales, g_rotations,
                 like(g_cov3Ds, cov3Ds_precomp), None)
-
-
-def _transforms_active():
-    """Whether more goes on than the call shows: inputs that may carry tangents of forward-mode differentiation or
-    functorch's levels (the autograd function refuses what it has no rule for), or a trace being recorded (the autograd
-    function is a node of it; its launches alone would leave only the empty output tensors there)."""
-    return (forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active()
-            or torch._C._get_tracing_state() is not None)
 
 
 def trace_surfels(optix_context, training, start_from_first, ray_o, ray_d, vertices, means3D, grads3D, shs,

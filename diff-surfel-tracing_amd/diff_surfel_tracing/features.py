@@ -9,6 +9,7 @@ which hands `out_aux` to its caller.
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _C
@@ -46,6 +47,14 @@ def _beside(t, first, name, dtype=None):
 
 def _wants_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _transforms_active():
+    """Whether more goes on than the call shows: inputs that may carry tangents of forward-mode differentiation or
+    functorch's levels (the autograd function refuses what it has no rule for), or a trace being recorded (the autograd
+    function is a node of it; its launches alone would leave only the empty output tensors there)."""
+    return (forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active()
+            or torch._C._get_tracing_state() is not None)
 
 
 class _on:
@@ -171,8 +180,26 @@ def label_loss(features, weight, targets, bias=None, *, ignore_index=-100, reduc
     x, w, t = _matrix(features, d), _matrix(weight, d), targets.reshape(-1).to(torch.int64).contiguous()
     b = None if bias is None else bias.to(torch.float32).contiguous()
     args = (x, w, t, b, ignore_index, _REDUCTIONS[reduction])
-    loss = _LabelLoss.apply(*args) if wants else _loss_forward(*args)[0]
+    loss = _LabelLoss.apply(*args) if wants or _transforms_active() else _loss_forward(*args)[0]
     return loss.reshape(shape) if reduction == "none" else loss
+
+
+def _best_forward(x, w, bias):
+    with _on(x):
+        p = _label_params(x, w, bias)
+        best = torch.empty(x.size(0), dtype=torch.int64, device=x.device)
+        log_prob = torch.empty(x.size(0), dtype=torch.float32, device=x.device)
+        p.best, p.log_prob = best.data_ptr(), log_prob.data_ptr()
+        _run_labels(p, _BEST, _C.load_library().dst_label_best, x)
+    return best, log_prob
+
+
+class _LabelRays(torch.autograd.Function):
+    """Only where a transform or a trace is under way; it has no rule for either derivative."""
+
+    @staticmethod
+    def forward(ctx, x, w, bias):
+        return _best_forward(x, w, bias)
 
 
 @torch.no_grad()
@@ -187,12 +214,7 @@ def label_rays(features, weight, bias=None):
     shape, d = features.shape[:-1], features.size(-1)
     x, w = _matrix(features, d), _matrix(weight, d)
     b = None if bias is None else bias.to(torch.float32).contiguous()
-    with _on(x):
-        p = _label_params(x, w, b)
-        best = torch.empty(x.size(0), dtype=torch.int64, device=x.device)
-        log_prob = torch.empty(x.size(0), dtype=torch.float32, device=x.device)
-        p.best, p.log_prob = best.data_ptr(), log_prob.data_ptr()
-        _run_labels(p, _BEST, _C.load_library().dst_label_best, x)
+    best, log_prob = _LabelRays.apply(x, w, b) if _transforms_active() else _best_forward(x, w, b)
     return best.reshape(shape), log_prob.reshape(shape)
 
 
@@ -298,4 +320,6 @@ def attend_memory(queries, keys, values, lengths=None, *, scale=None):
     scale = queries.size(3) ** -0.5 if scale is None else float(scale)
     wants = _wants_grad(queries, keys, values)
     q, k, v = _consecutive(queries), _consecutive(keys), _consecutive(values)
-    return _Attend.apply(q, k, v, lengths, scale) if wants else _attend_forward(q, k, v, lengths, scale, False)[0]
+    if wants or _transforms_active():
+        return _Attend.apply(q, k, v, lengths, scale)
+    return _attend_forward(q, k, v, lengths, scale, False)[0]
