@@ -317,7 +317,7 @@ def attend_memory(queries, keys, values, lengths=None, *, scale=None):
         if lengths.dtype != torch.int32:   # (clamped before 32 bits could wrap them)
             lengths = lengths.to(torch.int64).clamp(0, keys.size(1)).to(torch.int32)
         lengths = lengths.contiguous()
-    scale = queries.size(3) ** -0.5 if scale is None else float(scale)
+    scale = int(queries.size(3)) ** -0.5 if scale is None else float(scale)   # (a recorded trace gives sizes as tensors)
     wants = _wants_grad(queries, keys, values)
     q, k, v = _consecutive(queries), _consecutive(keys), _consecutive(values)
     if wants or _transforms_active():
