@@ -5,7 +5,8 @@
 //
 // The (rays, labels) matrix is never stored: the forward kernel goes over the table in tiles and keeps a running maximum
 // and sum for every ray; each of the two backward kernels forms the tiles again from the saved lse, one with the rays
-// as own rows (dx), one with the labels (dw, db). Every sum has one owner and one order: no atomics, the same bits every
+// as own rows (dx), one with the labels (dw, db). The weight of the label itself, less one, is not formed again: near a weight of 1 it
+// would be a difference of two rounded logits. The forward kernel leaves it, formed of the loss. Every sum has one owner and one order: no atomics, the same bits every
 // time. Own tiles that do not fill the device's last round, or are too few to fill it at all, are cut into parts of the streamed
 // rows, which a closing kernel adds.
 #include <type_traits>
@@ -27,6 +28,7 @@ struct LabelArgs {
     float2 *part;                   // of a part's rays: maximum and sum, in units of log 2
     float *target_logit;            // of the parted rays
     float *lse2;                    // (rays): log2 of the sum of exponentials; +inf where the ray is ignored
+    float *hit;                     // (rays): the weight of the ray's label less one, 0 where the ray is ignored; forward: or nullptr
     float *rows;                    // (rays) losses, or nullptr
     double *sums;                   // (blocks): sums of losses ...
     uint32_t *counts;               // ... and rays counted in them
@@ -73,15 +75,33 @@ __device__ inline float upstream_of(const LabelArgs &a, int64_t row, int64_t t) 
 }
 
 // ---- forward --------------------------------------------------------------------------------------------------------
+// What a logit lies below the logarithm of the sum, in units of log 2. The sum is 1 or more and relative to the maximum, and the logit is taken
+// relative to the maximum too, so of what both have in common nothing is rounded: a label with almost all of the weight keeps the digits of what it
+// lacks. (The maximum is a rounded product with log2 e; the sum's terms and the logit are both exact products less that number.)
+__device__ inline float below_sum(Running r, float logit) { return larger(log2_of(r.l) - __builtin_fmaf(logit, kLog2E, -r.m), 0.0f); }
+// Whether there is a logit above -inf and none is +inf.
+__device__ inline bool has_sum(Running r) { return r.l > 0.0f; }
+// The logit of each own row's own label, by the instructions that formed it among the others: the same bits.
+template <class TY, int NK> __device__ inline float logit_of(const Fragment<TY> (&own)[fragments<NK>()], const char *label_row, int words, float bias) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, l = lane & 15;
+    f4 s = {bias, bias, bias, bias};
+#pragma unroll
+    for (int k = 0; k < fragments<NK>(); ++k) s = fragment_product<TY, NK>(own_word<TY, NK>(label_row, k, words), own[k], s);
+    const float mine = (l & 2) ? ((l & 1) ? s[3] : s[2]) : ((l & 1) ? s[1] : s[0]);
+    return sum_group(g == (l >> 2) ? mine : 0.0f);   // (the diagonal's one value)
+}
+
 // A ray's loss from its maximum and sum; adds it to the thread's sums.
 __device__ inline void finish_row(const LabelArgs &a, int64_t row, Running r, float target_logit, double &sum, uint32_t &count) {
     const int64_t t = a.target[row];
     const bool ignored = t == a.ignore;
     const float lse2 = r.m + log2_of(r.l);
-    float loss = lse2 * kLn2 - target_logit;
-    if (t < 0 || t >= a.labels) loss = __builtin_nanf("");
+    float loss = below_sum(r, target_logit) * kLn2;
+    if (loss == kInf && target_logit > -kInf) loss = lse2 * kLn2 - target_logit;   // (its product with log2 e is beyond 32 bits)
+    if (!has_sum(r) || t < 0 || t >= a.labels) loss = __builtin_nanf("");
     if (ignored) loss = 0.0f;
     a.lse2[row] = ignored ? kInf : lse2;
+    if (a.hit) a.hit[row] = expm1f(-loss);
     if (a.rows) a.rows[row] = loss;
     sum += (double)loss;
     count += ignored ? 0u : 1u;
@@ -168,10 +188,11 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
     own.load(a.x, tile_base(a.x, row0), (int)min(a.rays - row0, (int64_t)(16 * QB)));
 
     Running run[QB];
+    float low[QB];   // what the running sum's additions added too much
     float best[QB], second[QB];
     int label[QB];
 #pragma unroll
-    for (int q = 0; q < QB; ++q) run[q] = Running{-kInf, 0.0f}, best[q] = second[q] = -kInf, label[q] = 0x7fffffff;
+    for (int q = 0; q < QB; ++q) run[q] = Running{-kInf, 0.0f}, low[q] = 0.0f, best[q] = second[q] = -kInf, label[q] = 0x7fffffff;
     rows_are_here(own);
     for (int at = first; at < last; at += T::kRows) {
         stage.store(tile);
@@ -220,7 +241,14 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
 #pragma unroll
                     for (int r = 0; r < 4; ++r) e[j][r] = exp2_of(__builtin_fmaf(s[j][q][r], kLog2E, -use));
                 const float sum = ((e[0][0] + e[0][1]) + (e[0][2] + e[0][3])) + ((e[1][0] + e[1][1]) + (e[1][2] + e[1][3]));
-                run[q].l = run[q].l * exp2_of(run[q].m - use) + sum;
+                const float by = exp2_of(run[q].m - use), l = run[q].l * by;
+                if constexpr (BEST) {
+                    run[q].l = l + sum;
+                } else {   // (a label near weight 1 would take a long tail's small terms in one by one, and lose them)
+                    const float more = sum - low[q] * by;
+                    run[q].l = l + more;
+                    low[q] = (run[q].l - l) - more;
+                }
                 run[q].m = top;
             }
         }
@@ -237,7 +265,7 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
 #pragma unroll
     for (int q = 0; q < QB; ++q) {
         const int64_t row = row0 + q * 16 + (lane & 15);
-        const Running r = merge_group(run[q]);
+        const Running r = merge_group(Running{run[q].m, run[q].l - low[q]});
         if constexpr (BEST) {
             float norm = 0.0f;
             uint32_t any = 0u;   // of the bits but the signs
@@ -267,16 +295,11 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
                 }
             }
         } else {
-            // the target's logit, from the own row in registers
             float logit = 0.0f;
             if (turn.split == 0) {
                 const int64_t t = row < a.rays ? a.target[row] : -1;
                 const bool there = t >= 0 && t < a.labels;
-#pragma unroll
-                for (int k = 0; k < fragments<NK>(); ++k)
-                    logit += fragment_dot<TY>(own.f[q][k], own_word<TY, NK>(there ? tile_base(a.w, t) : nullptr, k, a.w.words));
-                logit = sum_group(logit);
-                if (there && a.bias) logit += a.bias[t];
+                logit = logit_of<TY, NK>(own.f[q], there ? tile_base(a.w, t) : nullptr, a.w.words, there && a.bias ? a.bias[t] : 0.0f);
             }
             if (row < a.rays && g == 0) {
                 if (turn.part) {
@@ -301,19 +324,23 @@ template <bool BEST> __global__ __launch_bounds__(kThreads) void k_label_join(La
     float3 bound = {0.0f, 0.0f, 0.0f};
     if constexpr (BEST) bound = table_bound(a);
     if (row < a.rays) {
-        Running r = {-kInf, 0.0f};
+        float m = -kInf;
+        double l = 0.0;   // (hundreds of parts, of which one may have almost all of the sum)
         float best = -kInf, second = -kInf, norm = 0.0f;
         int label = 0x7fffffff;
         const int64_t from = i / a.own * a.cut.splits * a.own + i % a.own;
         for (int s = 0; s < a.cut.splits; ++s) {
             const float2 p = a.part[from + (int64_t)s * a.own];
-            r = merge(r, Running{p.x, p.y});
+            const float top = larger(m, p.x), use = finite_or_zero(top);
+            l = l * (double)exp2_of(m - use) + (double)p.y * (double)exp2_of(p.x - use);
+            m = top;
             if constexpr (BEST) {
                 const int4 b = a.best[from + (int64_t)s * a.own];
                 merge_best(best, label, second, __builtin_bit_cast(float, b.x), b.y, __builtin_bit_cast(float, b.z));
                 norm = __builtin_bit_cast(float, b.w);
             }
         }
+        const Running r = {m, (float)l};
         if constexpr (BEST) finish_best(a, row, r, best, label, second, norm, bound);
         else finish_row(a, row, r, a.target_logit[i], sum, count);
     }
@@ -451,7 +478,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads, TY::k
     fetch(first);
     Own<TY, NK, QB> own;
     own.load(a.x, tile_base(a.x, row0), (int)min(a.rays - row0, (int64_t)(16 * QB)));
-    float lse2[QB], up[QB];
+    float lse2[QB], up[QB], hit[QB];
     int label[QB];   // relative to the lane's first row of a tile
     f4 out[QB][NM];
 #pragma unroll
@@ -460,6 +487,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads, TY::k
         const int64_t t = row < a.rays ? a.target[row] : a.ignore;
         lse2[q] = row < a.rays ? a.lse2[row] : kInf;
         up[q] = row < a.rays ? upstream_of(a, row, t) : 0.0f;
+        hit[q] = row < a.rays ? a.hit[row] : 0.0f;
         label[q] = (t >= 0 && t < a.labels ? (int)t : -0x40000000) - 4 * g;
 #pragma unroll
         for (int m = 0; m < NM; ++m) out[q][m] = f4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -483,10 +511,8 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads, TY::k
                 for (int q = 0; q < QB; ++q)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        float e = exp2_of(__builtin_fmaf(p[j][q][r], kLog2E, -lse2[q]));
-                        // (of 32-bit rows the label's row is taken off the sum at the end; 16 bits would lose p - 1 where p is near 1)
-                        if constexpr (TY::kRounds) e -= label[q] - at == (pair + j) * 16 + r ? 1.0f : 0.0f;
-                        p[j][q][r] = e;
+                        const float e = exp2_of(__builtin_fmaf(p[j][q][r], kLog2E, -lse2[q]));
+                        p[j][q][r] = label[q] - at == (pair + j) * 16 + r ? hit[q] : e;
                     }
             }
             accumulate<TY, NK, QB, NM>(tile, pair, p[0], p[1], out);
@@ -500,13 +526,8 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads, TY::k
         const int64_t row = row0 + q * 16 + (lane & 15);
         whole_sums<TY>(out[q]);
         if (row >= a.rays) continue;
-        const int64_t t = a.target[row];
-        const bool label_here = !TY::kRounds && t >= first && t < last;   // (of a part: its labels' alone)
-        const char *label_row = tile_base(a.w, label_here ? t : 0);
 #pragma unroll
         for (int m = 0; m < NM; ++m) {
-            if constexpr (!TY::kRounds)
-                if (label_here) out[q][m] -= row_four<TY>(label_row, m * 16 + 4 * g, a.w.words);
             f4 v = out[q][m] * up[q];
             if (up[q] == 0.0f) v = f4{0.0f, 0.0f, 0.0f, 0.0f};   // (an ignored ray's channels may hold anything)
             if (turn.part) store_four(a.out_part + part_row(a.cut, turn, kWaves * 16 * QB, wave * 16 * QB + q * 16 + (lane & 15)) * a.d, m * 16 + 4 * g, a.d, v, four);
@@ -523,7 +544,7 @@ template <class TY, int NK, int QB, bool ONE> __global__ __launch_bounds__(kThre
     typedef Shape<TY, NK> T;
     constexpr int NM = depth_blocks<TY, NK>();
     __shared__ alignas(16) char tile[T::kTile];
-    __shared__ alignas(16) float tile_lse2[2][T::kRows], tile_up[2][T::kRows];
+    __shared__ alignas(16) float tile_lse2[2][T::kRows], tile_up[2][T::kRows], tile_hit[2][T::kRows];
     __shared__ alignas(16) int tile_label[2][T::kRows];
     const int lane = threadIdx.x & 63, g = lane >> 4, wave = wave_number();
     const Turn turn = turn_of(a.cut);
@@ -533,15 +554,15 @@ template <class TY, int NK, int QB, bool ONE> __global__ __launch_bounds__(kThre
 
     Stage<TY, NK> stage;
     stage.begin(a.x, tile_base(a.x, first));
-    // Of every ray: lse (+inf where it is ignored or behind the end, which makes its weights 0), upstream gradient, label. They are a tile
+    // Of every ray: lse (+inf where it is ignored or behind the end, which makes its weights 0), upstream gradient, label and its weight. They are a tile
     // ahead of the channels, which are read only of rays that are not ignored: those of the others may hold anything.
-    float stage_lse2 = kInf, stage_up = 0.0f;
+    float stage_lse2 = kInf, stage_up = 0.0f, stage_hit = 0.0f;
     int64_t stage_target = a.ignore;
     auto fetch_stats = [&](int64_t at) {   // (as they lie: what is made of them waits for them)
         const int64_t row = at + threadIdx.x;
         stage_target = a.ignore, stage_lse2 = kInf;
         if ((int)threadIdx.x < T::kRows && row < last) {
-            stage_target = a.target[row], stage_lse2 = a.lse2[row];
+            stage_target = a.target[row], stage_lse2 = a.lse2[row], stage_hit = a.hit[row];
             if (!ONE) stage_up = a.upstream[row];
         }
     };
@@ -550,6 +571,7 @@ template <class TY, int NK, int QB, bool ONE> __global__ __launch_bounds__(kThre
         const bool ignored = stage_target == a.ignore, none = !ignored && (stage_target < 0 || stage_target >= a.labels);
         tile_lse2[at][threadIdx.x] = none ? __builtin_nanf("") : stage_lse2;
         tile_label[at][threadIdx.x] = ignored || none ? -1 : (int)stage_target;
+        tile_hit[at][threadIdx.x] = stage_hit;
         if (!ONE) tile_up[at][threadIdx.x] = ignored ? 0.0f : stage_up;
     };
     auto fetch = [&](int64_t at, int half) {
@@ -593,6 +615,7 @@ template <class TY, int NK, int QB, bool ONE> __global__ __launch_bounds__(kThre
                 const int at4 = (pair + j) * 16 + 4 * g;
                 const f4 lse2 = *reinterpret_cast<const f4 *>(tile_lse2[half] + at4);
                 const f4 up = ONE ? f4{} : *reinterpret_cast<const f4 *>(tile_up[half] + at4);
+                const f4 hit = *reinterpret_cast<const f4 *>(tile_hit[half] + at4);
                 const int4 label = *reinterpret_cast<const int4 *>(tile_label[half] + at4);
                 const int labels[4] = {label.x, label.y, label.z, label.w};
 #pragma unroll
@@ -601,7 +624,7 @@ template <class TY, int NK, int QB, bool ONE> __global__ __launch_bounds__(kThre
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         float e = exp2_of(__builtin_fmaf(p[j][q][r], kLog2E, -lse2[r]));
-                        e -= labels[r] == v ? 1.0f : 0.0f;
+                        e = labels[r] == v ? hit[r] : e;
                         if constexpr (!ONE) e *= up[r];
                         p[j][q][r] = e;
                     }
@@ -660,7 +683,7 @@ LabelArgs arguments(const DstLabelParams *p) {
     LabelArgs a = {};
     a.bias = p->bias, a.target = p->targets;
     a.rays = p->rays, a.ignore = p->ignore_index, a.d = p->channels, a.labels = p->labels;
-    a.lse2 = p->lse;
+    a.lse2 = p->lse, a.hit = p->hit;
     return a;
 }
 
@@ -851,6 +874,7 @@ int dst_label_loss_backward(const DstLabelParams *p, void *stream) {
     if (p->reduction != DST_REDUCE_NONE && !p->inverse) return dst_op_fail(DST_E_INVALID, "a reduced loss needs inverse");
     if ((reinterpret_cast<uintptr_t>(p->grad_features) | reinterpret_cast<uintptr_t>(p->grad_weight)) & 15u)
         return dst_op_fail(DST_E_INVALID, "gradients must be aligned to 16 bytes");
+    if (p->rays > 0 && !p->hit) return dst_op_fail(DST_E_INVALID, "hit is required");
     return with_gradients(p, [&](auto ty, auto nk) {
         typedef decltype(ty) TY;
         typedef typename TY::E E;

@@ -103,35 +103,42 @@ def _run_labels(p, what, launch, like):
         _fail(rc)
 
 
+def _set_stats(p, stats):
+    """What the forward pass leaves of every ray for the backward pass: `lse` and `hit`."""
+    p.lse, p.hit = stats.data_ptr(), stats.data_ptr() + 4 * int(stats.size(1))   # (a recorded trace gives sizes as tensors)
+
+
 def _loss_forward(x, w, targets, bias, ignore_index, reduction):
     with _on(x):
         p = _label_params(x, w, bias)
         p.reduction, p.targets, p.ignore_index = reduction, targets.data_ptr(), ignore_index
         f32 = dict(dtype=torch.float32, device=x.device)
         loss = torch.empty(x.size(0) if reduction == 0 else (), **f32)
-        lse = torch.empty(x.size(0), **f32)
+        stats = torch.empty(2, x.size(0), **f32)
         inverse = None if reduction == 0 else torch.empty((), **f32)
-        p.loss, p.lse, p.inverse = loss.data_ptr(), lse.data_ptr(), None if inverse is None else inverse.data_ptr()
+        p.loss, p.inverse = loss.data_ptr(), None if inverse is None else inverse.data_ptr()
+        _set_stats(p, stats)
         _run_labels(p, _FORWARD, _C.load_library().dst_label_loss_forward, x)
-    return loss, lse, inverse
+    return loss, stats, inverse
 
 
 class _LabelLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, targets, bias, ignore_index, reduction):
-        loss, lse, inverse = _loss_forward(x, w, targets, bias, ignore_index, reduction)
-        ctx.save_for_backward(x, w, targets, bias, lse, inverse)
+        loss, stats, inverse = _loss_forward(x, w, targets, bias, ignore_index, reduction)
+        ctx.save_for_backward(x, w, targets, bias, stats, inverse)
         ctx.ignore_index, ctx.reduction = ignore_index, reduction
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, upstream):
-        x, w, targets, bias, lse, inverse = ctx.saved_tensors
+        x, w, targets, bias, stats, inverse = ctx.saved_tensors
         with _on(x):
             p = _label_params(x, w, bias)
             p.reduction, p.targets, p.ignore_index = ctx.reduction, targets.data_ptr(), ctx.ignore_index
-            p.lse, p.inverse = lse.data_ptr(), None if inverse is None else inverse.data_ptr()
+            p.inverse = None if inverse is None else inverse.data_ptr()
+            _set_stats(p, stats)
             upstream = upstream.contiguous()
             p.upstream = upstream.data_ptr()
             want_x, want_w, _, want_bias = ctx.needs_input_grad[:4]
