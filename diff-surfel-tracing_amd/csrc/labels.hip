@@ -77,8 +77,12 @@ __device__ inline float upstream_of(const LabelArgs &a, int64_t row, int64_t t) 
 // ---- forward --------------------------------------------------------------------------------------------------------
 // What a logit lies below the logarithm of the sum, in units of log 2. The sum is 1 or more and relative to the maximum, and the logit is taken
 // relative to the maximum too, so of what both have in common nothing is rounded: a label with almost all of the weight keeps the digits of what it
-// lacks. (The maximum is a rounded product with log2 e; the sum's terms and the logit are both exact products less that number.)
-__device__ inline float below_sum(Running r, float logit) { return larger(log2_of(r.l) - __builtin_fmaf(logit, kLog2E, -r.m), 0.0f); }
+// lacks. (The maximum is a rounded product with log2 e; the sum's terms and the logit are both exact products less that number. A term near 1
+// is taken as the sum has it, rounded: a label alone lacks nothing.)
+__device__ inline float below_sum(Running r, float logit) {
+    const float at = __builtin_fmaf(logit, kLog2E, -r.m);
+    return larger(log2_of(r.l) - (at > -1.0f ? log2_of(exp2_of(at)) : at), 0.0f);
+}
 // Whether there is a logit above -inf and none is +inf.
 __device__ inline bool has_sum(Running r) { return r.l > 0.0f; }
 // The logit of each own row's own label, by the instructions that formed it among the others: the same bits.
@@ -135,7 +139,7 @@ __device__ inline void finish_best(const LabelArgs &a, int64_t row, Running r, f
     const float reach = norm * bound.x, tall = fminf(bound.y, __builtin_fabsf(bound.z) + 2.1f * reach);
     const float off = norm > 0.0f ? a.margin * (reach + tall) + 1e-35f : 0.0f;
     a.label[row] = label == 0x7fffffff ? 0 : label;
-    a.log_prob[row] = -log2_of(r.l) * kLn2;
+    a.log_prob[row] = has_sum(r) ? -below_sum(r, best) * kLn2 : __builtin_nanf("");   // (no label left: there is no probability)
     if (best - second < 2.0f * off) {
         const uint32_t i = atomicAdd(a.near_count, 1u);
         a.near_list[i] = (uint32_t)row;
@@ -242,13 +246,10 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
                     for (int r = 0; r < 4; ++r) e[j][r] = exp2_of(__builtin_fmaf(s[j][q][r], kLog2E, -use));
                 const float sum = ((e[0][0] + e[0][1]) + (e[0][2] + e[0][3])) + ((e[1][0] + e[1][1]) + (e[1][2] + e[1][3]));
                 const float by = exp2_of(run[q].m - use), l = run[q].l * by;
-                if constexpr (BEST) {
-                    run[q].l = l + sum;
-                } else {   // (a label near weight 1 would take a long tail's small terms in one by one, and lose them)
-                    const float more = sum - low[q] * by;
-                    run[q].l = l + more;
-                    low[q] = (run[q].l - l) - more;
-                }
+                // (a label near weight 1 would take a long tail's small terms in one by one, and lose them)
+                const float more = sum - low[q] * by;
+                run[q].l = l + more;
+                low[q] = (run[q].l - l) - more;
                 run[q].m = top;
             }
         }

@@ -215,8 +215,8 @@ def label_rays(features, weight, bias=None):
     memory: (int64, float32) of the leading dimensions of features.
 
     The label is the one that 64 bits give: rays whose two best labels 32 bits cannot tell apart are decided again; the lowest
-    of equal ones.  A ray with NaN among its logits gets some label and log probability NaN.  Arguments as in `label_loss`;
-    not differentiable."""
+    of equal ones.  A ray with NaN among its logits, or with every label switched off, gets some label and log probability NaN.
+    Arguments as in `label_loss`; not differentiable."""
     _check_labels(features, weight, bias)
     shape, d = features.shape[:-1], features.size(-1)
     x, w = _matrix(features, d), _matrix(weight, d)

@@ -348,7 +348,8 @@ uint64_t dst_label_workspace_bytes(const DstLabelParams *params, int pass);
 int dst_label_loss_forward(const DstLabelParams *params, void *stream);
 int dst_label_loss_backward(const DstLabelParams *params, void *stream);
 /* The best label of every ray, as if the logits were formed in 64 bits (rays whose two best labels fp32 cannot tell
- * apart are decided again in 64 bits).  A ray with NaN among its logits gets some label and log probability NaN. */
+ * apart are decided again in 64 bits).  A ray with NaN among its logits, or with none above -inf, gets some label and log
+ * probability NaN. */
 int dst_label_best(const DstLabelParams *params, void *stream);
 
 /* Attention of queries to a memory of another length, no mask but each batch's length: for query head h of `heads`, which reads

@@ -125,3 +125,41 @@ def test_a_label_masked_by_the_lowest_value_as_target():
         assert (dst.label_loss(x, w, t, b, reduction="none") == float("inf")).all()
         for value in (low, float("-inf")):
             assert torch.isnan(dst.label_loss(x, w, t, torch.full((40,), value, device="cuda"), reduction="none")).all()
+
+
+@pytest.mark.parametrize("N,V", [(70, 40), (3, 20000), (70000, 333)], ids=str)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_best_label_where_every_label_is_masked(N, V, dtype):
+    """No label has a probability: NaN, not the most certain of all."""
+    import diff_surfel_tracing as dst
+    for D in (8, 40):
+        x, w = torch.ones(N, D, device="cuda", dtype=dtype), torch.ones(V, D, device="cuda", dtype=dtype)
+        b = torch.full((V,), float("-inf"), device="cuda")
+        label, log_prob = dst.label_rays(x, w, b)
+        assert torch.isnan(log_prob).all() and (label >= 0).all() and (label < V).all()
+        b[V // 2] = 0.0      # one that is not
+        label, log_prob = dst.label_rays(x, w, b)
+        assert (label == V // 2).all() and (log_prob == 0).all()
+
+
+@pytest.mark.parametrize("N,D,V,dtype", SIZES, ids=str)
+def test_best_label_of_sure_rays(N, D, V, dtype):
+    import diff_surfel_tracing as dst
+    for shift in (0.0, 1000.0):
+        x, w, b, t, up = _sure_rays(N, D, V, dtype, shift)
+        label, log_prob = dst.label_rays(x, w, b)
+        loss, bound = _reference(x, w, b, t, up)["loss"]
+        assert torch.equal(label, t) and float(log_prob.max()) <= 0.0
+        R.check(log_prob, (-loss, bound), "log_prob")
+
+
+def test_a_long_tail_behind_the_best_label_is_not_lost():
+    import diff_surfel_tracing as dst
+    V = 32001
+    b = torch.full((V,), -18.4, device="cuda")
+    b[0] = 0.0
+    label, log_prob = dst.label_rays(torch.zeros(70, 8, device="cuda"), torch.zeros(V, 8, device="cuda"), b)
+    others = float((b[1:].double().exp()).sum())
+    true = -torch.log1p(torch.tensor(others, dtype=torch.float64))
+    assert (label == 0).all()
+    assert float((log_prob.double() - true).abs().max()) <= NEAR_ONE * U + others * 60 * U
