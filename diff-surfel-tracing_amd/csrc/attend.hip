@@ -580,6 +580,12 @@ template <class TY, int NK> Sets row_sets(const DstAttendParams *p, AttendArgs &
     return s;
 }
 void prepare(const Sets &s, hipStream_t stream) { prepare({&s.q, &s.k, &s.v, &s.o, &s.low, &s.up}, stream); }
+int64_t copy_blocks(const Sets &s) { return copy_blocks({&s.q, &s.k, &s.v, &s.o, &s.low, &s.up}); }
+
+// DST_OK, or the refusal of rows that need more workgroups than a launch holds.
+int check_blocks(const Sets &s, const Cut &cut) {
+    return cut.blocks() <= kMostBlocks && copy_blocks(s) <= kMostBlocks ? (int)DST_OK : dst_op_fail(DST_E_UNSUPPORTED, "too many rows");
+}
 
 // Cuts a pass's own tiles; whether its rows are few. `kernel(few)`: the pass's kernel; `own_bytes`: of a part's row.
 template <class TY, int NK, class K>
@@ -674,11 +680,13 @@ uint64_t dst_attend_workspace_bytes(const DstAttendParams *p, int pass) {
             typedef decltype(ty) TY;
             constexpr int NK = decltype(nk)::value;
             AttendArgs a = arguments<TY>(p);
-            if (a.all_rows == 0) return DST_OK;
+            if (a.all_rows == 0) return (int)DST_OK;
             Carve c = {nullptr, 0};
-            row_sets<TY, NK>(p, a, false, c);
-            bytes = plan_forward<TY, NK>(a, heads, c).bytes;
-            return DST_OK;
+            const Sets sets = row_sets<TY, NK>(p, a, false, c);
+            const uint64_t need = plan_forward<TY, NK>(a, heads, c).bytes;
+            if (int rc = check_blocks(sets, a.cut)) return rc;
+            bytes = need;
+            return (int)DST_OK;
         });
     } else {
         with_gradients(p, [&](auto ty, auto nk) {
@@ -686,14 +694,17 @@ uint64_t dst_attend_workspace_bytes(const DstAttendParams *p, int pass) {
             constexpr int NK = decltype(nk)::value;
             AttendArgs a = arguments<TY>(p);
             Carve c = {nullptr, 0};
-            row_sets<TY, NK>(p, a, true, c);
+            const Sets sets = row_sets<TY, NK>(p, a, true, c);
             a.dq = p->grad_q;
-            bytes = plan_dq<TY, NK>(a, heads, c).bytes;
+            uint64_t need = plan_dq<TY, NK>(a, heads, c).bytes;
+            if (int rc = check_blocks(sets, a.cut)) return rc;
             if (p->grad_k || p->grad_v) {
                 const uint64_t more = plan_dkv<TY, NK>(a, heads, c).bytes;
-                bytes = more > bytes ? more : bytes;
+                if (int rc = check_blocks(sets, a.cut)) return rc;
+                need = more > need ? more : need;
             }
-            return DST_OK;
+            bytes = need;
+            return (int)DST_OK;
         });
     }
     return bytes;
@@ -711,6 +722,7 @@ int dst_attend_forward(const DstAttendParams *p, void *stream) {
         Carve c = {(char *)p->workspace, 0};
         const Sets sets = row_sets<TY, NK>(p, a, false, c);
         const Plan plan = plan_forward<TY, NK>(a, heads, c);
+        if (int rc = check_blocks(sets, a.cut)) return rc;
         if (int rc = check_workspace(p, plan.bytes)) return rc;
         const hipStream_t s = (hipStream_t)stream;
         prepare(sets, s);
@@ -753,9 +765,20 @@ int dst_attend_backward(const DstAttendParams *p, void *stream) {
         Carve c = {(char *)p->workspace, 0};
         const Sets sets = row_sets<TY, NK>(p, a, true, c);
         a.dq = p->grad_q, a.dk = p->grad_k, a.dvalue = p->grad_v;
-        if (a.all_rows > 0) {
-            const Plan plan = plan_dq<TY, NK>(a, heads, c);
-            if (int rc = check_workspace(p, plan.bytes)) return rc;
+        // (both passes are looked at before either runs)
+        const bool queries = a.all_rows > 0, memory = (a.dk || a.dvalue) && heads * a.memory > 0;
+        AttendArgs m = a;
+        Plan plan = {}, plan_m = {};
+        if (queries) {
+            plan = plan_dq<TY, NK>(a, heads, c);
+            if (int rc = check_blocks(sets, a.cut)) return rc;
+        }
+        if (memory) {
+            plan_m = plan_dkv<TY, NK>(m, heads, c);
+            if (int rc = check_blocks(sets, m.cut)) return rc;
+        }
+        if (int rc = check_workspace(p, plan.bytes > plan_m.bytes ? plan.bytes : plan_m.bytes)) return rc;
+        if (queries) {
             prepare(sets, s);
             const dim3 grid((uint32_t)a.cut.blocks());
             if (plan.few) k_attend_dq<TY, NK, 1><<<grid, kThreads, 0, s>>>(a);
@@ -768,17 +791,15 @@ int dst_attend_backward(const DstAttendParams *p, void *stream) {
             });
             DST_OP_LAUNCH("attention gradient, summing");
         }
-        if ((a.dk || a.dvalue) && heads * a.memory > 0) {
-            const Plan plan = plan_dkv<TY, NK>(a, heads, c);
-            if (int rc = check_workspace(p, plan.bytes)) return rc;
-            const dim3 grid((uint32_t)a.cut.blocks());
-            if (plan.few) k_attend_dkv<TY, NK, 1><<<grid, kThreads, 0, s>>>(a);
-            else k_attend_dkv<TY, NK, dkv_blocks<TY, NK>()><<<grid, kThreads, 0, s>>>(a);
+        if (memory) {
+            const dim3 grid((uint32_t)m.cut.blocks());
+            if (plan_m.few) k_attend_dkv<TY, NK, 1><<<grid, kThreads, 0, s>>>(m);
+            else k_attend_dkv<TY, NK, dkv_blocks<TY, NK>()><<<grid, kThreads, 0, s>>>(m);
             DST_OP_LAUNCH("attention gradient, memory");
-            const MemoryRow to = {a.cut.whole, a.tiles, a.own, a.memory, a.kv_heads};
-            with_output<E>(a.half, [&](auto one) {
+            const MemoryRow to = {m.cut.whole, m.tiles, m.own, m.memory, m.kv_heads};
+            with_output<E>(m.half, [&](auto one) {
                 typedef decltype(one) To;
-                sum_parts(Parts<To>{a.out_part, (To *)a.dk, a.d}, Parts<To>{a.out_part2, (To *)a.dvalue, a.dv}, a.cut, a.own, to, s);
+                sum_parts(Parts<To>{m.out_part, (To *)m.dk, m.d}, Parts<To>{m.out_part2, (To *)m.dvalue, m.dv}, m.cut, m.own, to, s);
             });
             DST_OP_LAUNCH("attention gradient, summing");
         }

@@ -800,6 +800,12 @@ struct LabelRow {
     }
 };
 
+// DST_OK, or the refusal of rows that need more workgroups than a launch holds.
+int check_blocks(const Sets &s, const Cut &cut) {
+    return cut.blocks() <= kMostBlocks && copy_blocks({&s.x, &s.w}) <= kMostBlocks ? (int)DST_OK
+                                                                                  : dst_op_fail(DST_E_UNSUPPORTED, "too many rays or labels");
+}
+
 int check_workspace(const DstLabelParams *p, uint64_t need) {
     if (need == 0) return DST_OK;
     if (!p->workspace || p->workspace_bytes < need)
@@ -820,17 +826,24 @@ uint64_t dst_label_workspace_bytes(const DstLabelParams *p, int pass) {
         with_gradients(p, [&](auto ty, auto nk) {
             typedef decltype(ty) TY;
             constexpr int NK = decltype(nk)::value;
-            const uint64_t x = p->grad_features ? backward_plan<TY, NK, true>(p, a, nullptr).bytes : 0;
-            const uint64_t w = p->grad_weight || p->grad_bias ? backward_plan<TY, NK, false>(p, a, nullptr).bytes : 0;
-            bytes = x > w ? x : w;
-            return DST_OK;
+            uint64_t need = 0;
+            for (int dx = 1; dx >= 0; --dx) {
+                if (dx ? !p->grad_features : !p->grad_weight && !p->grad_bias) continue;
+                const BackwardPlan b = dx ? backward_plan<TY, NK, true>(p, a, nullptr) : backward_plan<TY, NK, false>(p, a, nullptr);
+                if (int rc = check_blocks(b.sets, a.cut)) return rc;
+                need = b.bytes > need ? b.bytes : need;
+            }
+            bytes = need;
+            return (int)DST_OK;
         });
     } else {
         with_type(p, [&](auto ty, auto nk) {
             typedef decltype(ty) TY;
             constexpr int NK = decltype(nk)::value;
-            bytes = pass == DST_PASS_BEST ? forward_plan<TY, NK, true>(p, a, nullptr).bytes : forward_plan<TY, NK, false>(p, a, nullptr).bytes;
-            return DST_OK;
+            const ForwardPlan f = pass == DST_PASS_BEST ? forward_plan<TY, NK, true>(p, a, nullptr) : forward_plan<TY, NK, false>(p, a, nullptr);
+            if (int rc = check_blocks(f.sets, a.cut)) return rc;
+            bytes = f.bytes;
+            return (int)DST_OK;
         });
     }
     return bytes;
@@ -846,6 +859,7 @@ int dst_label_loss_forward(const DstLabelParams *p, void *stream) {
         constexpr int NK = decltype(nk)::value;
         LabelArgs a = arguments(p);
         const ForwardPlan f = forward_plan<TY, NK, false>(p, a, (char *)p->workspace);
+        if (int rc = check_blocks(f.sets, a.cut)) return rc;
         if (int rc = check_workspace(p, f.bytes)) return rc;
         if (p->reduction == DST_REDUCE_NONE) a.rows = p->loss;
         const hipStream_t s = (hipStream_t)stream;
@@ -881,13 +895,24 @@ int dst_label_loss_backward(const DstLabelParams *p, void *stream) {
         typedef typename TY::E E;
         constexpr int NK = decltype(nk)::value, QB = dw_blocks<TY, NK>();
         const hipStream_t s = (hipStream_t)stream;
+        const bool wanted[2] = {p->grad_features && p->rays > 0, p->grad_weight || p->grad_bias};   // dx, dw
+        LabelArgs args[2] = {arguments(p), arguments(p)};
+        BackwardPlan plans[2];
+        uint64_t need = 0;
+        for (int pass = 0; pass < 2; ++pass) {   // (both are looked at before either runs)
+            if (!wanted[pass]) continue;
+            plans[pass] = pass == 0 ? backward_plan<TY, NK, true>(p, args[0], (char *)p->workspace)
+                                    : backward_plan<TY, NK, false>(p, args[1], (char *)p->workspace);
+            if (int rc = check_blocks(plans[pass].sets, args[pass].cut)) return rc;
+            need = plans[pass].bytes > need ? plans[pass].bytes : need;
+        }
+        if (int rc = check_workspace(p, need)) return rc;
         bool copied = false;
         for (int pass = 0; pass < 2; ++pass) {
+            if (!wanted[pass]) continue;
             const bool dx = pass == 0;
-            if (dx ? !p->grad_features || p->rays == 0 : !p->grad_weight && !p->grad_bias) continue;
-            LabelArgs a = arguments(p);
-            const BackwardPlan b = dx ? backward_plan<TY, NK, true>(p, a, (char *)p->workspace) : backward_plan<TY, NK, false>(p, a, (char *)p->workspace);
-            if (int rc = check_workspace(p, b.bytes)) return rc;
+            LabelArgs &a = args[pass];
+            const BackwardPlan &b = plans[pass];
             a.half = p->dtype == DST_DTYPE_F16;
             a.upstream = p->upstream, a.upstream_rows = p->reduction == DST_REDUCE_NONE;
             a.inverse = a.upstream_rows ? nullptr : p->inverse;
@@ -922,6 +947,7 @@ int dst_label_best(const DstLabelParams *p, void *stream) {
         constexpr int NK = decltype(nk)::value;
         LabelArgs a = arguments(p);
         const ForwardPlan f = forward_plan<TY, NK, true>(p, a, (char *)p->workspace);
+        if (int rc = check_blocks(f.sets, a.cut)) return rc;
         if (int rc = check_workspace(p, f.bytes)) return rc;
         a.label = p->best, a.log_prob = p->log_prob;
         const hipStream_t s = (hipStream_t)stream;

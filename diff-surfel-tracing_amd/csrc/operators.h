@@ -62,6 +62,7 @@ inline uint64_t align_up(uint64_t bytes) { return (bytes + 255u) & ~(uint64_t)25
 // tiles that do not fill its last round (or are fewer than it holds) are cut into parts of the streamed tiles, whose sums a
 // closing kernel adds: 513 tiles on 512 places would take two rounds. Tiles below `whole` are not cut.
 constexpr int kMostSplits = 512;
+constexpr int64_t kMostBlocks = 0xffffff;   // workgroups of a launch, whose threads are counted in 32 bits
 struct Cut {
     int32_t tiles, whole, splits, per_split;   // per_split: streamed tiles of a part
     __host__ __device__ int64_t parted() const { return tiles - whole; }
@@ -270,6 +271,13 @@ RowSet row_set(const void *p, int dtype, int64_t batch, int64_t row, int64_t hea
         s.rows = Rows{(const char *)s.copy.to, (int64_t)heads * n * line, n * line, line, 0, 1, words};
     }
     return s;
+}
+// Workgroups of the launch that makes the copies.
+inline int64_t copy_blocks(std::initializer_list<const RowSet *> sets) {
+    int64_t blocks = 0;
+    for (const RowSet *s : sets)
+        if (s->copied) blocks += div_up(s->copy.all_words, 256);
+    return blocks;
 }
 // Makes the copies of the sets that have any.
 inline void prepare(std::initializer_list<const RowSet *> sets, hipStream_t stream) {

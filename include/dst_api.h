@@ -317,7 +317,8 @@ int dst_pack_sh_half(const float *shs, uint16_t *out, uint64_t n_values, void *s
 /* Softmax cross entropy of rays against a table of labels: s = features . weight^T + bias, loss = log sum exp s - s[target],
  * 0 where the target is ignore_index, NaN (and NaN gradients) where it is neither that nor in 0..labels-1. */
 typedef struct DstLabelParams {
-    int64_t rays;                 /* 0..2^31-1 */
+    int64_t rays;                 /* 0..2^31-1, as many as 2^24-1 workgroups of 64 to 256 hold where rows are read as they lie; of rows that
+                                   * are copied, fewer than 2^32 words of 16 bytes of both sets together.  More is refused, as too many labels are */
     int32_t channels, labels;     /* 1..DST_MAX_CHANNELS, 1..DST_MAX_LABELS */
     int32_t dtype;                /* DST_DTYPE_* of features and weight and of their gradients */
     int32_t reduction;            /* DST_REDUCE_*; the mean is over the rays that are not ignored (none: NaN) */
@@ -356,7 +357,8 @@ int dst_label_best(const DstLabelParams *params, void *stream);
  * kv head h / (heads / kv_heads):  p = softmax_j(scale q . k_j) over j < lengths[batch],  out = sum_j p_j v_j.
  * A length of 0 gives zeros and no gradient.  Keys and values behind the length are not used and may hold anything. */
 typedef struct DstAttendParams {
-    int32_t batch, queries, memory;   /* >= 0 */
+    int32_t batch, queries, memory;   /* >= 0; at most 2^24-1 workgroups of 64 or 128 rows of one kv head of one batch (queries of its heads, or
+                                       * memory for the gradients), and fewer than 2^32 words of 16 bytes of rows that are copied: more is refused */
     int32_t heads, kv_heads;          /* heads a multiple of kv_heads */
     int32_t channels, value_channels; /* 1..DST_MAX_CHANNELS */
     int32_t dtype;                    /* DST_DTYPE_* of all rows */
