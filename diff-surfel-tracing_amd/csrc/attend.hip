@@ -75,10 +75,17 @@ template <class TY, int NK, int QB> __device__ inline void carry_scale(Own<TY, N
 // The weight of a product of rows, `less` its row's maximum or lse. EXACT: the score is rounded before the difference is
 // formed, so a row with one weight gets exactly 1, its value and, in the backward pass, scores without a gradient. A forward pass that
 // a backward pass follows is exact; the others save the instruction (131,072 rows x 1024 in 4 heads of 64: 184 us, 176).
+// Weights of binary16 rows come 2^kLift larger: they are rounded to binary16 for the product with the values, where less than 2^-14 loses bits
+// and less than 2^-25 everything, while the sum of weights, in 32 bits, counts it. (A row with one strong score and 65,535 of weights
+// just below 2^-25 lost 0.2 % of its mass.) With kSlack the weights stay at or below 2^15. An exact weight takes an instruction more for
+// it: less - kLift would round.
+template <class TY> constexpr float kLift = std::is_same_v<TY, F16> ? 7.0f : 0.0f;
+template <class TY> constexpr float kLiftBack = std::is_same_v<TY, F16> ? 1.0f / 128.0f : 1.0f;
 template <class TY, bool EXACT> __device__ inline float weight_of(const AttendArgs &a, float s, float less) {
     if constexpr (TY::kDepth == 16) return exp2_of(s - less);
+    else if constexpr (EXACT && std::is_same_v<TY, F16>) return exp2_of(s * a.c - less + kLift<TY>);
     else if constexpr (EXACT || TY::kPlanes == 3) return exp2_of(s * a.c - less);
-    else return exp2_of(__builtin_fmaf(s, a.c, -less));
+    else return exp2_of(__builtin_fmaf(s, a.c, std::is_same_v<TY, F16> ? kLift<TY> - less : -less));
 }
 
 // A row of out, and of what its rounding leaves: delta, a difference of what cancels, is formed of both.
@@ -95,7 +102,7 @@ template <class E> __device__ inline void store_out(const AttendArgs &a, int64_t
 
 // ---- forward --------------------------------------------------------------------------------------------------------
 // The running maximum is raised (and the sums scaled) only when a value is more than 2^kSlack above it: the weights then
-// stay below 2^kSlack, which every type holds, and most tiles need no exchange between lanes.
+// stay below 2^kSlack, which every type holds (binary16 with kLift too), and most tiles need no exchange between lanes.
 constexpr float kSlack = 8.0f;
 
 // Bound by vector and matrix instructions together, which two waves on a SIMD overlap in part: 131,072 rows x 1024 in 4 heads of 64, bf16,
@@ -189,7 +196,7 @@ template <class TY, int NK, int QB, bool EXACT> __global__ __launch_bounds__(kTh
 #pragma unroll
     for (int q = 0; q < QB; ++q) {
         const int row = row0 + q * 16 + (lane & 15);
-        const float sum = sum_group(l[q]);
+        const float sum = sum_group(l[q]) * kLiftBack<TY>;
         if (row >= a.rows) continue;
         const int64_t at = stat_row(a, p, row);
         if (turn.part) {
@@ -197,10 +204,10 @@ template <class TY, int NK, int QB, bool EXACT> __global__ __launch_bounds__(kTh
             if (g == 0) a.part[part] = float2{m[q], sum};
             if (first < last)
 #pragma unroll
-                for (int i = 0; i < NM; ++i) store_four(a.out_part + part * a.dv, i * 16 + 4 * g, a.dv, out[q][i], four);
+                for (int i = 0; i < NM; ++i) store_four(a.out_part + part * a.dv, i * 16 + 4 * g, a.dv, out[q][i] * kLiftBack<TY>, four);
             continue;
         }
-        const float by = p.length > 0 ? 1.0f / sum : 0.0f;
+        const float by = p.length > 0 ? kLiftBack<TY> / sum : 0.0f;
         if (g == 0 && a.lse2) a.lse2[at] = p.length > 0 ? m[q] + log2_of(sum) : kInf;
         const int64_t to = out_row(a, p, row);
 #pragma unroll
