@@ -524,6 +524,9 @@ int check(const DstAttendParams *p) {
     if (rows > most || p->memory > most || (int64_t)p->batch * p->kv_heads > most ||
         (int64_t)p->batch * p->kv_heads * (div_up(rows, 16) > div_up(p->memory, 16) ? div_up(rows, 16) : div_up(p->memory, 16)) > most)
         return dst_op_fail(DST_E_UNSUPPORTED, "too many rows");
+    for (const int64_t *strides : {p->q_strides, p->k_strides, p->v_strides})
+        for (int i = 0; i < 3; ++i)
+            if (strides[i] < 0 || strides[i] > kLongestStride) return dst_op_fail(DST_E_INVALID, "strides must be in 0..2^44");
     const bool any = p->batch > 0 && p->queries > 0;
     if (any && (!p->q || !p->out || (p->memory > 0 && (!p->k || !p->v)))) return dst_op_fail(DST_E_INVALID, "q, k, v and out are required");
     return DST_OK;

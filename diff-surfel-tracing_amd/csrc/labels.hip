@@ -675,6 +675,7 @@ int check(const DstLabelParams *p) {
         return dst_op_fail(DST_E_UNSUPPORTED, "channels must be in 1..%d", DST_MAX_CHANNELS);
     if (p->features_stride < p->channels || p->weight_stride < p->channels)
         return dst_op_fail(DST_E_INVALID, "rows of features and weight must not overlap");
+    if (p->features_stride > kLongestStride || p->weight_stride > kLongestStride) return dst_op_fail(DST_E_INVALID, "strides must be in 0..2^44");
     if (p->reduction < DST_REDUCE_NONE || p->reduction > DST_REDUCE_MEAN) return dst_op_fail(DST_E_INVALID, "unknown reduction");
     if ((p->rays > 0 && !p->features) || !p->weight) return dst_op_fail(DST_E_INVALID, "features and weight are required");
     return DST_OK;

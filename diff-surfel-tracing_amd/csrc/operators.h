@@ -21,6 +21,7 @@ int dst_op_fail(int code, const char *format, ...) __attribute__((format(printf,
 
 namespace {
 
+constexpr int64_t kLongestStride = (int64_t)1 << 44;   // values; offsets of 256 rows in bytes are far from 64 bits' end
 inline int value_size(int dtype) { return dtype == DST_DTYPE_F32 ? 4 : 2; }
 // 32-bit rows longer than this are split into planes of 16 bits (tiles.inc).
 constexpr int kLongest32 = 16;

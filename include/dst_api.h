@@ -365,7 +365,7 @@ typedef struct DstAttendParams {
     float scale;
     int32_t reserved;
     const void *q, *k, *v;            /* rows of channels (value_channels) consecutive values; strides in values, by batch, */
-    int64_t q_strides[3], k_strides[3], v_strides[3];   /* row and head (0: shared) */
+    int64_t q_strides[3], k_strides[3], v_strides[3];   /* row and head (0: shared), 0..2^44 */
     const int32_t *lengths;           /* (batch), clamped to 0..memory; NULL: memory everywhere */
     void *out;                        /* (batch, queries, heads, value_channels), contiguous, as all that follow */
     float *lse;                       /* (batch, kv_heads, queries * heads / kv_heads): forward writes (NULL: not wanted),

@@ -86,3 +86,19 @@ def test_labels(lib):
     _refused(lib, calls[BACKWARD], size, _label(rays=2 ** 31 - 1, channels=8, dtype=BF16), BACKWARD, b"too many rays")
     _refused(lib, calls[BACKWARD], size, _label(labels=2 ** 30 - 1, channels=256, dtype=BF16, grad_features=None), BACKWARD, b"too many rays")
     _admitted(lib, calls[BEST], size, _label(rays=2 ** 31 - 1, channels=8, dtype=BF16), BEST)
+
+
+@pytest.mark.parametrize("name", ["q_strides", "k_strides", "v_strides"])
+@pytest.mark.parametrize("at", [0, 1, 2])
+@pytest.mark.parametrize("stride", [-1, -2 ** 62, 2 ** 44 + 1, 2 ** 62])
+def test_strides_that_offsets_are_not_made_for(lib, name, at, stride):
+    p = _attend()
+    getattr(p, name)[at] = stride
+    for what, call in ((FORWARD, lib.dst_attend_forward), (BACKWARD, lib.dst_attend_backward)):
+        _refused(lib, call, lib.dst_attend_workspace_bytes, p, what, b"strides")
+
+
+def test_label_strides_that_offsets_are_not_made_for(lib):
+    for what, call in enumerate((lib.dst_label_loss_forward, lib.dst_label_loss_backward, lib.dst_label_best)):
+        for name in ("features_stride", "weight_stride"):
+            _refused(lib, call, lib.dst_label_workspace_bytes, _label(**{name: 2 ** 62}), what, b"stride")
