@@ -442,8 +442,9 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
     };
     if (first < last) fetch(first);
     Own<TY, NK, QB> own_k, own_v;
-    own_k.load(a.k, tile_base(a.k, row0, p.batch, p.kv), p.length - row0);
-    own_v.load(a.v, tile_base(a.v, row0, p.batch, p.kv), p.length - row0);
+    const int own_rows = first < last ? p.length - row0 : 0;   // (without queries the memory need not be there)
+    own_k.load(a.k, tile_base(a.k, row0, p.batch, p.kv), own_rows);
+    own_v.load(a.v, tile_base(a.v, row0, p.batch, p.kv), own_rows);
     carry_scale(own_k, a);
     f4 dk[QB][NM], dv[QB][NM];
 #pragma unroll
