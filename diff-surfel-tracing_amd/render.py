@@ -16,6 +16,7 @@ import argparse
 import json
 import math
 import os
+import re
 import struct
 import sys
 import zlib
@@ -92,7 +93,7 @@ def load_surfel_model(path, max_sh_degree=3):
     rot = rot / rot.norm(dim=-1, keepdim=True)
     model = {"means3D": xyz.contiguous(), "shs": shs, "opacities": torch.sigmoid(f32("opacity"))[:, None].contiguous(),
              "scales": scales, "rotations": rot.contiguous()}
-    aux = numbered("aux_")
+    aux = sorted([n for n in names if re.fullmatch("aux_[0-9]+", n)], key=lambda n: int(n[4:]))
     if aux:
         model["others_precomp"] = torch.stack([f32(n) for n in aux], 1).contiguous()
     model["vertices"], model["faces"] = S.get_triangles(model["means3D"], model["scales"], model["rotations"])
@@ -234,6 +235,7 @@ def render_path(tracer, model, cameras, result_dir=None, white_bg=True, sh_degre
             raise ValueError("the model has %d auxiliary channels, %s is for %d"
                              % (channels, name, what[name].shape[1 if name == "weight" else 0]))
     label_head, memory_bank = ({k: v.to(dev) for k, v in d.items()} if d else None for d in (label_head, memory_bank))
+    others = g.get("others_precomp") if label_head or memory_bank else None   # (traced only for what reads them)
     bg = torch.tensor([1.0, 1.0, 1.0] if white_bg else [0.0, 0.0, 0.0], dtype=torch.float32, device=dev)
     grads3D = torch.zeros_like(g["means3D"])
     eye = torch.eye(4, device=dev)
@@ -249,7 +251,7 @@ def render_path(tracer, model, cameras, result_dir=None, white_bg=True, sh_degre
         with torch.no_grad():
             rgb, dpt, acc, norm, dist, aux, mid, wet = tracer(
                 ray_o.to(dev), ray_d.to(dev), g["vertices"], means3D=g["means3D"], grads3D=grads3D, shs=g.get("shs"),
-                colors_precomp=g.get("colors_precomp"), others_precomp=g.get("others_precomp"),
+                colors_precomp=g.get("colors_precomp"), others_precomp=others,
                 opacities=g["opacities"], scales=g["scales"], rotations=g["rotations"], cov3D_precomp=None,
                 tracer_settings=settings, start_from_first=True)
             labels = pixel_labels(aux, label_head)[0] if label_head else None
