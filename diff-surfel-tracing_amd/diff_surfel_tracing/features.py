@@ -182,6 +182,8 @@ def label_loss(features, weight, targets, bias=None, *, ignore_index=-100, reduc
         raise RuntimeError("targets must be whole numbers of dimensions %s, those of features without the last"
                            % (tuple(features.shape[:-1]),))
     ignore_index = int(ignore_index)
+    if not -2 ** 63 <= ignore_index < 2 ** 63:
+        raise RuntimeError("ignore_index must be a whole number of 64 bits (got %d)" % ignore_index)
     shape, d = features.shape[:-1], features.size(-1)
     wants = _wants_grad(features, weight, bias)
     x, w, t = _matrix(features, d), _matrix(weight, d), targets.reshape(-1).to(torch.int64).contiguous()

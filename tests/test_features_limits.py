@@ -102,3 +102,17 @@ def test_label_strides_that_offsets_are_not_made_for(lib):
     for what, call in enumerate((lib.dst_label_loss_forward, lib.dst_label_loss_backward, lib.dst_label_best)):
         for name in ("features_stride", "weight_stride"):
             _refused(lib, call, lib.dst_label_workspace_bytes, _label(**{name: 2 ** 62}), what, b"stride")
+
+
+@pytest.mark.parametrize("number", [2 ** 64 - 100, 2 ** 63, -2 ** 63 - 1])
+def test_an_ignore_index_beyond_64_bits_does_not_become_another(monkeypatch, number):
+    import torch
+
+    import diff_surfel_tracing as dst
+    import diff_surfel_tracing.features as F
+    monkeypatch.setattr(F, "_rows", lambda t, name: None)
+    monkeypatch.setattr(F, "_loss_forward", lambda x, *a: (torch.zeros(x.size(0)), None, None))
+    args = torch.zeros(4, 8), torch.zeros(5, 8), torch.zeros(4, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="ignore_index"):
+        dst.label_loss(*args, ignore_index=number, reduction="none")
+    assert dst.label_loss(*args, ignore_index=-2 ** 63, reduction="none").shape == (4,)
