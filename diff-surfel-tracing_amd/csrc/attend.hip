@@ -72,20 +72,19 @@ template <class TY, int NK, int QB> __device__ inline void carry_scale(Own<TY, N
                 else if (a.flip) w ^= u4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
             }
 }
-// The weight of a product of rows, `less` its row's maximum or lse. EXACT: the score is rounded before the difference is
-// formed, so a row with one weight gets exactly 1, its value and, in the backward pass, scores without a gradient. A forward pass that
-// a backward pass follows is exact; the others save the instruction (131,072 rows x 1024 in 4 heads of 64: 184 us, 176).
+// The weight of a product of rows, `less` its row's maximum or lse. The score is rounded before the difference is formed (no fused
+// multiply-add): both are then rounded alike, however large, and a row with one weight gets exactly 1, its value and, in the backward
+// pass, scores without a gradient. (With a fused one a score of 1.7e7 had weights of up to 2, and one of 1e10 had none: the exact score
+// lies that far from the rounded one. It saved 4 % of 131,072 rows x 1024 in 4 heads of 64.)
 // Weights of binary16 rows come 2^kLift larger: they are rounded to binary16 for the product with the values, where less than 2^-14 loses bits
 // and less than 2^-25 everything, while the sum of weights, in 32 bits, counts it. (A row with one strong score and 65,535 of weights
-// just below 2^-25 lost 0.2 % of its mass.) With kSlack the weights stay at or below 2^15. An exact weight takes an instruction more for
-// it: less - kLift would round.
+// just below 2^-25 lost 0.2 % of its mass.) With kSlack the weights stay at or below 2^15.
 template <class TY> constexpr float kLift = std::is_same_v<TY, F16> ? 7.0f : 0.0f;
 template <class TY> constexpr float kLiftBack = std::is_same_v<TY, F16> ? 1.0f / 128.0f : 1.0f;
-template <class TY, bool EXACT> __device__ inline float weight_of(const AttendArgs &a, float s, float less) {
+template <class TY> __device__ inline float weight_of(const AttendArgs &a, float s, float less) {
     if constexpr (TY::kDepth == 16) return exp2_of(s - less);
-    else if constexpr (EXACT && std::is_same_v<TY, F16>) return exp2_of(s * a.c - less + kLift<TY>);
-    else if constexpr (EXACT || TY::kPlanes == 3) return exp2_of(s * a.c - less);
-    else return exp2_of(__builtin_fmaf(s, a.c, std::is_same_v<TY, F16> ? kLift<TY> - less : -less));
+    else if constexpr (std::is_same_v<TY, F16>) return exp2_of(s * a.c - less + kLift<TY>);   // (less - kLift would round)
+    else return exp2_of(s * a.c - less);
 }
 
 // A row of out, and of what its rounding leaves: delta, a difference of what cancels, is formed of both.
@@ -109,7 +108,7 @@ constexpr float kSlack = 8.0f;
 // 175 us, 786 TFLOP/s, vector instructions 77 % of the cycles and matrix ones 40 %; 16384 x 8192 in 8 heads of 128, 645 us,
 // 852 TFLOP/s, 49 % and 42 %. One ray that asks a long memory is bound by reading it: 65,536 rows of 8 heads of 128, 45 us, 5.9 TB/s
 // (a large copy moves 4.7), in 64 parts a head, and 7 us to join them.
-template <class TY, int NK, int QB, bool EXACT> __global__ __launch_bounds__(kThreads) void k_attend_forward(AttendArgs a) {
+template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void k_attend_forward(AttendArgs a) {
     typedef Shape<TY, NK> T;
     typedef typename TY::E E;
     constexpr int NM = depth_blocks<TY, NK>();
@@ -184,7 +183,7 @@ template <class TY, int NK, int QB, bool EXACT> __global__ __launch_bounds__(kTh
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[j][q][r] = weight_of<TY, EXACT>(a, s[j][q][r], use);
+                    for (int r = 0; r < 4; ++r) s[j][q][r] = weight_of<TY>(a, s[j][q][r], use);
                 const f4 u = s[0][q], v = s[1][q];
                 l[q] += ((u[0] + u[1]) + (u[2] + u[3])) + ((v[0] + v[1]) + (v[2] + v[3]));
             }
@@ -390,7 +389,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
                 for (int q = 0; q < QB; ++q)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        s[j][q][r] = weight_of<TY, false>(a, s[j][q][r], lse2[q]) * (dp[q][r] - delta[q]);
+                        s[j][q][r] = weight_of<TY>(a, s[j][q][r], lse2[q]) * (dp[q][r] - delta[q]);
             }
             accumulate<TY, NK, QB, NM>(tile_k, pair, s[0], s[1], out);
         }
@@ -473,7 +472,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
                 for (int q = 0; q < QB; ++q)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float e = weight_of<TY, false>(a, s[j][q][r], lse2[r]);
+                        const float e = weight_of<TY>(a, s[j][q][r], lse2[r]);
                         s[j][q][r] = e;
                         dp[j][q][r] = e * (dp[j][q][r] - delta[r]);
                     }
@@ -618,9 +617,8 @@ struct Plan {
 };
 template <class TY, int NK> Plan plan_forward(AttendArgs &a, int64_t heads, Carve c) {
     Plan p;
-    constexpr bool some = !TY::kRounds;   // (32-bit rows are always exact)
     p.few = plan_cut<TY, NK>(a, forward_blocks<TY, NK>(), a.rows, a.memory, heads, 2, a.dv * 4.0 + 8.0, [](bool few) {
-        return few ? (const void *)&k_attend_forward<TY, NK, 1, some> : (const void *)&k_attend_forward<TY, NK, forward_blocks<TY, NK>(), some>;
+        return few ? (const void *)&k_attend_forward<TY, NK, 1> : (const void *)&k_attend_forward<TY, NK, forward_blocks<TY, NK>()>;
     });
     if (const uint64_t rows = parted_rows(a)) {
         a.part = c.take<float2>(rows);
@@ -738,13 +736,8 @@ int dst_attend_forward(const DstAttendParams *p, void *stream) {
         const hipStream_t s = (hipStream_t)stream;
         prepare(sets, s);
         const dim3 grid((uint32_t)a.cut.blocks());
-        if (TY::kRounds && !a.out_low) {
-            if (plan.few) k_attend_forward<TY, NK, 1, !TY::kRounds><<<grid, kThreads, 0, s>>>(a);
-            else k_attend_forward<TY, NK, QB, !TY::kRounds><<<grid, kThreads, 0, s>>>(a);
-        } else {
-            if (plan.few) k_attend_forward<TY, NK, 1, true><<<grid, kThreads, 0, s>>>(a);
-            else k_attend_forward<TY, NK, QB, true><<<grid, kThreads, 0, s>>>(a);
-        }
+        if (plan.few) k_attend_forward<TY, NK, 1><<<grid, kThreads, 0, s>>>(a);
+        else k_attend_forward<TY, NK, QB><<<grid, kThreads, 0, s>>>(a);
         DST_OP_LAUNCH("attention");
         if (a.cut.splits > 1) {
             const int64_t rows = a.cut.parted() * a.own;
