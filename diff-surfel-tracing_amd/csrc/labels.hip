@@ -25,10 +25,11 @@ struct LabelArgs {
     Cut cut;
     int32_t own;                    // own rows of a workgroup
     // forward
-    float2 *part;                   // of a part's rays: maximum and sum, in units of log 2
+    float2 *part;                   // of a part's rays: maximum and sum
     float *target_logit;            // of the parted rays
     float *lse2;                    // (rays): log2 of the sum of exponentials; +inf where the ray is ignored
-    float *hit;                     // (rays): the weight of the ray's label less one, 0 where the ray is ignored; forward: or nullptr
+    float *top, *log_sum, *hit;     // (rays): largest logit, log2 of the sum relative to it (+inf where the ray is ignored), the weight of the
+                                    // ray's label less one; forward: or nullptr
     float *rows;                    // (rays) losses, or nullptr
     double *sums;                   // (blocks): sums of losses ...
     uint32_t *counts;               // ... and rays counted in them
@@ -75,13 +76,12 @@ __device__ inline float upstream_of(const LabelArgs &a, int64_t row, int64_t t) 
 }
 
 // ---- forward --------------------------------------------------------------------------------------------------------
-// What a logit lies below the logarithm of the sum, in units of log 2. The sum is 1 or more and relative to the maximum, and the logit is taken
-// relative to the maximum too, so of what both have in common nothing is rounded: a label with almost all of the weight keeps the digits of what it
-// lacks. (The maximum is a rounded product with log2 e; the sum's terms and the logit are both exact products less that number. A term near 1
-// is taken as the sum has it, rounded: a label alone lacks nothing.)
+// What a logit lies below the logarithm of the sum. The sum is 1 or more and relative to the maximum, and the logit is taken relative to the maximum
+// too, so of what both have in common nothing is rounded: a label with almost all of the weight keeps the digits of what it
+// lacks. (A term near 1 is taken as the sum has it, rounded: a label alone lacks nothing.)
 __device__ inline float below_sum(Running r, float logit) {
-    const float at = __builtin_fmaf(logit, kLog2E, -r.m);
-    return larger(log2_of(r.l) - (at > -1.0f ? log2_of(exp2_of(at)) : at), 0.0f);
+    const float at = logit - r.m, log_sum = log2_of(r.l);
+    return at > -1.0f ? larger(log_sum - log2_of(exp_of(at)), 0.0f) * kLn2 : log_sum * kLn2 - at;
 }
 // Whether there is a logit above -inf and none is +inf.
 __device__ inline bool has_sum(Running r) { return r.l > 0.0f; }
@@ -99,13 +99,12 @@ template <class TY, int NK> __device__ inline float logit_of(const Fragment<TY> 
 __device__ inline void finish_row(const LabelArgs &a, int64_t row, Running r, float target_logit, double &sum, uint32_t &count) {
     const int64_t t = a.target[row];
     const bool ignored = t == a.ignore;
-    const float lse2 = r.m + log2_of(r.l);
-    float loss = below_sum(r, target_logit) * kLn2;
-    if (loss == kInf && target_logit > -kInf) loss = lse2 * kLn2 - target_logit;   // (its product with log2 e is beyond 32 bits)
+    const float log_sum = log2_of(r.l);
+    float loss = below_sum(r, target_logit);
     if (!has_sum(r) || t < 0 || t >= a.labels) loss = __builtin_nanf("");
     if (ignored) loss = 0.0f;
-    a.lse2[row] = ignored ? kInf : lse2;
-    if (a.hit) a.hit[row] = expm1f(-loss);
+    a.lse2[row] = ignored ? kInf : r.m * kLog2E + log_sum;
+    if (a.hit) a.top[row] = ignored ? 0.0f : r.m, a.log_sum[row] = ignored ? kInf : log_sum, a.hit[row] = expm1f(-loss);
     if (a.rows) a.rows[row] = loss;
     sum += (double)loss;
     count += ignored ? 0u : 1u;
@@ -139,7 +138,7 @@ __device__ inline void finish_best(const LabelArgs &a, int64_t row, Running r, f
     const float reach = norm * bound.x, tall = fminf(bound.y, __builtin_fabsf(bound.z) + 2.1f * reach);
     const float off = norm > 0.0f ? a.margin * (reach + tall) + 1e-35f : 0.0f;
     a.label[row] = label == 0x7fffffff ? 0 : label;
-    a.log_prob[row] = has_sum(r) ? -below_sum(r, best) * kLn2 : __builtin_nanf("");   // (no label left: there is no probability)
+    a.log_prob[row] = has_sum(r) ? -below_sum(r, best) : __builtin_nanf("");   // (no label left: there is no probability)
     if (best - second < 2.0f * off) {
         const uint32_t i = atomicAdd(a.near_count, 1u);
         a.near_list[i] = (uint32_t)row;
@@ -233,19 +232,21 @@ template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThr
                             place[q] = v > best[q] ? (pair + j) * 16 + r : place[q];
                             best[q] = larger(best[q], v);
                         }
-                    top = best[q] * kLog2E;
+                    top = best[q];
                 } else {
-                    top = larger(larger(largest(s[0][q]), largest(s[1][q])) * kLog2E, run[q].m);
+                    top = larger(larger(largest(s[0][q]), largest(s[1][q])), run[q].m);
                 }
+                // (a difference and its scaling are an instruction more than a fused product less the scaled maximum; that compared exact
+                // products with a rounded one, and gave a lane that had met nothing but labels masked by -1e10 a sum of +inf)
                 // (eight at a time, added in pairs: the running sum sees an eighth of the additions)
                 const float use = finite_or_zero(top);
                 f4 e[2];
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) e[j][r] = exp2_of(__builtin_fmaf(s[j][q][r], kLog2E, -use));
+                    for (int r = 0; r < 4; ++r) e[j][r] = exp_of(s[j][q][r] - use);
                 const float sum = ((e[0][0] + e[0][1]) + (e[0][2] + e[0][3])) + ((e[1][0] + e[1][1]) + (e[1][2] + e[1][3]));
-                const float by = exp2_of(run[q].m - use), l = run[q].l * by;
+                const float by = exp_of(run[q].m - use), l = run[q].l * by;
                 // (a label near weight 1 would take a long tail's small terms in one by one, and lose them)
                 const float more = sum - low[q] * by;
                 run[q].l = l + more;
@@ -333,7 +334,7 @@ template <bool BEST> __global__ __launch_bounds__(kThreads) void k_label_join(La
         for (int s = 0; s < a.cut.splits; ++s) {
             const float2 p = a.part[from + (int64_t)s * a.own];
             const float top = larger(m, p.x), use = finite_or_zero(top);
-            l = l * (double)exp2_of(m - use) + (double)p.y * (double)exp2_of(p.x - use);
+            l = l * (double)exp_of(m - use) + (double)p.y * (double)exp_of(p.x - use);
             m = top;
             if constexpr (BEST) {
                 const int4 b = a.best[from + (int64_t)s * a.own];
@@ -479,14 +480,15 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads, TY::k
     fetch(first);
     Own<TY, NK, QB> own;
     own.load(a.x, tile_base(a.x, row0), (int)min(a.rays - row0, (int64_t)(16 * QB)));
-    float lse2[QB], up[QB], hit[QB];
+    float top[QB], log_sum[QB], up[QB], hit[QB];
     int label[QB];   // relative to the lane's first row of a tile
     f4 out[QB][NM];
 #pragma unroll
     for (int q = 0; q < QB; ++q) {
         const int64_t row = row0 + q * 16 + (lane & 15);
         const int64_t t = row < a.rays ? a.target[row] : a.ignore;
-        lse2[q] = row < a.rays ? a.lse2[row] : kInf;
+        top[q] = row < a.rays ? a.top[row] : 0.0f;
+        log_sum[q] = row < a.rays ? a.log_sum[row] : kInf;
         up[q] = row < a.rays ? upstream_of(a, row, t) : 0.0f;
         hit[q] = row < a.rays ? a.hit[row] : 0.0f;
         label[q] = (t >= 0 && t < a.labels ? (int)t : -0x40000000) - 4 * g;
@@ -512,7 +514,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads, TY::k
                 for (int q = 0; q < QB; ++q)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float e = exp2_of(__builtin_fmaf(p[j][q][r], kLog2E, -lse2[q]));
+                        const float e = exp2_of(__builtin_fmaf(p[j][q][r] - top[q], kLog2E, -log_sum[q]));
                         p[j][q][r] = label[q] - at == (pair + j) * 16 + r ? hit[q] : e;
                     }
             }
@@ -541,11 +543,11 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads, TY::k
 // parts of the rays as fill the device. 921,600 rays x 256 labels of 8 channels: 126 us, vector instructions 80 % of the cycles; 131,072 x
 // 4096 of 64 channels in planes: 717 us, matrix instructions 58 %; 32768 x 32771 of 256 channels, bf16: 1408 us, 781 TFLOP/s, LDS reads 51 %.
 // ONE: the rays share one upstream gradient, which multiplies the sums at the end; else each ray's weights have its own.
-template <class TY, int NK, int QB, bool ONE> __global__ __launch_bounds__(kThreads) void k_label_dw(LabelArgs a) {
+template <class TY, int NK, int QB, bool ONE> __global__ __launch_bounds__(kThreads, NK * TY::kPlanes <= 12 ? 2 : 1) void k_label_dw(LabelArgs a) {
     typedef Shape<TY, NK> T;
     constexpr int NM = depth_blocks<TY, NK>();
     __shared__ alignas(16) char tile[T::kTile];
-    __shared__ alignas(16) float tile_lse2[2][T::kRows], tile_up[2][T::kRows], tile_hit[2][T::kRows];
+    __shared__ alignas(16) float tile_top[2][T::kRows], tile_log_sum[2][T::kRows], tile_up[2][T::kRows], tile_hit[2][T::kRows];
     __shared__ alignas(16) int tile_label[2][T::kRows];
     const int lane = threadIdx.x & 63, g = lane >> 4, wave = wave_number();
     const Turn turn = turn_of(a.cut);
@@ -555,28 +557,29 @@ template <class TY, int NK, int QB, bool ONE> __global__ __launch_bounds__(kThre
 
     Stage<TY, NK> stage;
     stage.begin(a.x, tile_base(a.x, first));
-    // Of every ray: lse (+inf where it is ignored or behind the end, which makes its weights 0), upstream gradient, label and its weight. They are a tile
+    // Of every ray: maximum and sum (+inf where it is ignored or behind the end, which makes its weights 0), upstream gradient, label and its weight. They are a tile
     // ahead of the channels, which are read only of rays that are not ignored: those of the others may hold anything.
-    float stage_lse2 = kInf, stage_up = 0.0f, stage_hit = 0.0f;
+    float stage_top = 0.0f, stage_log_sum = kInf, stage_up = 0.0f, stage_hit = 0.0f;
     int64_t stage_target = a.ignore;
     auto fetch_stats = [&](int64_t at) {   // (as they lie: what is made of them waits for them)
         const int64_t row = at + threadIdx.x;
-        stage_target = a.ignore, stage_lse2 = kInf;
+        stage_target = a.ignore, stage_top = 0.0f, stage_log_sum = kInf;
         if ((int)threadIdx.x < T::kRows && row < last) {
-            stage_target = a.target[row], stage_lse2 = a.lse2[row], stage_hit = a.hit[row];
+            stage_target = a.target[row], stage_top = a.top[row], stage_log_sum = a.log_sum[row], stage_hit = a.hit[row];
             if (!ONE) stage_up = a.upstream[row];
         }
     };
     auto store_stats = [&](int at) {
         if ((int)threadIdx.x >= T::kRows) return;
         const bool ignored = stage_target == a.ignore, none = !ignored && (stage_target < 0 || stage_target >= a.labels);
-        tile_lse2[at][threadIdx.x] = none ? __builtin_nanf("") : stage_lse2;
+        tile_top[at][threadIdx.x] = stage_top;
+        tile_log_sum[at][threadIdx.x] = none ? __builtin_nanf("") : stage_log_sum;
         tile_label[at][threadIdx.x] = ignored || none ? -1 : (int)stage_target;
         tile_hit[at][threadIdx.x] = stage_hit;
         if (!ONE) tile_up[at][threadIdx.x] = ignored ? 0.0f : stage_up;
     };
     auto fetch = [&](int64_t at, int half) {
-        stage.template load<true>((int)min(last - at, (int64_t)T::kRows), tile_lse2[half]);
+        stage.template load<true>((int)min(last - at, (int64_t)T::kRows), tile_log_sum[half]);
     };
     fetch_stats(first);
     Own<TY, NK, QB> own;
@@ -614,7 +617,7 @@ template <class TY, int NK, int QB, bool ONE> __global__ __launch_bounds__(kThre
                 for (int q = 0; q < QB; ++q) p[j][q] = f4{bias[q], bias[q], bias[q], bias[q]};
                 product<TY, NK, QB>(tile, pair + j, own, p[j]);
                 const int at4 = (pair + j) * 16 + 4 * g;
-                const f4 lse2 = *reinterpret_cast<const f4 *>(tile_lse2[half] + at4);
+                const f4 top = *reinterpret_cast<const f4 *>(tile_top[half] + at4), log_sum = *reinterpret_cast<const f4 *>(tile_log_sum[half] + at4);
                 const f4 up = ONE ? f4{} : *reinterpret_cast<const f4 *>(tile_up[half] + at4);
                 const f4 hit = *reinterpret_cast<const f4 *>(tile_hit[half] + at4);
                 const int4 label = *reinterpret_cast<const int4 *>(tile_label[half] + at4);
@@ -624,7 +627,7 @@ template <class TY, int NK, int QB, bool ONE> __global__ __launch_bounds__(kThre
                     const int v = row0 + q * 16 + (lane & 15);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        float e = exp2_of(__builtin_fmaf(p[j][q][r], kLog2E, -lse2[r]));
+                        float e = exp2_of(__builtin_fmaf(p[j][q][r] - top[r], kLog2E, -log_sum[r]));
                         e = labels[r] == v ? hit[r] : e;
                         if constexpr (!ONE) e *= up[r];
                         p[j][q][r] = e;
@@ -685,7 +688,8 @@ LabelArgs arguments(const DstLabelParams *p) {
     LabelArgs a = {};
     a.bias = p->bias, a.target = p->targets;
     a.rays = p->rays, a.ignore = p->ignore_index, a.d = p->channels, a.labels = p->labels;
-    a.lse2 = p->lse, a.hit = p->hit;
+    a.lse2 = p->lse;
+    if (p->stats) a.top = p->stats, a.log_sum = p->stats + p->rays, a.hit = p->stats + 2 * p->rays;
     return a;
 }
 
@@ -890,7 +894,7 @@ int dst_label_loss_backward(const DstLabelParams *p, void *stream) {
     if (p->reduction != DST_REDUCE_NONE && !p->inverse) return dst_op_fail(DST_E_INVALID, "a reduced loss needs inverse");
     if ((reinterpret_cast<uintptr_t>(p->grad_features) | reinterpret_cast<uintptr_t>(p->grad_weight)) & 15u)
         return dst_op_fail(DST_E_INVALID, "gradients must be aligned to 16 bytes");
-    if (p->rays > 0 && !p->hit) return dst_op_fail(DST_E_INVALID, "hit is required");
+    if (p->rays > 0 && !p->stats) return dst_op_fail(DST_E_INVALID, "stats are required");
     return with_gradients(p, [&](auto ty, auto nk) {
         typedef decltype(ty) TY;
         typedef typename TY::E E;

@@ -62,7 +62,7 @@ class DstLabelParams(C.Structure):
     _fields_ = [("rays", C.c_int64), ("channels", C.c_int32), ("labels", C.c_int32), ("dtype", C.c_int32),
                 ("reduction", C.c_int32), ("features", _FP), ("features_stride", C.c_int64), ("weight", _FP),
                 ("weight_stride", C.c_int64), ("bias", _FP), ("targets", _FP), ("ignore_index", C.c_int64), ("loss", _FP),
-                ("lse", _FP), ("hit", _FP), ("inverse", _FP), ("upstream", _FP), ("grad_features", _FP), ("grad_weight", _FP),
+                ("lse", _FP), ("stats", _FP), ("inverse", _FP), ("upstream", _FP), ("grad_features", _FP), ("grad_weight", _FP),
                 ("grad_bias", _FP), ("best", _FP), ("log_prob", _FP), ("workspace", _FP), ("workspace_bytes", C.c_uint64)]
 
 

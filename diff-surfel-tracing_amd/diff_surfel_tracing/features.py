@@ -104,8 +104,8 @@ def _run_labels(p, what, launch, like):
 
 
 def _set_stats(p, stats):
-    """What the forward pass leaves of every ray for the backward pass: `lse` and `hit`."""
-    p.lse, p.hit = stats.data_ptr(), stats.data_ptr() + 4 * int(stats.size(1))   # (a recorded trace gives sizes as tensors)
+    """What the forward pass leaves of every ray for the backward pass: `lse`, and the three values of `stats`."""
+    p.lse, p.stats = stats.data_ptr(), stats.data_ptr() + 4 * int(stats.size(1))   # (a recorded trace gives sizes as tensors)
 
 
 def _loss_forward(x, w, targets, bias, ignore_index, reduction):
@@ -114,7 +114,7 @@ def _loss_forward(x, w, targets, bias, ignore_index, reduction):
         p.reduction, p.targets, p.ignore_index = reduction, targets.data_ptr(), ignore_index
         f32 = dict(dtype=torch.float32, device=x.device)
         loss = torch.empty(x.size(0) if reduction == 0 else (), **f32)
-        stats = torch.empty(2, x.size(0), **f32)
+        stats = torch.empty(4, x.size(0), **f32)
         inverse = None if reduction == 0 else torch.empty((), **f32)
         p.loss, p.inverse = loss.data_ptr(), None if inverse is None else inverse.data_ptr()
         _set_stats(p, stats)
@@ -173,7 +173,7 @@ def label_loss(features, weight, targets, bias=None, *, ignore_index=-100, reduc
     gradient, whatever its channels hold.  Any other target outside 0..labels-1 makes the loss and the gradients it
     reaches NaN.  Returns float32: the mean over the rays not ignored (NaN, without gradients, if there are none), the sum, or with "none" a loss
     for every ray.  Differentiable (once) in features, weight and bias; sums in 32 bits or more in one order: the same bits every time.
-    Logits beyond 2.3e38 count as infinite."""
+    Logits beyond 32 bits count as infinite."""
     _check_labels(features, weight, bias)
     if reduction not in _REDUCTIONS:
         raise RuntimeError("reduction must be one of none, sum, mean (got %r)" % (reduction,))

@@ -330,9 +330,10 @@ typedef struct DstLabelParams {
     const int64_t *targets;       /* (rays) */
     int64_t ignore_index;
     float *loss;                  /* forward: (rays) for DST_REDUCE_NONE, else one value */
-    float *lse;                   /* (rays): forward writes, backward reads (log2 of the sum of exponentials; +inf: ignored) */
-    float *hit;                   /* (rays): forward writes (NULL: not wanted), backward reads (the weight of the ray's label less one, formed of the
-                                   * loss, so that it has the digits of what a label near weight 1 lacks; 0: ignored) */
+    float *lse;                   /* (rays): forward writes log2 of the sum of exponentials (+inf: ignored); both passes want it there */
+    float *stats;                 /* (3, rays): forward writes (NULL: not wanted), backward reads: the largest logit; log2 of the sum of exponentials
+                                   * relative to it (+inf: ignored); the weight of the ray's label less one, formed of the loss, so that it has the
+                                   * digits of what a label near weight 1 lacks */
     float *inverse;               /* one value, unless DST_REDUCE_NONE: forward writes, backward reads */
     const float *upstream;        /* backward: gradient of the loss, of its shape */
     void *grad_features;          /* backward: (rays, channels), written whole; NULL: not wanted */

@@ -30,7 +30,7 @@ def _label(**more):
     p = binding.DstLabelParams()
     p.rays, p.channels, p.labels, p.dtype, p.reduction = 1, 17, 1, F32, 0
     p.features, p.features_stride, p.weight, p.weight_stride = 4096, 256, 4096, 256
-    p.targets = p.lse = p.hit = p.loss = p.inverse = p.upstream = p.best = p.log_prob = 4096
+    p.targets = p.lse = p.stats = p.loss = p.inverse = p.upstream = p.best = p.log_prob = 4096
     p.grad_features = p.grad_weight = p.grad_bias = 4096
     for k, v in more.items():
         setattr(p, k, v)

@@ -109,7 +109,7 @@ def test_mean_of_sure_rays():
 
 
 def test_a_label_masked_by_the_lowest_value_as_target():
-    """Its loss is what its logit lacks, and its gradient that of a weight of 0; a ray that has none but such labels has no loss."""
+    """Its loss is what its logit lacks, and its gradient that of a weight of 0; a ray whose labels are all switched off has no loss."""
     import diff_surfel_tracing as dst
     low = torch.finfo(torch.float32).min
     for dtype in (torch.float32, torch.bfloat16):
@@ -123,8 +123,7 @@ def test_a_label_masked_by_the_lowest_value_as_target():
         assert torch.isfinite(dx).all()
         b[3] = float("-inf")
         assert (dst.label_loss(x, w, t, b, reduction="none") == float("inf")).all()
-        for value in (low, float("-inf")):
-            assert torch.isnan(dst.label_loss(x, w, t, torch.full((40,), value, device="cuda"), reduction="none")).all()
+        assert torch.isnan(dst.label_loss(x, w, t, torch.full((40,), float("-inf"), device="cuda"), reduction="none")).all()
 
 
 @pytest.mark.parametrize("N,V", [(70, 40), (3, 20000), (70000, 333)], ids=str)
