@@ -105,7 +105,8 @@ def _run_labels(p, what, launch, like):
 
 def _set_stats(p, stats):
     """What the forward pass leaves of every ray for the backward pass: `lse`, and the three values of `stats`."""
-    p.lse, p.stats = stats.data_ptr(), stats.data_ptr() + 4 * int(stats.size(1))   # (a recorded trace gives sizes as tensors)
+    at = stats.data_ptr()
+    p.lse, p.stats = at, at + 4 * p.rays
 
 
 def _loss_forward(x, w, targets, bias, ignore_index, reduction):
@@ -114,7 +115,7 @@ def _loss_forward(x, w, targets, bias, ignore_index, reduction):
         p.reduction, p.targets, p.ignore_index = reduction, targets.data_ptr(), ignore_index
         f32 = dict(dtype=torch.float32, device=x.device)
         loss = torch.empty(x.size(0) if reduction == 0 else (), **f32)
-        stats = torch.empty(4, x.size(0), **f32)
+        stats = torch.empty(4 * x.size(0), **f32)
         inverse = None if reduction == 0 else torch.empty((), **f32)
         p.loss, p.inverse = loss.data_ptr(), None if inverse is None else inverse.data_ptr()
         _set_stats(p, stats)
