@@ -105,9 +105,9 @@ template <class E> __device__ inline void store_out(const AttendArgs &a, int64_t
 constexpr float kSlack = 8.0f;
 
 // Bound by vector and matrix instructions together, which two waves on a SIMD overlap in part: 131,072 rows x 1024 in 4 heads of 64, bf16,
-// 175 us, 786 TFLOP/s, vector instructions 77 % of the cycles and matrix ones 40 %; 16384 x 8192 in 8 heads of 128, 645 us,
-// 852 TFLOP/s, 49 % and 42 %. One ray that asks a long memory is bound by reading it: 65,536 rows of 8 heads of 128, 45 us, 5.9 TB/s
-// (a large copy moves 4.7), in 64 parts a head, and 7 us to join them.
+// 185 us, 743 TFLOP/s, vector instructions 83 % of the cycles and matrix ones 38 %; 16384 x 8192 in 8 heads of 128, 656 us,
+// 838 TFLOP/s, 49 % and 42 %. One ray that asks a long memory is bound by reading it: 65,536 rows of 8 heads of 128, 46 us, 5.8 TB/s
+// (a kernel that only reads gets 5.95 out of 4 GiB), in 64 parts a head, and 7 us to join them.
 template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void k_attend_forward(AttendArgs a) {
     typedef Shape<TY, NK> T;
     typedef typename TY::E E;
@@ -324,8 +324,8 @@ __device__ inline void deltas(const Own<TY, NK, QB> &o, const Own<TY, NK, QB> &l
     }
 }
 
-// dq, and delta for the other kernel: queries as own rows, the memory streamed. 16384 x 8192 in 8 heads of 128, bf16: 774 us,
-// 1065 TFLOP/s, matrix instructions 53 % of the cycles.
+// dq, and delta for the other kernel: queries as own rows, the memory streamed. 16384 x 8192 in 8 heads of 128, bf16: 842 us,
+// 979 TFLOP/s, matrix instructions 49 % of the cycles.
 template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void k_attend_dq(AttendArgs a) {
     typedef Shape<TY, NK> T;
     typedef typename TY::E E;
@@ -412,7 +412,7 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void 
 }
 
 // dk and dv: the memory's rows as own rows, the queries streamed. Four products of a tile with one own block a wave (two would leave one
-// wave on a SIMD): 16384 x 8192 in 8 heads of 128, bf16: 1230 us, 894 TFLOP/s, LDS reads 61 % of the cycles.
+// wave on a SIMD): 16384 x 8192 in 8 heads of 128, bf16: 1271 us, 865 TFLOP/s, LDS reads 59 % of the cycles.
 template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads) void k_attend_dkv(AttendArgs a) {
     typedef Shape<TY, NK> T;
     typedef typename TY::E E;

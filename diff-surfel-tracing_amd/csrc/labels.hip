@@ -133,7 +133,7 @@ constexpr float kNormLost = 2e-18f;
 // bits), twice that between two. A ray without channels (norm 0)
 // has the biases themselves. Of the biases those count that can be the best label's: one more than 2 norms below the largest cannot, so a
 // label that is masked by the lowest value of its type does not bring every ray onto the list. (Full-HD rays, 8 channels, 151 labels, a third
-// of them so masked: 3767 us with all biases counted, 173 with these.)
+// of them so masked: 3767 us with all biases counted, 173 with these, when both were tried.)
 __device__ inline void finish_best(const LabelArgs &a, int64_t row, Running r, float best, int label, float second, float norm, float3 bound) {
     const float reach = norm * bound.x, tall = fminf(bound.y, __builtin_fabsf(bound.z) + 2.1f * reach);
     const float off = norm > 0.0f ? a.margin * (reach + tall) + 1e-35f : 0.0f;
@@ -165,10 +165,10 @@ __device__ inline void merge_best(float &best, int &label, float &second, float 
 
 // Rays as own rows, the table streamed. BEST: the best label instead of the loss.
 // A lane keeps the maximum and sum of its own quarter of the table (its group's rows of every block), so nothing is exchanged until the
-// end. Short rows are bound by the vector unit, not by the products: fused multiply-add, exponential, half a maximum and an
-// addition for a logit, and four instructions more for the best label (full-HD, 8 channels, 151 labels: 155 us, vector
-// instructions 83 % of the cycles). Long ones by vector and matrix instructions, 50 % and 47 % of the cycles, which overlap in part (32768 rays x
-// 32771 labels of 256 channels, bf16: 560 us, 981 TFLOP/s, of the 1119 that a large library product reaches).
+// end. Short rows are bound by the vector unit, not by the products: a difference, its scaling, an exponential, half a maximum and an
+// addition for a logit, and four instructions more for the best label (full-HD, 8 channels, 151 labels: 167 us, vector
+// instructions 88 % of the cycles). Long ones by vector and matrix instructions, 56 % and 46 % of the cycles, which overlap in part (32768 rays x
+// 32771 labels of 256 channels, bf16: 583 us, 943 TFLOP/s, of the 1119 to 1206 that a large library product reaches).
 template <class TY, int NK, int QB, bool BEST> __global__ __launch_bounds__(kThreads) void k_label_forward(LabelArgs a) {
     typedef Shape<TY, NK> T;
     __shared__ alignas(16) char tile[T::kTile > kThreads * 12 ? T::kTile : kThreads * 12];
@@ -457,8 +457,8 @@ template <class TY> __global__ __launch_bounds__(kThreads) void k_label_near(Lab
 }
 // ---- backward -------------------------------------------------------------------------------------------------------
 // dx: rays as own rows, the table streamed; the tile is read twice from LDS, by rows for the logits and turned for the sums.
-// 921,600 rays x 256 labels of 8 channels: 111 us, vector instructions 81 % of the cycles; 131,072 x 4096 of 64 channels
-// in planes: 602 us, matrix instructions 71 %; 32768 x 32771 of 256 channels, bf16: 1027 us, 1070 TFLOP/s, matrix instructions 49 %.
+// 921,600 rays x 256 labels of 8 channels: 125 us, vector instructions 88 % of the cycles; 131,072 x 4096 of 64 channels
+// in planes: 641 us, matrix instructions 68 %; 32768 x 32771 of 256 channels, bf16: 1044 us, 1053 TFLOP/s, matrix instructions 49 %.
 template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads, TY::kPlanes == 1 ? 2 : 1) void k_label_dx(LabelArgs a) {
     typedef Shape<TY, NK> T;
     constexpr int NM = depth_blocks<TY, NK>();
@@ -540,8 +540,9 @@ template <class TY, int NK, int QB> __global__ __launch_bounds__(kThreads, TY::k
 }
 
 // dw and db: labels as own rows, the rays streamed, with their lse, upstream gradient and label in LDS. Few labels are cut into as many
-// parts of the rays as fill the device. 921,600 rays x 256 labels of 8 channels: 126 us, vector instructions 80 % of the cycles; 131,072 x
-// 4096 of 64 channels in planes: 717 us, matrix instructions 58 %; 32768 x 32771 of 256 channels, bf16: 1408 us, 781 TFLOP/s, LDS reads 51 %.
+// parts of the rays as fill the device. 921,600 rays x 256 labels of 8 channels: 130 us, vector instructions 80 % of the cycles; 131,072 x
+// 4096 of 64 channels in planes: 742 us, matrix instructions 58 % (one wave on a SIMD, of four registers too many: 907); 32768 x 32771 of 256
+// channels, bf16: 1529 us, 719 TFLOP/s, LDS reads 52 %.
 // ONE: the rays share one upstream gradient, which multiplies the sums at the end; else each ray's weights have its own.
 template <class TY, int NK, int QB, bool ONE> __global__ __launch_bounds__(kThreads, NK * TY::kPlanes <= 12 ? 2 : 1) void k_label_dw(LabelArgs a) {
     typedef Shape<TY, NK> T;
